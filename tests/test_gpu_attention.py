@@ -1,0 +1,505 @@
+"""The attention operators (exl3_b200.attention) against plain 64-bit forms.
+
+Tolerances, with u = 2^-24 (half a step of f32) and e = half a step of the output's type:
+  qk_norm_rope  norm: sum of D squares, rsqrt and three products, at most 10 u; cosine and sine: reduced
+                angle below pi, 2 u, the function 2 u, the factor 1 u; product and fma 2 u.  Per element
+                20 u (|a| + |b|) factor over its pair, and e |result|.
+  cache         exact: codes and scales are defined by comparisons that floating point can decide.
+  attend        score error of at most 32 u A, A = scale max_k sum |q k| (sums of D products and the group
+                scales); it moves a weight by at most twice that; sums of a few thousand weights and
+                products 64 u.  (64 A + 64) u max|v|, and e |result|.
+  prompt        weights rounded to the 16-bit type, half a step of each: e_in W, W = sum p |v|, half as
+                much again for what the exponential and its argument are off; the score as above.
+                1.5 e_in W + (64 A + 64) u W, and e |result|.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+@pytest.fixture(scope="module")
+def A(cuda_lib):
+    from exl3_b200 import attention
+
+    return attention
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):  # half a step of the type's subnormals
+    return torch.finfo(t).tiny * torch.finfo(t).eps
+
+
+def gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def randn(g, *shape):
+    return torch.randn(shape, generator=g, device="cuda")
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def offsets(lens):
+    o = [0]
+    for n in lens:
+        o.append(o[-1] + n)
+    return ints(o)
+
+
+def close(got, want, tol, where=""):
+    got, want = got.double(), want.double()
+    same = (got == want) | (got.isnan() & want.isnan())
+    bad = ~(same | ((got - want).abs() <= tol))
+    assert not bool(bad.any()), (where, int(bad.sum()), float((got - want).abs()[bad].max()))
+
+
+# -- norm and rotary positions ----------------------------------------------------------------------
+
+def ref_rope(x, w, pos, inv_freq, eps, interleaved, factor):
+    """64-bit result and the sum |a| + |b| over each dimension's pair."""
+    y = x.double()
+    if w is not None:
+        y = y / (y.pow(2).mean(-1, keepdim=True) + eps).sqrt() * w.double()
+    r = 2 * len(inv_freq) if inv_freq is not None else 0
+    out, size = y.clone(), y.abs()
+    if r:
+        th = (pos.double()[:, None] * inv_freq.double())[:, None]
+        c, s = th.cos() * factor, th.sin() * factor
+        one = torch.arange(r // 2, device=x.device) * (2 if interleaved else 1)
+        two = one + (1 if interleaved else r // 2)
+        out[..., one] = y[..., one] * c - y[..., two] * s
+        out[..., two] = y[..., two] * c + y[..., one] * s
+        size[..., one] = size[..., two] = (y[..., one].abs() + y[..., two].abs()) * factor
+    return out, size
+
+
+def check_rope(got, x, w, pos, inv_freq, eps, interleaved, factor):
+    want, size = ref_rope(x, w, pos, inv_freq, eps, interleaved, factor)
+    close(got, want, 20 * U * size + half_step(got.dtype) * want.abs() + tiny(got.dtype))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,rotary,interleaved,rows,heads,kv", [
+    (128, 128, False, 1, 16, 4), (128, 64, True, 77, 16, 4), (128, 32, False, 5, 12, 4), (64, 64, True, 33, 8, 8),
+    (64, 16, False, 3, 10, 2), (128, 0, False, 9, 3, 1), (64, 64, False, 513, 1, 1)])
+def test_rope(A, dtype, dim, rotary, interleaved, rows, heads, kv):
+    g = gen(rows)
+    qkv = (randn(g, rows, heads + 2 * kv, dim) * 2).to(dtype)
+    q, k = qkv[:, :heads], qkv[:, heads:heads + kv]  # strided rows of one projection
+    qw, kw = 1 + 0.1 * randn(g, dim), 1 + 0.1 * randn(g, dim)
+    pos = torch.randint(0, 2_000_000, (rows,), generator=g, device="cuda").to(torch.int32)
+    freq, factor = None, 1.0
+    if rotary:
+        f, factor = A.rope_frequencies(rotary, 1e6, 8.0 if rotary > 16 else 1.0, 32768)
+        freq = torch.from_numpy(f).cuda()
+    qo, ko = A.qk_norm_rope(q, k, pos, freq, qw, kw, eps=1e-6, interleaved=interleaved, attention_factor=factor)
+    assert qo.dtype == ko.dtype == dtype
+    check_rope(qo, q, qw, pos, freq, 1e-6, interleaved, factor)
+    check_rope(ko, k, kw, pos, freq, 1e-6, interleaved, factor)
+
+
+def test_rope_without_weights_in_place_and_mixed_types(A):
+    g = gen(3)
+    q, k = randn(g, 21, 6, 128), randn(g, 21, 2, 128)
+    pos = ints([-1 if i % 5 == 4 else i * 1000 for i in range(21)])
+    live = pos >= 0
+    freq = torch.from_numpy(A.rope_frequencies(64)[0]).cuda()
+    q16 = torch.full((21, 6, 128), 7.0, dtype=torch.float16, device="cuda")
+    q0, k0 = q.clone(), k.clone()
+    _, ko = A.qk_norm_rope(q, k, pos, freq, None, None, q_out=q16, k_out=k)
+    assert ko is k
+    check_rope(q16[live], q0[live], None, pos[live], freq, 0, False, 1.0)
+    check_rope(k[live], k0[live], None, pos[live], freq, 0, False, 1.0)
+    assert bool((q16[~live] == 7).all()) and torch.equal(k[~live], k0[~live])  # rows without a position: as they were
+    only, none = A.qk_norm_rope(q0, None, pos.clamp(min=0), freq, k0[0, 0].contiguous(), out_dtype=torch.bfloat16)
+    assert none is None
+    check_rope(only, q0, k0[0, 0], pos.clamp(min=0), freq, 1e-6, False, 1.0)
+    empty, _ = A.qk_norm_rope(q[:0], k[:0], pos[:0], freq)
+    assert empty.shape == (0, 6, 128)
+
+
+def test_rope_rows_of_zeros_and_not_finite(A):
+    q = torch.zeros((3, 2, 64), device="cuda")
+    q[1, 0, 5], q[2, 1, 7] = math.inf, math.nan
+    w = torch.ones(64, device="cuda")
+    out, _ = A.qk_norm_rope(q, None, ints([0, 1, 2]), torch.from_numpy(A.rope_frequencies(64)[0]).cuda(), w)
+    assert bool((out[0] == 0).all()) and bool((out[1, 1] == 0).all()) and bool((out[2, 0] == 0).all())
+    assert bool(out[1, 0, 5].isnan()) and bool(out[2, 1].isnan().all())
+
+
+# -- the cache ------------------------------------------------------------------------------------------
+
+def ref_quantise(x):
+    """(code - 8 per dimension, scale per group [.., G] as f64) of rows [.., D], from the definition."""
+    x = x.double()
+    G = x.shape[-1] // 32
+    xg = x.unflatten(-1, (32, G))
+    top = xg.abs().amax(-2)
+    s = (top.clamp(max=7 * 65504) / 7).half()
+    s = torch.where((s.double() * 7 < top) & (s < 65504), (s.view(torch.int16) + 1).view(torch.float16), s)
+    s = torch.where(top.isfinite(), s.double(), torch.nan)
+    code = torch.where(s.unsqueeze(-2) > 0, torch.round(xg / s.unsqueeze(-2)), 0.0).clamp(-7, 7)
+    return code.flatten(-2), s
+
+
+def values(code, s):
+    return (code.unflatten(-1, (32, s.shape[-1])) * s.unsqueeze(-2)).flatten(-2)
+
+
+def stored(codes, scales):
+    """(code - 8 [.., D], scale [.., G]) of a cache's memory."""
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).double() - 8
+    return c, scales.double()
+
+
+def fill(cache, g, garbage=True):
+    """Random codes and scales everywhere; with garbage, some scales not finite (set only where no test looks)."""
+    for codes, scales in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)):
+        codes.copy_(torch.randint(0, 256, codes.shape, generator=g, device="cuda", dtype=torch.uint8))
+        scales.copy_(torch.rand(scales.shape, generator=g, device="cuda") * 0.2 + 0.01)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,kv,rows", [(128, 4, 37), (64, 3, 130), (128, 1, 1)])
+def test_append_then_read(A, dtype, dim, kv, rows):
+    g = gen(dim + rows)
+    cache = A.Kv4Cache(3, kv, 150, dim)
+    assert cache.max_len == 192
+    fill(cache, g)
+    before = [t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    kvs = (randn(g, rows, 2 * kv, dim) * torch.logspace(-4, 3, rows, device="cuda")[:, None, None]).to(dtype)
+    k, v = kvs[:, :kv], kvs[:, kv:]
+    seq_slot = ints([2, 0])
+    n0 = rows // 3
+    lens = [n0, rows - n0]
+    row_seq = ints([0] * n0 + [1] * (rows - n0))
+    pos = list(range(n0)) + list(range(rows - n0))
+    cache.append(k, v, row_seq, ints(pos), seq_slot)
+    touched = torch.zeros((3, 192), dtype=torch.bool, device="cuda")
+    touched[2, :n0] = touched[0, :rows - n0] = True
+    at = (seq_slot.long()[row_seq.long()], slice(None), torch.tensor(pos, device="cuda"))
+    for x, codes, scales, c0, s0 in ((k, cache.k_codes, cache.k_scales, *before[:2]),
+                                     (v, cache.v_codes, cache.v_scales, *before[2:])):
+        want_c, want_s = ref_quantise(x)
+        got_c, got_s = stored(codes[at], scales[at])
+        assert torch.equal(got_s, want_s) and torch.equal(got_c, want_c)
+        keep = ~touched[:, None, :].expand(3, kv, 192)
+        assert torch.equal(codes[keep], c0[keep]) and torch.equal(scales[keep], s0[keep])
+    for out_type in TYPES:
+        ko, vo = cache.read(seq_slot, offsets(lens), rows, dtype=out_type)
+        assert torch.equal(ko, values(*ref_quantise(k)).to(out_type))
+        assert torch.equal(vo, values(*ref_quantise(v)).to(out_type))
+
+
+def test_append_edges(A):
+    """Ties, saturated, zero, subnormal and not finite groups; rows that are skipped."""
+    cache = A.Kv4Cache(1, 1, 64, 64)
+    x = torch.zeros((8, 1, 64), device="cuda")
+    x[0, 0, 0::2] = torch.tensor([3.5, 7, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5] * 4, device="cuda") * 0.25  # s = 0.25
+    x[0, 0, 1::2] = torch.nextafter(x[0, 0, 0::2], torch.tensor(-1e9, device="cuda"))
+    x[1, 0, 3], x[1, 0, 0] = 1e30, 458528.0
+    x[2, 0, 4], x[2, 0, 5] = math.nan, 3.0
+    x[3, 0, 6], x[3, 0, 7] = -math.inf, -3.0
+    x[4, 0, 0], x[4, 0, 1] = 1e-42, 3e-7
+    x[5, 0] = 1.0
+    seq = ints([0, 0, 0, 0, 0, 0, 1, -1])
+    pos = ints([0, 1, 2, 3, 63, 64, 5, 6])  # row 5: past the end; rows 6 and 7: no such sequence
+    before = cache.k_codes.clone()
+    cache.append(x, x, seq, pos, ints([0]))
+    want_c, want_s = ref_quantise(x)
+    for i, p in ((0, 0), (1, 1), (2, 2), (3, 3), (4, 63)):
+        c, s = stored(cache.k_codes[0, 0, p], cache.k_scales[0, 0, p])
+        assert torch.equal(s.nan_to_num(-1), want_s[i, 0].nan_to_num(-1)), i
+        assert torch.equal(torch.where(s.isnan().repeat(32), 0.0, c), torch.where(s.isnan().repeat(32), 0.0, want_c[i, 0])), i
+    assert torch.equal(cache.k_codes[0, 0, 4:63], before[0, 0, 4:63])
+    k, _ = cache.read(ints([0]), ints([0, 4]), 4, dtype=torch.float32)
+    assert bool(k[2, 0, 0::2].isnan().all()) and bool((k[2, 0, 1::2] == values(want_c, want_s)[2, 0, 1::2]).all())
+    assert float(k[1, 0, 3]) == 7 * 65504.0
+
+
+def test_read_rows_outside_the_cache(A):
+    g = gen(5)
+    cache = A.Kv4Cache(2, 2, 64, 128)
+    fill(cache, g)
+    k = torch.full((140, 2, 128), 5.0, device="cuda")
+    v = k.clone()
+    # sequence 0: 66 positions of a slot of 64; 1: empty; 2: no such slot; 3: three rows; the rest: left alone
+    cache.read(ints([1, 0, 2, 0]), ints([0, 66, 66, 68, 71]), 140, k_out=k, v_out=v)
+    c, s = stored(cache.k_codes, cache.k_scales)
+    want = values(c, s).transpose(1, 2)
+    assert torch.equal(k[:64], want[1].float()) and torch.equal(k[68:71], want[0, :3].float())
+    assert bool((k[64:68] == 0).all()) and bool((v[64:68] == 0).all())
+    assert bool((k[71:] == 5).all()) and bool((v[71:] == 5).all())
+
+
+# -- attention ------------------------------------------------------------------------------------------
+
+def ref_attention(q, k, v, first, scale):
+    """One head in 64 bits: query i of q [n, D] sees keys 0 .. first + i.  (out, A, W, max |v|)."""
+    n, m = len(q), len(k)
+    q, k, v = q.double(), k.double(), v.double()
+    seen = torch.arange(m, device=q.device) <= first + torch.arange(n, device=q.device)[:, None]
+    s = torch.where(seen, q @ k.t() * scale, -torch.inf)
+    size = torch.where(seen, q.abs() @ k.abs().t() * scale, 0.0)
+    p = torch.where(seen.any(-1, keepdim=True), torch.softmax(s, -1), 0.0)
+    a = size.amax(-1, keepdim=True) if m else torch.zeros(n, 1, device=q.device, dtype=torch.float64)
+    return p @ v, a, p @ v.abs(), (v.abs().max() if m else torch.zeros((), device=q.device))
+
+
+def check_attend(got, q, cache, slots, lens, scale=None):
+    rows, heads, dim = q.shape
+    scale = dim ** -0.5 if scale is None else scale
+    share = heads // cache.kv_heads
+    kv, vv = (values(*stored(c, s)) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+    for r, (slot, n) in enumerate(zip(slots, lens)):
+        for h in range(heads):
+            want, a, _, top = ref_attention(q[r, h:h + 1], kv[slot, h // share, :n], vv[slot, h // share, :n], n, scale)
+            tol = (64 * a + 64) * U * top + half_step(got.dtype) * want.abs() + tiny(got.dtype)
+            close(got[r, h:h + 1], want, tol, (r, h, n))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,lens", [
+    (16, 4, 128, [1]), (16, 4, 128, [767]), (16, 4, 128, [1, 2, 63, 64, 65, 1000, 2049, 31]), (32, 4, 64, [5, 300, 128]),
+    (8, 8, 128, [129, 15]), (12, 4, 128, [70, 200]), (10, 2, 64, [257]), (1, 1, 64, [3, 1]), (64, 2, 128, [100, 17])])
+def test_attend(A, dtype, heads, kv, dim, lens):
+    g = gen(heads + len(lens))
+    n = len(lens)
+    cache = A.Kv4Cache(n + 1, kv, max(lens) + 7, dim)
+    fill(cache, g)
+    slots = [(i * 5 + 1) % (n + 1) if (n + 1) % 5 else n - i for i in range(n)]
+    for i, m in zip(slots, lens):  # what lies past the last visible position must not matter
+        for s in (cache.k_scales, cache.v_scales):
+            s[i, :, m:] = math.nan
+            s[i, :, m + 1::2] = math.inf
+    qkv = (randn(g, n, heads + 2, dim) * 1.5).to(dtype)
+    q = qkv[:, :heads]
+    got = cache.attend(q, ints(list(range(n))), ints([m - 1 for m in lens]), ints(slots))
+    clean = A.Kv4Cache.from_tensors(cache.k_codes, cache.k_scales.nan_to_num(0, 0, 0), cache.v_codes,
+                                    cache.v_scales.nan_to_num(0, 0, 0))
+    check_attend(got, q, clean, slots, lens)
+
+
+def test_attend_long_and_many_rows(A):
+    """A context long enough to be split many ways, and more rows than the GPU has places."""
+    g = gen(11)
+    cache = A.Kv4Cache(2, 2, 20000, 128)
+    fill(cache, g)
+    q = randn(g, 1, 8, 128)
+    check_attend(cache.attend(q, ints([0]), ints([19990]), ints([1])), q, cache, [1], [19991])
+    lens = [int(x) for x in torch.randint(1, 400, (150,), generator=g, device="cuda")]
+    q = randn(g, 150, 8, 128).half()
+    got = cache.attend(q, ints([i % 2 for i in range(150)]), ints([m - 1 for m in lens]), ints([1, 0]))
+    check_attend(got, q, cache, [1 - i % 2 for i in range(150)], lens)
+
+
+def test_attend_rows_that_see_nothing(A):
+    g = gen(6)
+    cache = A.Kv4Cache(2, 4, 128, 128)
+    fill(cache, g)
+    q = randn(g, 6, 16, 128)
+    out = torch.full((6, 16, 128), 9.0, device="cuda")
+    # row 0: no position; 1: ordinary; 2: no such slot; 3 and 4: no such sequence; 5: past the end, the whole slot
+    cache.attend(q, ints([0, 1, 2, -1, 3, 1]), ints([-1, 40, 3, 3, 3, 1000]), ints([0, 1, 7]), out=out)
+    assert bool((out[0] == 0).all()) and bool((out[2] == 0).all())
+    assert bool((out[3] == 9).all()) and bool((out[4] == 9).all())
+    check_attend(out[[1, 5]], q[[1, 5]], cache, [1, 1], [41, 128])
+
+
+def test_attend_extreme_values(A):
+    """Scores of hundreds, scales from the smallest to the largest half, queries of any size."""
+    g = gen(8)
+    cache = A.Kv4Cache(1, 2, 128, 128)
+    fill(cache, g)
+    cache.k_scales.mul_(8)
+    q = randn(g, 3, 8, 128) * torch.tensor([20.0, 1e-6, 1e-30], device="cuda")[:, None, None]
+    check_attend(cache.attend(q, ints([0, 0, 0]), ints([99, 99, 99]), ints([0])), q, cache, [0] * 3, [100] * 3)
+    cache.v_scales.copy_(torch.logspace(-7, 4.5, 128, device="cuda")[None, None, :, None].expand_as(cache.v_scales))
+    cache.k_scales.copy_(torch.rand(cache.k_scales.shape, generator=g, device="cuda") * 0.1)
+    q = randn(g, 1, 8, 128)
+    for n in (1, 10, 40, 128):  # early positions: the smallest values
+        check_attend(cache.attend(q, ints([0]), ints([n - 1]), ints([0])), q, cache, [0], [n])
+    cache.v_scales.copy_(cache.v_scales.flip(2))
+    for n in (1, 40, 128):
+        check_attend(cache.attend(q, ints([0]), ints([n - 1]), ints([0])), q, cache, [0], [n])
+    cache.k_scales[0, 0, 3] = math.nan  # a visible NaN reaches its own head group and no other
+    out = cache.attend(q, ints([0]), ints([9]), ints([0]))
+    assert bool(out[0, :4].isnan().all()) and bool(out[0, 4:].isfinite().all())
+    q[0, 5, 0] = math.nan
+    out = cache.attend(q, ints([0]), ints([2]), ints([0]))
+    assert bool(out[0, 5].isnan().all()) and bool(out[0, :5].isfinite().all()) and bool(out[0, 6:].isfinite().all())
+
+
+def ref_prompt(q, k, v, q_lens, kv_spans, scale):
+    outs, tols = [], []
+    heads, share = q.shape[1], q.shape[1] // k.shape[1]
+    e_in, at = half_step(q.dtype), 0
+    for n, (b, e) in zip(q_lens, kv_spans):
+        for h in range(heads):
+            want, a, w, _ = ref_attention(q[at:at + n, h], k[b:e, h // share], v[b:e, h // share], e - b - n, scale)
+            outs.append(want)
+            tols.append(1.5 * e_in * w + (64 * a + 64) * U * w)
+        at += n
+    def pack(parts):
+        return torch.cat([torch.stack(parts[i * heads:(i + 1) * heads], 1) for i in range(len(q_lens))])
+    return pack(outs), pack(tols)
+
+
+def check_prompt(got, q, k, v, q_lens, kv_spans, scale=None):
+    want, tol = ref_prompt(q, k, v, q_lens, kv_spans, q.shape[2] ** -0.5 if scale is None else scale)
+    close(got[:len(want)], want, tol + half_step(got.dtype) * want.abs() + tiny(q.dtype) * 8, q_lens)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("heads,kv,dim,q_lens,past", [
+    (16, 4, 128, [1], 0), (16, 4, 128, [37], 0), (16, 4, 128, [128, 1, 0, 65, 200], 0), (16, 4, 128, [512, 1, 64], 300),
+    (32, 4, 64, [130, 7], 0), (8, 8, 128, [257, 128], 0), (8, 8, 64, [300], 77), (12, 4, 128, [100, 31], 5),
+    (10, 2, 64, [66], 129), (1, 1, 128, [700], 0), (64, 2, 128, [50], 0), (6, 2, 128, [129], 1000), (7, 1, 64, [40], 0)])
+def test_prompt(A, dtype, heads, kv, dim, q_lens, past):
+    g = gen(heads + dim + len(q_lens))
+    rows, kv_lens = sum(q_lens), [n + past if n else 0 for n in q_lens]
+    q = (randn(g, rows, heads, dim) * 1.5).to(dtype)
+    k, v = (randn(g, sum(kv_lens), kv, dim).to(dtype) for _ in range(2))
+    ko = offsets(kv_lens).tolist()
+    got = A.prompt_attention(q, k, v, offsets(q_lens), ints(ko))
+    check_prompt(got, q, k, v, q_lens, list(zip(ko, ko[1:])))
+    got = A.prompt_attention(q, k, v, offsets(q_lens), ints(ko), out=torch.empty_like(q, dtype=torch.float32), scale=0.05)
+    check_prompt(got, q, k, v, q_lens, list(zip(ko, ko[1:])), 0.05)
+
+
+def test_prompt_rows_that_see_nothing_and_rows_behind(A):
+    """More queries than keys, no keys at all, and rows behind the last sequence."""
+    g = gen(9)
+    q = randn(g, 300, 8, 128).half()
+    k, v = randn(g, 90, 2, 128).half(), randn(g, 90, 2, 128).half()
+    out = torch.full((300, 8, 128), 3.0, device="cuda").half()
+    q_lens, spans = [140, 10, 70], [(0, 5), (5, 5), (5, 90)]
+    A.prompt_attention(q, k, v, offsets(q_lens), kv_begin=ints([0, 5, 5]), kv_end=ints([5, 5, 90]), out=out)
+    check_prompt(out, q, k, v, q_lens, spans)
+    assert bool((out[:135] == 0).all()) and bool((out[140:150] == 0).all()) and bool((out[220:] == 3).all())
+    none = A.prompt_attention(q, k[:0], v[:0], ints([0, 300]), ints([0, 0]))
+    assert bool((none == 0).all())
+
+
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_prompt_not_finite_where_masked(A, value):
+    """Keys and values that a query does not see never reach it; what it sees does."""
+    g = gen(10)
+    n = 200
+    q = randn(g, n, 4, 128).half()
+    k, v = randn(g, n + 100, 1, 128).half(), randn(g, n + 100, 1, 128).half()
+    clean = A.prompt_attention(q, k, v, ints([0, n]), ints([0, n]))
+    k2, v2 = k.clone(), v.clone()
+    k2[n:], v2[n:] = value, value                   # behind the sequence
+    v2[150, 0, 7] = value                           # one channel of a later value
+    k2[170] = math.nan                              # a later key
+    got = A.prompt_attention(q, k2, v2, ints([0, n]), ints([0, n]))
+    assert torch.equal(got[:150], clean[:150])
+    keep = [d for d in range(128) if d != 7]
+    assert torch.equal(got[150:170][..., keep], clean[150:170][..., keep])
+    seven = got[150:170, :, 7]
+    assert bool(seven.isnan().all()) if math.isnan(value) else bool((seven == value).all())
+    assert bool(got[170:].isnan().all())
+
+
+def test_prompt_in_a_slot_cache_and_strided(A):
+    """Keys in fp16 slots [slots][kv][max_len][D], queries as columns of a packed projection."""
+    g = gen(12)
+    slots, kv, max_len, dim, heads = 3, 4, 160, 128, 16
+    kc, vc = randn(g, slots, kv, max_len, dim).half(), randn(g, slots, kv, max_len, dim).half()
+    rows = slots * kv * max_len - (kv - 1) * max_len
+    kview, vview = (t.as_strided((rows, kv, dim), (dim, max_len * dim, 1)) for t in (kc, vc))
+    q_lens, lens, order = [70, 1, 30], [150, 97, 30], [2, 0, 1]
+    proj = randn(g, 101, heads + 2 * kv, dim).half()
+    q = proj[:, :heads]
+    begin = [s * kv * max_len for s in order]
+    out = torch.zeros((101, heads + 1, dim), device="cuda")[:, :heads]
+    A.prompt_attention(q, kview, vview, offsets(q_lens), kv_begin=ints(begin),
+                       kv_end=ints([b + n for b, n in zip(begin, lens)]), out=out)
+    check_prompt(out, q, kview, vview, q_lens, [(b, b + n) for b, n in zip(begin, lens)])
+
+
+def test_layer_in_4_bits(A):
+    """The operators together, as a layer runs them: a ragged prefill step through norm, cache, read and
+    prompt attention, then captured decode steps through norm, cache and attend, replayed at later
+    positions.  Both forms are held to 64-bit attention over what the cache holds."""
+    g = gen(13)
+    heads, kv, dim, max_len = 16, 4, 128, 256
+    cache = A.Kv4Cache(4, kv, max_len, dim)
+    freq = torch.from_numpy(A.rope_frequencies(dim, 1e7)[0]).cuda()
+    qw, kw = 1 + 0.1 * randn(g, dim), 1 + 0.1 * randn(g, dim)
+    lens, slots = [100, 1, 63], [3, 0, 2]
+    total = sum(lens)
+    seq_slot, kv_offs = ints(slots), offsets(lens)
+    row_seq = ints([s for s, n in enumerate(lens) for _ in range(n)])
+    row_pos = ints([i for n in lens for i in range(n)])
+    qkv = randn(g, total, heads + 2 * kv, dim)
+    q16 = torch.empty((total, heads, dim), dtype=torch.float16, device="cuda")
+    q16, k32 = A.qk_norm_rope(qkv[:, :heads], qkv[:, heads:heads + kv], row_pos, freq, qw, kw, q_out=q16)
+    cache.append(k32, qkv[:, heads + kv:], row_seq, row_pos, seq_slot)
+    k, v = cache.read(seq_slot, kv_offs, total)
+    out = A.prompt_attention(q16, k, v, kv_offs, kv_offs)
+    o = kv_offs.tolist()
+    check_prompt(out, q16, k, v, lens, list(zip(o, o[1:])))
+
+    one, new = ints([0, 1, 2]), torch.empty((3, heads + 2 * kv, dim), device="cuda")
+    pos = ints(lens)
+    result = torch.empty((3, heads, dim), device="cuda")
+    qs = torch.empty((3, heads, dim), device="cuda")
+
+    def step():
+        _, kr = A.qk_norm_rope(new[:, :heads], new[:, heads:heads + kv], pos, freq, qw, kw, q_out=qs)
+        cache.append(kr, new[:, heads + kv:], one, pos, seq_slot)
+        cache.attend(qs, one, pos, seq_slot, out=result)
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    new.copy_(randn(g, 3, heads + 2 * kv, dim))
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for t in range(3):
+        new.copy_(randn(g, 3, heads + 2 * kv, dim))
+        pos.copy_(ints([n + t for n in lens]))
+        graph.replay()
+        check_attend(result, qs, cache, slots, [n + t + 1 for n in lens])
+
+
+def test_calls_on_two_streams_at_once(A):
+    """Calls that overlap on two streams, given as arguments, leave each other's results alone."""
+    g = gen(14)
+    cache = A.Kv4Cache(2, 4, 4096, 128)
+    fill(cache, g)
+    q = [randn(g, 2, 16, 128) for _ in range(2)]
+    seqs, slots = ints([0, 1]), ints([0, 1])
+    pos = [ints([4000, 77]), ints([3, 2500])]
+    want = [cache.attend(q[i], seqs, pos[i], slots) for i in range(2)]
+    qp, kp = randn(g, 600, 4, 128).half(), randn(g, 600, 2, 128).half()
+    offs = ints([0, 200, 600])
+    want_p = A.prompt_attention(qp, kp, kp, offs, offs)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            got[i].append((cache.attend(q[i], seqs, pos[i], slots, stream=s),
+                           A.prompt_attention(qp, kp, kp, offs, offs, stream=s)))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for a, p in got[i]:
+            assert torch.equal(a, want[i]) and torch.equal(p, want_p)

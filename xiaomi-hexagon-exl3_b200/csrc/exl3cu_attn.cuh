@@ -1,0 +1,95 @@
+// Shared by the attention operators (exl3cu_attn.cu, exl3cu_attn_prompt.cu): element types, the 4-bit
+// code and scale of a cached value, and the launch helper.
+#pragma once
+#include "exl3cu.h"
+#include "exl3cu_attn.h"
+#include "exl3cu_internal.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace exl3cu {
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// exl3cu_kv4_cache without head_dim (a template argument of the kernels).
+struct Kv4 {
+    uint8_t * k_codes;
+    uint16_t * k_scales;
+    uint8_t * v_codes;
+    uint16_t * v_scales;
+    int n_slots, kv_heads, max_len;
+};
+
+// The scale of a group from the bits of its largest |x| (compared as integers, so that a NaN is the
+// largest): the smallest half with 7 * scale >= |x|.  Rounding up twice, the quotient to float and that to
+// half, is the half above the exact quotient, since every half is a float.
+__device__ __forceinline__ __half kv4_scale(uint32_t most_bits) {
+    if (most_bits >= 0x7f800000u) return __ushort_as_half(0x7fff);  // an infinity or a NaN in the group
+    const float s = __fdiv_ru(__uint_as_float(most_bits), 7.0f);
+    return s > 65504.0f ? __ushort_as_half(0x7bff) : __float2half_ru(s);
+}
+
+// 8 + x / s rounded to the nearest integer, ties to even, from -7 to 7.  The approximate quotient is at
+// most one step off; x - t s is exact (t s has 15 bits at most, and t s and x are within a factor of
+// two of one another where t is not zero), and so is its comparison with s / 2.
+__device__ __forceinline__ uint32_t kv4_code(float x, float s) {
+    if (!(s > 0.f)) return 8u;  // a group of zeros, or a NaN scale
+    float t = rintf(__fdividef(x, s));
+    t = fminf(fmaxf(t, -8.f), 8.f);  // saturated groups
+    const float d = fmaf(-t, s, x), h = 0.5f * s;
+    const bool odd = (int(t) & 1) != 0;
+    if (d > h || (d == h && odd)) t += 1.f;
+    else if (d < -h || (d == -h && odd)) t -= 1.f;
+    return uint32_t(int(fminf(fmaxf(t, -7.f), 7.f)) + 8);
+}
+
+// The segment s of [offsets[s], offsets[s + 1]) that holds row r, or -1.  Offsets ascend; empty segments hold
+// nothing.
+__device__ __forceinline__ int find_segment(const int32_t * offsets, int n, int r) {
+    if (r < offsets[0] || r >= offsets[n]) return -1;
+    int lo = 0, hi = n;  // offsets[lo] <= r < offsets[hi]
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (offsets[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Calls f with a value of the element type that `dtype` names.
+template <typename F>
+int with_type(int dtype, F && f) {
+    if (dtype == EXL3CU_F32) return f(float{});
+    if (dtype == EXL3CU_F16) return f(__half{});
+    return f(__nv_bfloat16{});
+}
+
+// Launch with programmatic stream serialization (the kernels wait for their predecessor with
+// griddepcontrol.wait before touching memory).
+template <typename... KArgs, typename... Args>
+int attn_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void * stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+    if (e == cudaSuccess) return EXL3CU_OK;
+    (void)cudaGetLastError();
+    return api_cuda_fail(e, "attention operator");
+}
+
+}  // namespace exl3cu

@@ -25,4 +25,9 @@ def __getattr__(name):
 
         mod = importlib.import_module(".model", __name__)
         return mod if name == "model" else mod.Exl3Model
+    if name in ("attention", "Kv4Cache"):
+        import importlib
+
+        mod = importlib.import_module(".attention", __name__)
+        return mod if name == "attention" else mod.Kv4Cache
     raise AttributeError(name)
