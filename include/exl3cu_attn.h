@@ -103,7 +103,7 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
  * (kv_begin = slot * kv_heads * max_len); kv_rows is the number of rows that every
  * head can address.  A key or value that a query does not see never reaches its
  * result, whatever it holds.  Packed K/V: kv_begin = offsets, kv_end = offsets + 1.
- * dtype (q, k, v): EXL3CU_F16 or EXL3CU_BF16; out_dtype: the same or EXL3CU_F32.
+ * dtype (q, k, v): EXL3CU_F16 or EXL3CU_BF16; scale > 0; out_dtype: the same or EXL3CU_F32.
  * Query rows outside every sequence are left as they were; q_rows is the rows
  * that d_q and d_out hold. */
 int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void * d_k, size_t k_row_stride, size_t k_head_stride,

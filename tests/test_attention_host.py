@@ -97,7 +97,7 @@ PROMPT = dict(q=P, qs=2048, k=P, krs=512, khs=128, v=P, vrs=512, vhs=128, kv_row
 
 
 @pytest.mark.parametrize("kw", [
-    dict(dtype=0), dict(dtype=3), dict(ot=4), dict(dim=80), dict(heads=15), dict(kv=0), dict(heads=2048, qs=1 << 20),
+    dict(dtype=0), dict(dtype=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(ot=4), dict(dim=80), dict(heads=15), dict(kv=0), dict(heads=2048, qs=1 << 20),
     dict(n=-1), dict(rows=-1), dict(kv_rows=-1), dict(q=None), dict(q=P + 2), dict(qs=2044), dict(qs=1024), dict(k=None),
     dict(krs=100), dict(krs=132), dict(khs=64), dict(vhs=129), dict(v=P + 8), dict(qo=None), dict(b=None), dict(e=None),
     dict(out=None), dict(os=2040), dict(krs=1 << 40)])

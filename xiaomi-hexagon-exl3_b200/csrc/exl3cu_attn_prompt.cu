@@ -1,76 +1,586 @@
-// Causal attention of packed sequences with grouped heads (exl3cu_prompt_attn; contract in exl3cu_attn.h).
+// Causal attention of packed sequences with grouped heads on the 5th-generation tensor cores
+// (exl3cu_prompt_attn; contract in exl3cu_attn.h).
+//
+// out = softmax(scale Q K^T) V per query head, one pass over the keys in tiles of 128 with a running
+// maximum and sum per query row.  4 D flops a visible (query, key) pair and head: bound by the tensor cores
+// and, at the same rate at D = 128, by the exponentials (16 a clock and SM).
+//
+// One CTA serves one sequence's block of query rows for a group of P heads that share a K/V head (P: the largest
+// power of two, at most 16, that divides heads / kv_heads): two tiles of 128 rows, row = position * P + head, so
+// that the heads of a group share the K/V tiles and a causal block wastes at most one tile of keys.  The
+// blocks of a sequence are launched longest first.
+//
+// Per tile of keys:  S = Q K^T (tcgen05, operands in shared memory by TMA, 128-byte swizzle), S in TMEM;
+// a thread owns a row of S: maximum, P = exp2(scale log2e (S - m)), row sum in f32, P rounded to the 16-bit
+// type (half a step each, as the library of any such kernel does: the product needs 16-bit operands) and
+// stored over S in TMEM;  O += P V with P from TMEM, V from shared memory as it lies (MN-major), O in TMEM.  The
+// maximum that the weights refer to follows the true one only when it has grown by more than 2^8, so O is
+// rescaled rarely; weights stay at or below 256.
+//
+// Warps: 0-3 and 4-7 the rows of the two tiles; 8 loads; 9 issues the products and owns TMEM.  While one
+// tile's rows work on their exponentials, the other tile's products run.
+//
+// Values that a row does not see must not reach it even if they are not finite (0 * NaN is NaN in a product).
+// Scores are replaced where masked.  For values the load warp reads the tiles of V in which some row's view
+// ends, sets elements that are not finite to zero and notes per dimension the first key that held a NaN, +inf
+// or -inf; the rows that see that key get it back at the end.
+//
+// Every wait is bounded; a wait that runs out sets a status bit, and the CTA ends without its result.
 #include "exl3cu.h"
 #include "exl3cu_async.cuh"
 #include "exl3cu_attn.cuh"
 #include "exl3cu_attn.h"
 #include "exl3cu_internal.h"
 
+#include <cuda.h>
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 namespace exl3cu {
+
+static __device__ unsigned g_prompt_status;
 
 namespace {
 
+constexpr int kTile = 128;      // keys per tile, rows per query tile
+constexpr int kThreads = 384;   // 8 warps of rows, load warp, product warp, two idle
+// Registers a thread: a row's 128 scores need more than the 168 that 384 threads can have alike.  The last four
+// warps give theirs up to the rows' eight: 8 * 216 + 4 * 72 = 12 * 168.
+constexpr int kRegs = 168, kRegsRows = 216, kRegsRest = 72;
+static_assert(8 * kRegsRows + 4 * kRegsRest <= 12 * kRegs, "more registers than the launch has would wait forever");
+constexpr int kBlockBytes = kTile * 128;  // 64 dimensions of 128 rows
+constexpr uint32_t kNever = 0x7fffffffu;
+// Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
+// at most three tiles.
+constexpr int kMasked = 3;
+
+template <int D> struct Shape {
+    static constexpr int kBlocks = D / 64;                     // 64-dimension blocks of a row
+    static constexpr int kTileBytes = kBlocks * kBlockBytes;
+    static constexpr int kSlots = D == 128 ? 5 : 8;            // ring of K and V tiles
+    static constexpr int kSmem = 2 * kTileBytes + kSlots * kTileBytes + 2048 + 1024;
+};
+static_assert(Shape<128>::kSmem <= 232448 && 2 * Shape<64>::kSmem > 232448, "one CTA per SM: it holds all of TMEM");
+
 struct PromptArgs {
-    const void * q;
-    const void * k;
-    const void * v;
     void * out;
-    long long q_stride, k_row, k_head, v_row, v_head, out_stride;
+    long long out_stride;
     const int32_t * q_offsets;
     const int32_t * kv_begin;
     const int32_t * kv_end;
-    int n_seq, q_rows, kv_rows, heads, kv_heads, out_dtype;
-    float scale;
+    int n_seq, q_rows, kv_rows, heads, kv_heads, out_f32;
+    int log_p;        // heads per group P = 1 << log_p
+    float scale_log2; // scale * log2(e)
 };
 
-// One warp per (query row, head), one pass over the visible keys: lane holds dimensions [lane * D/32, +D/32).
+__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
+    return uint64_t((saddr >> 4) & 0x3fffu) | uint64_t((lbo >> 4) & 0x3fffu) << 16 | uint64_t((sbo >> 4) & 0x3fffu) << 32 |
+           uint64_t(1) << 46 |  // descriptor version for sm_100
+           uint64_t(2) << 61;   // 128-byte swizzle
+}
+
+__device__ __forceinline__ void commit(uint64_t * bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// D = A B (+ D): both operands in shared memory / A in TMEM.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        : "memory");
+}
+
+// 32 consecutive TMEM columns of this thread's lane (wait_ld() before use).
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t * r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t * r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+// A box of the map at (x, y, z) into shared memory; x is a multiple of 64 elements.
+__device__ __forceinline__ void tma_load(void * dst, const CUtensorMap * map, int x, int y, int z, uint64_t * bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(smem_addr(dst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_addr(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t y;
+    if constexpr (std::is_same_v<T, __half>) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+
+struct Bars {
+    uint64_t full[8], empty[8], q_full, clean[kMasked], s_full[2], p_full[2], o_done[2];
+    uint32_t tmem, dirty;
+    int seq, q0, q1, k0, k1, p0;  // the CTA's work; q1 <= q0: none
+};
+
+// Elements of a 16-bit pair whose exponent is all ones, as a mask of the pair.
+template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+    return ((w & e) == e ? 0xffffu : 0u) | ((w >> 16 & e) == e ? 0xffff0000u : 0u);
+}
+
+// Clears what is not finite in keys [first, 128) of the V tile at `tile` (whose keys start at `base`); first
+// keys that held a NaN, +inf or -inf go to seen[0 .. 2][dimension], keys from `keys` on are only cleared.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) k_prompt_attn(const PromptArgs a) {
-    pdl_trigger();
-    pdl_wait_primary();
-    constexpr int E = D / 32;
+__device__ __noinline__ void clean_values(unsigned char * tile, int first, int base, int keys, uint32_t * seen,
+                                          uint32_t * dirty) {
     const int lane = threadIdx.x & 31;
-    const long long item = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (item >= (long long)a.q_rows * a.heads) return;
-    const int r = int(item / a.heads), h = int(item % a.heads);
-    const int s = find_segment(a.q_offsets, a.n_seq, r);
-    if (s < 0) return;
-    const int k0 = max(a.kv_begin[s], 0), k1 = min(a.kv_end[s], a.kv_rows);
-    const int n = k1 - k0 - (a.q_offsets[s + 1] - 1 - r);  // visible keys
-    const int kvh = h / (a.heads / a.kv_heads);
-    const T * q = static_cast<const T *>(a.q) + r * a.q_stride + h * D + lane * E;
-    const T * k = static_cast<const T *>(a.k) + k0 * a.k_row + kvh * a.k_head + lane * E;
-    const T * v = static_cast<const T *>(a.v) + k0 * a.v_row + kvh * a.v_head + lane * E;
-    float qv[E], acc[E];
+    constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
+    constexpr uint32_t e2 = e | e << 16, one = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+    // 8 lanes to a 128-byte row of a block, 4 rows at a time
+    for (int b = 0; b < D / 64; ++b)
+#pragma unroll 8
+        for (int r = (first & ~3) + (lane >> 3); r < kTile; r += 4) {
+            uint4 * at = reinterpret_cast<uint4 *>(tile + b * kBlockBytes + r * 128 + (lane & 7) * 16);
+            const uint4 w = *at;
+            // an exponent of all ones carries into the sign's place
+            const uint32_t any = (((w.x & e2) + one) | ((w.y & e2) + one) | ((w.z & e2) + one) | ((w.w & e2) + one)) & 0x80008000u;
+            if (any && r >= first) {
+                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+                uint32_t o[4];
+                const int d0 = b * 64 + (((lane & 7) ^ (r & 7)) << 3);  // the swizzle: 16-byte chunk ^ (row mod 8)
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t mask = not_finite<T>(v[i]);
+                    o[i] = v[i] & ~mask;
+                    for (int h = 0; h < 2; ++h)
+                        if ((mask >> 16 * h & 1u) && base + r < keys) {
+                            const uint32_t x = v[i] >> 16 * h & 0xffffu;
+                            const int kind = (x & 0x7fffu) != e ? 0 : x & 0x8000u ? 2 : 1;
+                            atomicMin(seen + kind * D + d0 + 2 * i + h, uint32_t(base + r));
+                            *dirty = 1u;
+                        }
+                }
+                *at = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the products read them
+    __syncwarp();
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v) {
+    using Sh = Shape<D>;
+    extern __shared__ unsigned char raw[];
+    unsigned char * smem = raw + ((1024u - (smem_addr(raw) & 1023u)) & 1023u);
+    unsigned char * sq = smem;                          // two query tiles
+    unsigned char * ring = smem + 2 * Sh::kTileBytes;
+    uint32_t * seen = reinterpret_cast<uint32_t *>(ring + Sh::kSlots * Sh::kTileBytes);  // [3][D]
+    Bars & bars = *reinterpret_cast<Bars *>(seen + 3 * 128);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+
+    const int groups = a.heads >> a.log_p;
+    const int hg = int(blockIdx.x) % groups, blk = int(blockIdx.x) / groups;
+    const int head0 = hg << a.log_p, kvh = head0 / (a.heads / a.kv_heads);
+    const int ppt = kTile >> a.log_p;  // positions per tile
+
+    if (warp == 8) {
+        if (lane == 0) {
+            for (int i = 0; i < Sh::kSlots; ++i) {
+                mbar_init(&bars.full[i], 1);
+                mbar_init(&bars.empty[i], 1);
+            }
+            mbar_init(&bars.q_full, 1);
+            for (int i = 0; i < kMasked; ++i) mbar_init(&bars.clean[i], 1);
+            for (int t = 0; t < 2; ++t) {
+                mbar_init(&bars.s_full[t], 1);
+                mbar_init(&bars.p_full[t], 4);  // the tile's warps
+                mbar_init(&bars.o_done[t], 1);
+            }
+            bars.dirty = 0;
+            mbar_init_fence();
+        }
+    } else if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars.tmem)),
+                     "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else if (warp == 0) {
+        // which sequence and block: blocks of all sequences in order, counted from the end so that a
+        // sequence's longest block starts first
+        pdl_wait_primary();
+        int total = 0;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+            const int s = s0 + lane;
+            const int n = s < a.n_seq ? min(a.q_offsets[s + 1], a.q_rows) - max(a.q_offsets[s], 0) : 0;
+            total += __reduce_add_sync(0xffffffffu, unsigned(n > 0 ? (n + 2 * ppt - 1) / (2 * ppt) : 0));
+        }
+        int want = total - 1 - blk, seq = -1, before = 0;
+        for (int s0 = 0; want >= 0 && s0 < a.n_seq; s0 += 32) {
+            const int s = s0 + lane;
+            const int n = s < a.n_seq ? min(a.q_offsets[s + 1], a.q_rows) - max(a.q_offsets[s], 0) : 0;
+            const int mine = n > 0 ? (n + 2 * ppt - 1) / (2 * ppt) : 0;
+            int upto = mine;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        qv[i] = to_f32(q[i]);
-        acc[i] = 0.f;
+            for (int x = 1; x < 32; x <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, upto, x);
+                if (lane >= x) upto += o;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, want < upto);
+            if (hit) {
+                const int src = __ffs(hit) - 1;
+                before = want - __shfl_sync(0xffffffffu, upto - mine, src);
+                seq = s0 + src;
+                break;
+            }
+            want -= __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (lane == 0) {
+            bars.seq = seq;
+            if (seq >= 0) {
+                bars.q0 = max(a.q_offsets[seq], 0);
+                bars.q1 = min(a.q_offsets[seq + 1], a.q_rows);
+                bars.k0 = min(max(a.kv_begin[seq], 0), a.kv_rows);
+                bars.k1 = max(min(a.kv_end[seq], a.kv_rows), bars.k0);
+                bars.p0 = before * 2 * ppt;
+            }
+        }
     }
-    float m = -INFINITY, l = 0.f;
-    for (int p = 0; p < n; ++p) {
-        float sc = 0.f;
+    for (int i = threadIdx.x; i < 3 * D; i += kThreads) seen[i] = kNever;
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = bars.tmem;
+    const bool work = bars.seq >= 0;
+    const int q0 = bars.q0, k0 = bars.k0, keys = bars.k1 - bars.k0, nq = bars.q1 - bars.q0, p0 = bars.p0;
+    // keys that position p of the sequence sees, and the tiles of each query tile
+    const auto sees = [&](int p) { return p < nq ? max(0, min(keys, p + 1 + keys - nq)) : 0; };
+    const auto tiles_of = [&](int t) {
+        const int first = p0 + t * ppt;
+        return !work || first >= nq ? 0 : (sees(min(first + ppt, nq) - 1) + kTile - 1) / kTile;
+    };
+    const int nt[2] = {tiles_of(0), tiles_of(1)};
+    const int n = max(nt[0], nt[1]);
+    const int all_see = work ? sees(p0) : 0;  // keys that every row of the CTA sees
+    const int masked0 = all_see / kTile;      // first tile of keys in which some row's view ends
+
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    if (warp == 8) {
+        // ---- loads, and the cleaning of V where views end ----
+        pdl_wait_primary();
+        if (n > 0) {
+            if (lane == 0) {
+                mbar_arrive_expect_tx(&bars.q_full, uint32_t(2 * Sh::kTileBytes));
+                for (int t = 0; t < 2; ++t)
+                    for (int b = 0; b < Sh::kBlocks; ++b)
+                        tma_load(sq + t * Sh::kTileBytes + b * kBlockBytes, &map_q, b * 64, head0, q0 + p0 + t * ppt,
+                                 &bars.q_full);
+            }
+            bool ok = true;
+            int it = 0;
+            for (int j = 0; j <= n && ok; ++j) {
+                if (j < n) {
+                    for (int w = 0; w < 2 && ok; ++w, ++it) {
+                        const int slot = it % Sh::kSlots;
+                        if (it >= Sh::kSlots) ok = mbar_wait_sleep(&bars.empty[slot], unsigned(it / Sh::kSlots - 1) & 1u);
+                        if (ok && lane == 0) {
+                            mbar_arrive_expect_tx(&bars.full[slot], uint32_t(Sh::kTileBytes));
+                            for (int b = 0; b < Sh::kBlocks; ++b)
+                                tma_load(ring + slot * Sh::kTileBytes + b * kBlockBytes, w ? &map_v : &map_k, b * 64,
+                                         kvh, k0 + j * kTile, &bars.full[slot]);
+                        }
+                        ok = __all_sync(0xffffffffu, ok);
+                    }
+                }
+                // one tile behind the loads, so that the next tile's are under way
+                if (ok && j > 0 && j - 1 >= masked0) {
+                    const int vi = 2 * (j - 1) + 1, slot = vi % Sh::kSlots;
+                    ok = __all_sync(0xffffffffu, mbar_wait_sleep(&bars.full[slot], unsigned(vi / Sh::kSlots) & 1u));
+                    if (ok) {
+                        clean_values<T, D>(ring + slot * Sh::kTileBytes, max(0, all_see - (j - 1) * kTile), (j - 1) * kTile,
+                                           keys, seen, &bars.dirty);
+                        if (lane == 0) mbar_arrive(&bars.clean[j - 1 - masked0]);
+                    }
+                }
+            }
+            if (!ok) {
+                if (lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
+                for (int i = max(0, it - Sh::kSlots); i < it; ++i)  // copies in flight end before the CTA does
+                    (void)mbar_wait_sleep(&bars.full[i % Sh::kSlots], unsigned(i / Sh::kSlots) & 1u);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 9) {
+        // ---- products (one thread) ----
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
+            constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | 8u << 24;  // f32 sums, M = 128
+            constexpr uint32_t idesc_s = common | uint32_t(kTile >> 3) << 17;
+            constexpr uint32_t idesc_o = common | uint32_t(D >> 3) << 17 | 1u << 16;  // V: MN-major
+            const uint64_t desc_q = smem_desc(smem_addr(sq), 16, 1024);
+            const uint64_t desc_k = smem_desc(smem_addr(ring), 16, 1024);
+            const uint64_t desc_v = smem_desc(smem_addr(ring), kBlockBytes, 1024);
+            constexpr uint64_t tile16 = Sh::kTileBytes >> 4;
+            const auto product_s = [&](int t, int slot) {
 #pragma unroll
-        for (int i = 0; i < E; ++i) sc = fmaf(qv[i], to_f32(k[p * a.k_row + i]), sc);
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint64_t at = uint64_t((kk / 4) * kBlockBytes + (kk % 4) * 32) >> 4;
+                    mma_ss(tmem + t * 128, desc_q + t * tile16 + at, desc_k + slot * tile16 + at, idesc_s, kk > 0);
+                }
+            };
+            const auto product_o = [&](int t, int slot, bool add) {
 #pragma unroll
-        for (int x = 16; x; x >>= 1) sc += __shfl_xor_sync(0xffffffffu, sc, x);
-        sc *= a.scale;
-        const float mn = fmaxf(m, sc);
-        const float corr = m == -INFINITY ? 1.f : expf(m - mn), e = sc == -INFINITY ? 0.f : expf(sc - mn);
-        l = l * corr + e;
-#pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] = fmaf(e, to_f32(v[p * a.v_row + i]), acc[i] * corr);
-        m = mn;
+                for (int kk = 0; kk < kTile / 16; ++kk)
+                    mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_v + slot * tile16 + kk * (2048 >> 4), idesc_o,
+                           add || kk > 0);
+            };
+            bool ok = mbar_wait(&bars.q_full, 0) && mbar_wait(&bars.full[0], 0);
+            if (ok) {
+                for (int t = 0; t < 2; ++t)
+                    if (nt[t] > 0) {
+                        product_s(t, 0);
+                        commit(&bars.s_full[t]);
+                    }
+            }
+            // a slot is handed back only where a later load waits for it: no arrival outlives the CTA
+            const auto hand_back = [&](int item) {
+                if (item + Sh::kSlots < 2 * n) commit(&bars.empty[item % Sh::kSlots]);
+            };
+            if (ok) hand_back(0);
+            for (int j = 0; j < n && ok; ++j) {
+                const int vi = 2 * j + 1, ki = 2 * j + 2;
+                const int vs = vi % Sh::kSlots, ks = ki % Sh::kSlots;
+                ok = mbar_wait(&bars.full[vs], unsigned(vi / Sh::kSlots) & 1u);
+                if (ok && j >= masked0) ok = mbar_wait(&bars.clean[j - masked0], 0);
+                if (ok && j + 1 < n) ok = mbar_wait(&bars.full[ks], unsigned(ki / Sh::kSlots) & 1u);
+                for (int t = 0; t < 2 && ok; ++t) {
+                    if (j < nt[t]) {
+                        ok = mbar_wait(&bars.p_full[t], unsigned(j) & 1u);
+                        if (!ok) break;
+                        fence_after();
+                        product_o(t, vs, j > 0);
+                        if (j + 1 == nt[t]) commit(&bars.o_done[t]);
+                    }
+                    if (t == 1 || nt[1] <= j) hand_back(vi);
+                    if (j + 1 < nt[t]) {
+                        product_s(t, ks);
+                        commit(&bars.s_full[t]);
+                    }
+                    if (t == 0 && nt[1] <= j) break;  // the second tile has no more
+                }
+                if (ok && j + 1 < n) hand_back(ki);
+            }
+            if (!ok) atomicOr(&g_prompt_status, kStatusWaitTimeout);
+        }
+        __syncwarp();
     }
-    const long long at = r * a.out_stride + h * D + lane * E;
+    } else {
+        // ---- rows: thread = row of tile t ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRows));
+        const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
+        const int p = p0 + t * ppt + (row >> a.log_p), head = head0 + (row & ((1 << a.log_p) - 1));
+        const int lim = work ? sees(p) : 0;
+        const int tile_sees = work ? sees(p0 + t * ppt) : 0;
+        const float c = a.scale_log2;
+        float m = -INFINITY, sum = 0.f;
+        const int tiles = nt[t];
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&bars.s_full[t], unsigned(j) & 1u));
+            if (!ok) break;
+            fence_after();
+            uint32_t s[kTile];
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const float o = n > 0 ? acc[i] / l : 0.f;
-        if (a.out_dtype == EXL3CU_F32) static_cast<float *>(a.out)[at + i] = o;
-        else static_cast<T *>(a.out)[at + i] = from_f32<T>(o);
+            for (int i = 0; i < 4; ++i) tmem_ld(ts + 32 * i, s + 32 * i);
+            wait_ld();
+            if ((j + 1) * kTile > tile_sees) {
+                const int left = lim - j * kTile;
+#pragma unroll
+                for (int i = 0; i < kTile; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+            }
+            float mx = m;
+#pragma unroll
+            for (int i = 0; i < kTile; i += 2) mx = max3(mx, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            // m: what the weights refer to.  It moves with the first tile, and when the true maximum is more
+            // than 2^8 above; then the sums so far are scaled down.  (mx - m is NaN where both are -inf.)
+            if (__any_sync(0xffffffffu, (mx - m) * c > 8.f)) {
+                const float f = mx == m ? 1.f : exp2_fast((m - mx) * c);
+                m = mx;
+                sum *= f;
+                if (j > 0) {  // every product up to the tile before is complete: S of this tile came after them
+                    for (int i = 0; i < D; i += 32) {
+                        uint32_t o[32];
+                        tmem_ld(to + i, o);
+                        wait_ld();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                        tmem_st(to + i, o);
+                    }
+                }
+            }
+            const float mc = m == -INFINITY ? 0.f : m * c;  // a row that has seen nothing: all weights are 0
+            float add0 = 0.f, add1 = 0.f;
+#pragma unroll
+            for (int i = 0; i < kTile; i += 2) {
+                const float e0 = exp2_fast(fmaf(__uint_as_float(s[i]), c, -mc));
+                const float e1 = exp2_fast(fmaf(__uint_as_float(s[i + 1]), c, -mc));
+                add0 += e0;
+                add1 += e1;
+                s[i / 2] = pack2<T>(e0, e1);
+            }
+            sum += add0 + add1;
+            tmem_st(ts, s);
+            tmem_st(ts + 32, s + 32);
+            wait_st();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.p_full[t]);
+        }
+        if (ok && tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[t], 0));
+        if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
+        fence_after();
+        const bool live = work && ok && p < nq;
+        const float inv = lim > 0 ? 1.f / sum : 0.f;
+        const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
+        const long long at = live ? (long long)(q0 + p) * a.out_stride + head * D : 0;
+#pragma unroll 1
+        for (int i = 0; i < D; i += 32) {
+            uint32_t o[32];
+            if (tiles > 0 && ok) {
+                tmem_ld(to + i, o);
+                wait_ld();
+            }
+            if (!live) continue;
+            float v[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) v[x] = lim > 0 ? __uint_as_float(o[x]) * inv : 0.f;
+            if (dirty) {
+#pragma unroll
+                for (int x = 0; x < 32; ++x) {
+                    if (seen[D + i + x] < uint32_t(lim)) v[x] += INFINITY;
+                    if (seen[2 * D + i + x] < uint32_t(lim)) v[x] -= INFINITY;
+                    if (seen[i + x] < uint32_t(lim)) v[x] = NAN;
+                }
+            }
+            if (a.out_f32) {
+                float4 * dst = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at + i);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) dst[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+            } else {
+                uint4 * dst = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + at + i);
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    dst[x] = make_uint4(pack2<T>(v[8 * x], v[8 * x + 1]), pack2<T>(v[8 * x + 2], v[8 * x + 3]),
+                                        pack2<T>(v[8 * x + 4], v[8 * x + 5]), pack2<T>(v[8 * x + 6], v[8 * x + 7]));
+            }
+        }
     }
+    fence_before();
+    __syncthreads();
+    if (warp == 9)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void * p = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            p = nullptr;
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return fn;
+}
+
+// Rows of `heads` heads of D 16-bit values; boxes of 64 values x box_heads x box_rows.
+bool encode(CUtensorMap * map, const void * p, bool bf16, int D, size_t heads, size_t rows, size_t head_stride,
+            size_t row_stride, unsigned box_heads, unsigned box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {cuuint64_t(D), heads, rows};
+    const cuuint64_t strides[2] = {head_stride * 2, row_stride * 2};
+    const cuuint32_t box[3] = {64, box_heads, box_rows}, steps[3] = {1, 1, 1};
+    return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(p), dims,
+              strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+std::atomic<unsigned long long> g_attr[4];
+
+template <typename T, int D>
+int launch(const PromptArgs & a, const CUtensorMap (&maps)[3], unsigned blocks, void * stream) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return api_cuda_fail(cudaGetLastError(), "prompt_attn");
+    auto & done = g_attr[(std::is_same_v<T, __half> ? 0 : 2) + (D == 128)];
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(done.load() & bit)) {
+        const cudaError_t e =
+            cudaFuncSetAttribute(k_prompt_attn<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<D>::kSmem);
+        if (e != cudaSuccess) return api_cuda_fail(e, "prompt_attn: shared memory");
+        cudaFuncAttributes f;
+        if (cudaFuncGetAttributes(&f, k_prompt_attn<T, D>) != cudaSuccess || f.numRegs != kRegs)
+            return api_fail(EXL3CU_NO_SUPPORT, "prompt_attn: built with another number of registers than it divides up");
+        done.fetch_or(bit);
+    }
+    return attn_launch(k_prompt_attn<T, D>, dim3(blocks), dim3(kThreads), size_t(Shape<D>::kSmem), stream, a, maps[0],
+                       maps[1], maps[2]);
 }
 
 }  // namespace
+
+cudaError_t prompt_read_status(unsigned * out, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(out, g_prompt_status, sizeof(unsigned));
+    if (e == cudaSuccess && clear && *out) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(g_prompt_status, &zero, sizeof(unsigned));
+    }
+    return e;
+}
 
 }  // namespace exl3cu
 
@@ -89,6 +599,7 @@ extern "C" int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void 
     if (heads <= 0 || kv_heads <= 0 || heads % kv_heads || heads > 1024)
         return bad("prompt_attn: heads must be a multiple of kv_heads, at most 1024");
     if (n_seq < 0 || q_rows < 0 || kv_rows < 0) return bad("prompt_attn: negative count");
+    if (!(scale > 0.f) || scale > 1e30f) return bad("prompt_attn: scale must be positive and finite");
     if (!n_seq || !q_rows) return EXL3CU_OK;
     constexpr size_t kMaxStride = size_t(1) << 36;  // 2^37 bytes: below the tensor map's limit
     const auto aligned = [](const void * p) { return p && reinterpret_cast<uintptr_t>(p) % 16 == 0; };
@@ -102,15 +613,28 @@ extern "C" int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void 
                     !stride_ok(v_head_stride, head_dim, 8)))
         return bad("prompt_attn: k or v null or misaligned, or a stride below head_dim or no multiple of 8");
     if (!d_q_offsets || !d_kv_begin || !d_kv_end) return bad("prompt_attn: offsets are NULL");
-    const PromptArgs a{d_q, d_k, d_v, d_out, (long long)q_stride, (long long)k_row_stride, (long long)k_head_stride,
-                       (long long)v_row_stride, (long long)v_head_stride, (long long)out_stride, d_q_offsets, d_kv_begin,
-                       d_kv_end, n_seq, q_rows, kv_rows, heads, kv_heads, out_dtype, scale};
-    const long long items = (long long)q_rows * heads;
-    if (items > (1ll << 32)) return bad("prompt_attn: too many query rows");
-    const dim3 grid(unsigned((items + 3) / 4)), block(128);
-    if (dtype == EXL3CU_F16)
-        return attn_launch(head_dim == 128 ? k_prompt_attn<__half, 128> : k_prompt_attn<__half, 64>, grid, block, 0,
-                           stream, a);
-    return attn_launch(head_dim == 128 ? k_prompt_attn<__nv_bfloat16, 128> : k_prompt_attn<__nv_bfloat16, 64>, grid,
-                       block, 0, stream, a);
+
+    int log_p = 0;  // heads per CTA: the power of two in heads / kv_heads, at most 16
+    while (log_p < 4 && (heads / kv_heads) % (2 << log_p) == 0) ++log_p;
+    const int positions = 2 * kTile >> log_p;
+    // blocks of all sequences: at most one part block per sequence more than the rows fill
+    const long long blocks = ((long long)q_rows / positions + n_seq) * (heads >> log_p);
+    if (blocks > 0x7fffffffll) return bad("prompt_attn: too many query rows");
+    const bool bf16 = dtype == EXL3CU_BF16;
+    CUtensorMap maps[3];
+    const bool any = kv_rows > 0;  // without keys the maps of k and v are never used
+    if (!encode(&maps[0], d_q, bf16, head_dim, size_t(heads), size_t(q_rows), size_t(head_dim), q_stride, 1u << log_p,
+                unsigned(kTile >> log_p)) ||
+        !encode(&maps[1], any ? d_k : d_q, bf16, head_dim, any ? size_t(kv_heads) : 1, any ? size_t(kv_rows) : 1,
+                any ? k_head_stride : head_dim, any ? k_row_stride : head_dim, 1, kTile) ||
+        !encode(&maps[2], any ? d_v : d_q, bf16, head_dim, any ? size_t(kv_heads) : 1, any ? size_t(kv_rows) : 1,
+                any ? v_head_stride : head_dim, any ? v_row_stride : head_dim, 1, kTile))
+        return api_fail(EXL3CU_CUDA_ERROR, "prompt_attn: cuTensorMapEncodeTiled failed");
+    const PromptArgs a{d_out, (long long)out_stride, d_q_offsets, d_kv_begin, d_kv_end, n_seq, q_rows, kv_rows, heads,
+                       kv_heads, out_dtype == EXL3CU_F32, log_p, scale * 1.4426950408889634f};
+    if (!bf16)
+        return head_dim == 128 ? launch<__half, 128>(a, maps, unsigned(blocks), stream)
+                               : launch<__half, 64>(a, maps, unsigned(blocks), stream);
+    return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, maps, unsigned(blocks), stream)
+                           : launch<__nv_bfloat16, 64>(a, maps, unsigned(blocks), stream);
 }
