@@ -81,7 +81,8 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
 
 /* Attention of single rows over the cache: query head h of row r attends to
  * positions 0 .. min(row_pos[r], max_len - 1) of its slot, K/V head
- * h / (heads / kv_heads); out = softmax(scale * q . k) v.  A row of a negative
+ * h / (heads / kv_heads); out = softmax(scale * q . k) v, scale > 0, at most
+ * 65535 rows.  A row of a negative
  * position, or of a slot outside the cache, becomes zero (nothing is visible); a
  * row whose sequence is outside [0, n_seq) is left as it was.  What the cache
  * holds past the last visible position never reaches a result.  d_scratch:

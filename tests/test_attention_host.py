@@ -85,7 +85,7 @@ ATTN = dict(q=P, qs=2048, dtype=0, rows=1, heads=16, seq=P, pos=P, slot=P, n_seq
 
 @pytest.mark.parametrize("kw", [
     dict(q=None), dict(q=P + 4), dict(qs=2047), dict(dtype=3), dict(rows=-1), dict(rows=70000), dict(heads=18),
-    dict(heads=0), dict(heads=2048), dict(seq=None), dict(pos=None), dict(slot=None), dict(n_seq=-1), dict(out=None),
+    dict(heads=0), dict(heads=2048), dict(scale=0.0), dict(scale=math.inf), dict(scratch=None), dict(scratch=P + 4), dict(bytes=1000), dict(seq=None), dict(pos=None), dict(slot=None), dict(n_seq=-1), dict(out=None),
     dict(os=1024)])
 def test_bad_attend_arguments_are_refused(L, kw):
     assert L.exl3cu_kv4_attn(cache(), *{**ATTN, **kw}.values()) == INVALID

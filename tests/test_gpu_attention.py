@@ -7,7 +7,11 @@ Tolerances, with u = 2^-24 (half a step of f32) and e = half a step of the outpu
   cache         exact: codes and scales are defined by comparisons that floating point can decide.
   attend        score error of at most 32 u A, A = scale max_k sum |q k| (sums of D products and the group
                 scales); it moves a weight by at most twice that; sums of a few thousand weights and
-                products 64 u.  (64 A + 64) u max|v|, and e |result|.
+                products 64 u.  (64 A + 64) u max|v|, and e |result|.  Rows of a 16-bit type have each weight
+                times its value scale rounded to a half: result = sum_k w_k (c_k - 8) with w_k off by at most
+                2^-11 w_k (the offset is taken off the rounded weights), which sums to at most 2^-11 W,
+                W = sum p |v|, and 2^-25 of the largest scale where w_k is below the normal halves (the
+                largest scale seen is at 2^13 there, far above).
   prompt        weights rounded to the 16-bit type, half a step of each: e_in W, W = sum p |v|, half as
                 much again for what the exponential and its argument are off; the score as above.
                 1.5 e_in W + (64 A + 64) u W, and e |result|.
@@ -264,8 +268,10 @@ def check_attend(got, q, cache, slots, lens, scale=None):
     kv, vv = (values(*stored(c, s)) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
     for r, (slot, n) in enumerate(zip(slots, lens)):
         for h in range(heads):
-            want, a, _, top = ref_attention(q[r, h:h + 1], kv[slot, h // share, :n], vv[slot, h // share, :n], n, scale)
+            want, a, w, top = ref_attention(q[r, h:h + 1], kv[slot, h // share, :n], vv[slot, h // share, :n], n, scale)
             tol = (64 * a + 64) * U * top + half_step(got.dtype) * want.abs() + tiny(got.dtype)
+            if got.dtype != torch.float32:
+                tol = tol + 2.0 ** -11 * w
             close(got[r, h:h + 1], want, tol, (r, h, n))
 
 

@@ -11,7 +11,13 @@
 #include "exl3cu_attn.h"
 #include "exl3cu_internal.h"
 
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
 namespace exl3cu {
+
+static __device__ unsigned g_attn_status;
 
 namespace {
 
@@ -186,75 +192,674 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 }
 
 // ---- attention of single rows over the cache ------------------------------------------------------
+//
+// One pass over the keys of a row in tiles of 64, on the matrix instructions, with the running maximum and sum
+// of a softmax.  Bound by the bytes of the cache (2 (D/2 + D/16) a key and K/V head) as long as a code costs about
+// one instruction; so codes are never multiplied out:
+//
+//   A code c of 4 bits becomes the half 1 + c/16 by a shift and one logic operation on two codes at a time: the
+//   bits go to the top of the mantissa of 1.0.  (c - 8) s = 16 s ((1 + c/16) - 1.5), and the 1.5 comes off sums:
+//   off the scores as the initial accumulator -1.5 sum q, off the result as -1.5 sum of the weights.
+//   Scales stay out of the operands.  A score is sum over groups of s_g (q_g . codes_g): a group (d mod D/32) is
+//   two steps of 16 of the product, so s_g multiplies the group's sum.  On the value side the weight times s_g is the
+//   other operand, one fragment per group; the 16 dimensions of a product's rows are of one group.
+//
+//   S^T [16 keys x 8] = K codes (A, as they lie: lane t of a row's four holds 16 bytes) times q (B).
+//   O^T [16 dimensions x 8] += V codes (A: pairs of keys brought together by a byte permutation) times weights
+//   (B: the score fragment, transposed by movmatrix).
+//
+// LO (f32 rows): a column pair holds the high and the low half of one head's operand, x = hi + lo to 2^-22, so
+// 4 heads share a tile; 16-bit rows have 8 heads of one half each (weights rounded to 2^-12 of their value).  Both
+// operands are scaled by powers of two into the half's range: q by its largest element, the weights by the
+// largest value scale seen, so that nothing overflows or vanishes whatever the cache holds.  Masked keys get a
+// score of -inf and scales of zero; codes are finite whatever they are.
+//
+// The tiles of all rows form one list that is cut into equal shares, one per CTA, so that a batch of a long and
+// many short contexts fills the GPU evenly.  A CTA's part of a row that it does not hold whole goes to scratch
+// as (maximum, sum, accumulator), and k_kv4_merge joins the parts in order.
 
-// One CTA of 4 warps per (query head, row): warp w takes positions w, w + 4, ...; one pass with the running
-// maximum and sum per warp, merged in warp order.
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-k_kv4_attn(const Kv4 c, const T * q, long long q_stride, int heads, const int32_t * row_seq, const int32_t * row_pos,
-           const int32_t * seq_slot, int n_seq, float scale, T * out, long long out_stride) {
-    pdl_trigger();
-    pdl_wait_primary();
-    constexpr int G = D / 32;
-    __shared__ float sm_m[4], sm_l[4], sm_acc[4][D];
-    const int h = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int seq = row_seq[r];
-    if (seq < 0 || seq >= n_seq) return;
-    const int slot = seq_slot[seq];
-    const int n = slot >= 0 && slot < c.n_slots ? min(row_pos[r], c.max_len - 1) + 1 : 0;
-    T * dst = out + r * out_stride + h * D;
-    if (n <= 0) {
-        for (int d = threadIdx.x; d < D; d += 128) dst[d] = from_f32<T>(0.f);
-        return;
-    }
-    float qv[G], acc[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        qv[g] = to_f32(q[r * q_stride + h * D + lane * G + g]);
-        acc[g] = 0.f;
-    }
-    const size_t base = (size_t(slot) * c.kv_heads + h / (heads / c.kv_heads)) * c.max_len;
-    float m = -INFINITY, l = 0.f;
-    for (int p = warp; p < n; p += 4) {
-        const uint8_t * kc = c.k_codes + (base + p) * (D / 2) + lane * (G / 2);
-        const uint8_t * vc = c.v_codes + (base + p) * (D / 2) + lane * (G / 2);
-        float s = 0.f, vv[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int sh = 4 * (g & 1);
-            s = fmaf(qv[g], float(((kc[g / 2] >> sh) & 15) - 8) * __half2float(__ushort_as_half(c.k_scales[(base + p) * G + g])), s);
-            vv[g] = float(((vc[g / 2] >> sh) & 15) - 8) * __half2float(__ushort_as_half(c.v_scales[(base + p) * G + g]));
-        }
-        s = warp_sum(s) * scale;
-        const float mn = fmaxf(m, s);
-        const float corr = m == -INFINITY ? 1.f : expf(m - mn), e = s == -INFINITY ? 0.f : expf(s - mn);
-        l = l * corr + e;
-#pragma unroll
-        for (int g = 0; g < G; ++g) acc[g] = fmaf(e, vv[g], acc[g] * corr);
-        m = mn;
-    }
-    if (lane == 0) {
-        sm_m[warp] = m;
-        sm_l[warp] = l;
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) sm_acc[warp][lane * G + g] = acc[g];
-    __syncthreads();
-    if (warp) return;
-    float M = -INFINITY, L = 0.f, A[G] = {};
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w]);
-    for (int w = 0; w < 4; ++w) {
-        if (sm_l[w] == 0.f) continue;  // a warp that saw no position
-        const float f = expf(sm_m[w] - M);
-        L = fmaf(sm_l[w], f, L);
-#pragma unroll
-        for (int g = 0; g < G; ++g) A[g] = fmaf(sm_acc[w][lane * G + g], f, A[g]);
-    }
-#pragma unroll
-    for (int g = 0; g < G; ++g) dst[lane * G + g] = from_f32<T>(A[g] / L);
+constexpr int kKeys = 64;        // keys per tile
+constexpr int kAttnWarps = 4;    // warps of a CTA, each with tiles of its own
+constexpr int kStages = 2;       // tiles in flight per warp
+constexpr int kSplitRows = 512;  // rows up to which the tiles of all rows are cut into equal shares
+constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
+
+template <int D> struct Kv4Tile {
+    static constexpr int kCodes = kKeys * D / 2, kScales = kKeys * D / 16;  // bytes of one of K and V
+    static constexpr int kBytes = 2 * (kCodes + kScales);
+};
+
+struct Kv4Attn {
+    Kv4 c;
+    const void * q;
+    void * out;
+    long long q_stride, out_stride;
+    const int32_t * row_seq;
+    const int32_t * row_pos;
+    const int32_t * seq_slot;
+    float * part;  // [y][x][2][HC][D + 4]: a CTA's unfinished first part of a row, and its continued one
+    int rows, n_seq, heads, chunks;
+    int split;          // 0: one CTA per row
+    float scale_log2;   // scale * log2(e)
+};
+
+// Visible keys of row r: -1 for a row of no sequence.
+__device__ __forceinline__ int visible(const Kv4Attn & a, int r) {
+    const int seq = a.row_seq[r], pos = a.row_pos[r];
+    if (seq < 0 || seq >= a.n_seq) return -1;
+    const int slot = a.seq_slot[seq];
+    return slot >= 0 && slot < a.c.n_slots ? max(0, min(pos, a.c.max_len - 1) + 1) : 0;
 }
 
+// Visible keys of rows 4 i .. 4 i + 3 for thread i of the first 128, tiles of all rows before them, and of all rows together.
+// sm: 4 ints.
+__device__ __forceinline__ void scan_tiles(const Kv4Attn & a, int (&n)[4], int & before, int & total, int * sm) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = threadIdx.x * 4 + i;
+        n[i] = r < a.rows && threadIdx.x < 128 ? visible(a, r) : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mine += (max(n[i], 0) + kKeys - 1) / kKeys;
+    int upto = mine;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, x);
+        if (lane >= x) upto += o;
+    }
+    if (lane == 31 && warp < 4) sm[warp] = upto;
+    __syncthreads();
+    before = upto - mine;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        if (w < warp) before += sm[w];
+        total += sm[w];
+    }
+}
+
+__device__ __forceinline__ int tiles_per_share(int total, int shares) {
+    const int each = (total + shares - 1) / shares;
+    return max(kMinShare, (each + kAttnWarps - 1) / kAttnWarps * kAttnWarps);
+}
+
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Codes i and i + 4 of a word as halves 1 + c / 16.
+// Centred: c / 16 - 1/2, exact, one operation more.
+template <int i, bool CENTRED> __device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
+    uint32_t y = (x & 0x03c003c0u) | 0x3c003c00u;
+    if (CENTRED) {
+        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x3e00)));
+        y = *reinterpret_cast<const uint32_t *>(&v);
+    }
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    uint32_t y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
+
+// The key of a 16-key step that row g (and, 8 further, row g + 8) of the score fragment stands for.  Chosen so
+// that both the rows read for the scores (g = 2 i, 2 i + 1 together) and those read for the values (g = 2 t) fall
+// on different banks as far as a row of 64 or 32 bytes allows.
+template <int D> __device__ __forceinline__ int key_of(int g) {
+    return g & 1 ? 4 + ((g >> 1) ^ (D == 128 ? 1 : 2)) : g >> 1;
+}
+
+// W words of 4 bytes (1, 2 or 4) from shared memory.
+template <int W> __device__ __forceinline__ void lds(const unsigned char * p, uint32_t (&w)[W]) {
+    if constexpr (W == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+template <typename T, int D, bool LO>
+__global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
+    using Tile = Kv4Tile<D>;
+    constexpr int G = D / 32, HC = LO ? 4 : 8, H = LO ? 1 : 2;  // groups, heads of the CTA, heads of a lane's scores
+    extern __shared__ __align__(128) unsigned char ring_all[];
+    __shared__ uint64_t full[kAttnWarps][kStages];
+    __shared__ int sm_n[kSplitRows], sm_scan[4], sm_row, sm_off;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    unsigned char * ring = ring_all + warp * kStages * Tile::kBytes;
+    const int share_heads = a.heads / a.c.kv_heads;
+    const int kvh = blockIdx.y / a.chunks, chunk = blockIdx.y % a.chunks;
+    const int head0 = kvh * share_heads + chunk * HC, nh = min(HC, share_heads - chunk * HC);
+    T * const out = static_cast<T *>(a.out) + head0 * D;
+    pdl_trigger();
+    if (threadIdx.x < kAttnWarps * kStages) mbar_init(&full[0][0] + threadIdx.x, 1);
+    mbar_init_fence();
+    pdl_wait_primary();
+
+    const auto zero_row = [&](int r) {
+        for (int i = 0; i < nh * D; ++i) out[r * a.out_stride + i] = from_f32<T>(0.f);
+    };
+    int row, off = 0, left;  // the next row, its first tile, tiles left of the share
+    if (a.split) {
+        int n[4], before, total;
+        scan_tiles(a, n, before, total, sm_scan);
+        const int share = tiles_per_share(total, gridDim.x), begin = blockIdx.x * share;
+        left = min(share, total - begin);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = threadIdx.x * 4 + i, tiles = (max(n[i], 0) + kKeys - 1) / kKeys;
+            if (r < a.rows) sm_n[r] = n[i];
+            if (n[i] == 0 && r % gridDim.x == blockIdx.x) zero_row(r);
+            if (before <= begin && begin < before + tiles) {
+                sm_row = r;
+                sm_off = begin - before;
+            }
+            before += tiles;
+        }
+        __syncthreads();
+        if (left <= 0) return;
+        row = sm_row;
+        off = sm_off;
+    } else {
+        row = blockIdx.x;
+        const int n = visible(a, row);
+        if (threadIdx.x == 0) sm_n[0] = n;
+        if (n == 0 && threadIdx.x == 0) zero_row(row);
+        __syncthreads();
+        if (n <= 0) return;
+        left = (n + kKeys - 1) / kKeys;
+    }
+
+    unsigned issued = 0, used = 0;  // tiles of this warp: copies started, waited for
+    bool ok = true;
+    while (left > 0) {
+        const int n = sm_n[a.split ? row : 0];
+        if (n <= 0) {
+            ++row;
+            continue;
+        }
+        const int tiles = (n + kKeys - 1) / kKeys, t0 = off, t1 = min(tiles, off + left);
+        const int slot = a.seq_slot[a.row_seq[row]];
+        const size_t base = (size_t(slot) * a.c.kv_heads + kvh) * a.c.max_len;
+        const auto start = [&](int tile) {
+            unsigned char * dst = ring + (issued % kStages) * Tile::kBytes;
+            uint64_t * bar = &full[warp][issued % kStages];
+            ++issued;
+            if (lane == 0) {
+                const size_t key = base + size_t(tile) * kKeys;
+                mbar_arrive_expect_tx(bar, Tile::kBytes);
+                bulk_g2s(dst, a.c.k_codes + key * (D / 2), Tile::kCodes, bar);
+                bulk_g2s(dst + Tile::kCodes, a.c.k_scales + key * G, Tile::kScales, bar);
+                bulk_g2s(dst + Tile::kCodes + Tile::kScales, a.c.v_codes + key * (D / 2), Tile::kCodes, bar);
+                bulk_g2s(dst + 2 * Tile::kCodes + Tile::kScales, a.c.v_scales + key * G, Tile::kScales, bar);
+            }
+        };
+        int next = t0 + warp;
+        for (int i = 0; i < kStages && next < t1; ++i, next += kAttnWarps) start(next);
+
+        // q as the B operand: column g is a head (and, with LO, its high or low half); this lane's dimensions are
+        // [t D/4, +D/4), words of 8, codes i and i + 4 of a word a pair.  Scaled by 2^e to a largest element in [2^8, 2^9).
+        uint32_t qb[D / 16][2];
+        float init[G][2], cs[H];
+        {
+            const int col_head = LO ? g >> 1 : g;
+            float x[D / 4], top = 0.f;
+            const T * src = static_cast<const T *>(a.q) + row * a.q_stride + (head0 + min(col_head, nh - 1)) * D + t * (D / 4);
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                x[i] = col_head < nh ? to_f32(src[i]) : 0.f;
+                top = fmaxf(top, fabsf(x[i]));
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int ex = int(__float_as_uint(top) >> 23);  // 255: an infinity
+            const int e = ex == 255 ? 0 : min(135 - ex, 126);
+            const float up = pow2(e);
+            float gs[G] = {};
+#pragma unroll
+            for (int i = 0; i < D / 4; ++i) {
+                x[i] *= up;
+                if (LO) {
+                    const float hi = __half2float(__float2half_rn(x[i]));
+                    x[i] = g & 1 ? __half2float(__float2half_rn(x[i] - hi)) : hi;
+                } else {
+                    x[i] = __half2float(__float2half_rn(x[i]));
+                }
+                gs[i % G] += x[i];
+            }
+#pragma unroll
+            for (int st = 0; st < D / 16; ++st) {
+                const int i = st & 3, w = 2 * (st >> 2);  // code of a word, first of the step's two words
+                qb[st][0] = pack_h2(x[8 * w + i], x[8 * w + i + 4]);
+                qb[st][1] = pack_h2(x[8 * w + 8 + i], x[8 * w + 12 + i]);
+            }
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                gs[j] += __shfl_xor_sync(0xffffffffu, gs[j], 1);
+                gs[j] += __shfl_xor_sync(0xffffffffu, gs[j], 2);
+                // the accumulator's columns are 2 t and 2 t + 1
+                init[j][0] = -1.5f * __shfl_sync(0xffffffffu, gs[j], 8 * t);
+                init[j][1] = -1.5f * __shfl_sync(0xffffffffu, gs[j], 8 * t + 4);
+            }
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+                const int eh = __shfl_sync(0xffffffffu, e, 8 * t + 4 * j);
+                cs[j] = 16.f * a.scale_log2 * pow2(-eh);
+            }
+        }
+
+        float o[D / 16][4] = {}, ws[H][G] = {}, m[H], l[H] = {};  // accumulators, sums of the weights times scale
+#pragma unroll
+        for (int j = 0; j < H; ++j) m[j] = -INFINITY;
+        int ev = 0;  // exponent of the largest value scale seen: weights are scaled by 2^(28 - ev)
+        for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
+            const unsigned char * kc = ring + (used % kStages) * Tile::kBytes;
+            const unsigned char * ks = kc + Tile::kCodes, * vc = ks + Tile::kScales, * vs = vc + Tile::kCodes;
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[warp][used % kStages], (used / kStages) & 1u));
+            ++used;
+            if (!ok) break;
+            const int keys = n - tile * kKeys;  // visible keys of the tile, >= 1
+            // scores of keys 16 x + key_of(g) (+ 8), heads t (LO) or 2 t, 2 t + 1
+            float sc[4][2][H];
+            float mx[H];
+#pragma unroll
+            for (int j = 0; j < H; ++j) mx[j] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int k0 = 16 * x + key_of<D>(g);
+                uint32_t w0[D / 32], w1[D / 32], s0[G / 2], s1[G / 2];
+                lds(kc + k0 * (D / 2) + t * (D / 8), w0);
+                lds(kc + (k0 + 8) * (D / 2) + t * (D / 8), w1);
+                lds(ks + k0 * (2 * G), s0);
+                lds(ks + (k0 + 8) * (2 * G), s1);
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int j = 0; j < H; ++j) sc[x][y][j] = 0.f;
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    if (!LO) {
+                        acc[0] = acc[2] = init[j][0];
+                        acc[1] = acc[3] = init[j][1];
+                    }
+#pragma unroll
+                    for (int i = j; i < 4; i += G)  // codes of a word of group j
+#pragma unroll
+                        for (int w = 0; w < D / 32; w += 2) {
+                            const auto take = [&](auto ic) {
+                                constexpr int I = decltype(ic)::value;
+                                const uint32_t f[4] = {codes2<I, LO>(w0[w]), codes2<I, LO>(w1[w]), codes2<I, LO>(w0[w + 1]),
+                                                       codes2<I, LO>(w1[w + 1])};
+                                mma16816(acc, f, qb[2 * w + I][0], qb[2 * w + I][1]);
+                            };
+                            if (i == 0) take(std::integral_constant<int, 0>{});
+                            else if (i == 1) take(std::integral_constant<int, 1>{});
+                            else if (i == 2) take(std::integral_constant<int, 2>{});
+                            else take(std::integral_constant<int, 3>{});
+                        }
+                    const float2 f0 = h2f2(s0[j / 2]), f1 = h2f2(s1[j / 2]);
+                    const float a0 = j & 1 ? f0.y : f0.x, a1 = j & 1 ? f1.y : f1.x;
+                    if (LO) {
+                        sc[x][0][0] = fmaf(a0, acc[0] + acc[1], sc[x][0][0]);
+                        sc[x][1][0] = fmaf(a1, acc[2] + acc[3], sc[x][1][0]);
+                    } else {
+#pragma unroll
+                        for (int jj = 0; jj < H; ++jj) {
+                            sc[x][0][jj] = fmaf(a0, acc[jj], sc[x][0][jj]);
+                            sc[x][1][jj] = fmaf(a1, acc[2 + jj], sc[x][1][jj]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int j = 0; j < H; ++j) {
+                        float v = sc[x][y][j] * cs[j];
+                        if (keys < kKeys && k0 + 8 * y >= keys) v = -INFINITY;
+                        sc[x][y][j] = v;
+                        mx[j] = fmaxf(mx[j], v);
+                    }
+            }
+            // largest value scale of the visible keys: two keys a lane
+            uint32_t top;
+            {
+                uint32_t w[G];
+                lds(vs + lane * (4 * G), w);
+                uint32_t first = w[0] & 0x7fff7fffu, second = w[G / 2] & 0x7fff7fffu;
+                if (G == 4) {
+                    first = __vmaxu2(first, w[1] & 0x7fff7fffu);
+                    second = __vmaxu2(second, w[G - 1] & 0x7fff7fffu);
+                }
+                if (2 * lane >= keys) first = 0;
+                if (2 * lane + 1 >= keys) second = 0;
+                first = __vmaxu2(first, second);
+                top = __reduce_max_sync(0xffffffffu, max(first & 0xffffu, first >> 16)) >> 10;  // its exponent
+            }
+            const int grown = max(int(top) - ev, 0);
+            bool moved = grown > 0;
+            float corr[H];
+#pragma unroll
+            for (int j = 0; j < H; ++j) {
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+                const float mn = fmaxf(m[j], mx[j]);
+                corr[j] = mn == m[j] ? 1.f : exp2_approx(m[j] - mn);
+                moved = moved || mn != m[j];
+                m[j] = mn;
+                l[j] *= corr[j];
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+                ev += grown;
+                const float down = pow2(-grown);
+#pragma unroll
+                for (int j = 0; j < H; ++j) {
+                    const float f = corr[j] * down;
+#pragma unroll
+                    for (int i = 0; i < D / 16; ++i) {
+                        o[i][j] *= f;
+                        o[i][2 + j] *= f;
+                        if (LO) {
+                            o[i][1] *= f;
+                            o[i][3] *= f;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < G; ++i) ws[j][i] *= f;
+                }
+            }
+            const float wf = pow2(28 - ev);
+            float ref[H];
+#pragma unroll
+            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : m[j];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int k0 = 16 * x + key_of<D>(g);
+                uint32_t s0[G / 2], s1[G / 2];
+                lds(vs + k0 * (2 * G), s0);
+                lds(vs + (k0 + 8) * (2 * G), s1);
+                if (keys < kKeys) {
+#pragma unroll
+                    for (int j = 0; j < G / 2; ++j) {
+                        if (k0 >= keys) s0[j] = 0;
+                        if (k0 + 8 >= keys) s1[j] = 0;
+                    }
+                }
+                float p[2][H];
+#pragma unroll
+                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                    for (int j = 0; j < H; ++j) {
+                        p[y][j] = exp2_approx(sc[x][y][j] - ref[j]);
+                        l[j] += p[y][j];
+                        p[y][j] *= wf;
+                    }
+                uint32_t pb[G][2];
+#pragma unroll
+                for (int j = 0; j < G; ++j)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const float2 f = h2f2(y ? s1[j / 2] : s0[j / 2]);
+                        const float sv = j & 1 ? f.y : f.x;
+                        const float v0 = p[y][0] * sv;
+                        uint32_t w;
+                        if (LO) {
+                            w = pack_h2(v0, v0 - __half2float(__float2half_rn(v0)));
+                        } else {  // the 1.5 comes off the weights as the product sees them
+                            w = pack_h2(v0, p[y][H - 1] * sv);
+                            const float2 r = h2f2(w);
+                            ws[0][j] += r.x;
+                            ws[H - 1][j] += r.y;
+                        }
+                        pb[j][y] = transpose8x8(w);
+                    }
+                // values of keys 2 t, 2 t + 1 and 8 further (as the score rows count them): dimensions of word(s) g
+                uint32_t va[D / 64], vb[D / 64], vc2[D / 64], vd[D / 64];
+                const int ka = 16 * x + t, kb = 16 * x + 4 + (t ^ (D == 128 ? 1 : 2));
+                lds(vc + ka * (D / 2) + g * (D / 16), va);
+                lds(vc + kb * (D / 2) + g * (D / 16), vb);
+                lds(vc + (ka + 8) * (D / 2) + g * (D / 16), vc2);
+                lds(vc + (kb + 8) * (D / 2) + g * (D / 16), vd);
+                uint32_t lo01[D / 64], hi01[D / 64], lo23[D / 64], hi23[D / 64];  // codes 0-3, 4-7 of two keys
+#pragma unroll
+                for (int w = 0; w < D / 64; ++w) {
+                    lo01[w] = __byte_perm(va[w], vb[w], 0x5410);
+                    hi01[w] = __byte_perm(va[w], vb[w], 0x7632);
+                    lo23[w] = __byte_perm(vc2[w], vd[w], 0x5410);
+                    hi23[w] = __byte_perm(vc2[w], vd[w], 0x7632);
+                }
+                const auto take = [&](auto ic) {
+                    constexpr int I = decltype(ic)::value;
+                    if constexpr (D == 128) {  // dimensions 16 g + I, 16 g + 8 + I; then the same 4 further
+                        const uint32_t f[4] = {codes2<I, LO>(lo01[0]), codes2<I, LO>(lo01[1]), codes2<I, LO>(lo23[0]), codes2<I, LO>(lo23[1])};
+                        mma16816(o[I], f, pb[I][0], pb[I][1]);
+                        const uint32_t h[4] = {codes2<I, LO>(hi01[0]), codes2<I, LO>(hi01[1]), codes2<I, LO>(hi23[0]), codes2<I, LO>(hi23[1])};
+                        mma16816(o[I + 4], h, pb[I][0], pb[I][1]);
+                    } else {  // dimensions 8 g + I, 8 g + 4 + I
+                        const uint32_t f[4] = {codes2<I, LO>(lo01[0]), codes2<I, LO>(hi01[0]), codes2<I, LO>(lo23[0]), codes2<I, LO>(hi23[0])};
+                        mma16816(o[I], f, pb[I % G][0], pb[I % G][1]);
+                    }
+                };
+                take(std::integral_constant<int, 0>{});
+                take(std::integral_constant<int, 1>{});
+                take(std::integral_constant<int, 2>{});
+                take(std::integral_constant<int, 3>{});
+            }
+            __syncwarp();  // every lane has read the tile
+            if (next < t1) {
+                start(next);
+                next += kAttnWarps;
+            }
+        }
+
+        for (; used < issued; ++used)  // after a wait that ran out: copies in flight end before their memory is used
+            (void)mbar_wait(&full[warp][used % kStages], (used / kStages) & 1u);
+        // the warp's part: sums over the lanes of a head, then into the warp's own ring (its copies have landed)
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
+#pragma unroll
+                for (int i = 0; i < G; ++i) ws[j][i] += __shfl_xor_sync(0xffffffffu, ws[j][i], x);
+            }
+        }
+        constexpr int kRec = D + 4;
+        float * const mine = reinterpret_cast<float *>(ring);  // [HC][D + 4]: accumulator, maximum, sum
+        __syncwarp();
+        const float back = 16.f * pow2(ev - 28);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            float * rec = mine + (LO ? t : 2 * t + j) * kRec;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const float w = LO ? 0.f : 1.5f * ws[j][i % G];
+                const float v0 = (LO ? o[i][0] + o[i][1] : o[i][j]) - w, v1 = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) - w;
+                const int d = D == 128 ? 16 * g + i : 8 * g + i;
+                rec[d] = v0 * back;
+                rec[d + (D == 128 ? 8 : 4)] = v1 * back;
+            }
+            if (g == 0) {
+                rec[D] = m[j];
+                rec[D + 1] = l[j];
+            }
+        }
+        __syncthreads();
+        const bool whole = t0 == 0 && t1 == tiles;
+        float * part = whole ? nullptr
+                             : a.part + ((size_t(blockIdx.y) * gridDim.x + blockIdx.x) * 2 + (t0 ? 1 : 0)) * (HC * kRec);
+        for (int i = threadIdx.x; i < nh * D; i += 128) {
+            const int h = i / D, d = i % D;
+            const float * rec = reinterpret_cast<const float *>(ring_all) + h * kRec;
+            constexpr int kNext = kStages * Tile::kBytes / 4;
+            float M = -INFINITY, L = 0.f, A = 0.f;
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) M = fmaxf(M, rec[w * kNext + D]);
+            const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float f = exp2_approx(rec[w * kNext + D] - ref);
+                L = fmaf(rec[w * kNext + D + 1], f, L);
+                A = fmaf(rec[w * kNext + d], f, A);
+            }
+            if (whole) {
+                out[row * a.out_stride + i] = from_f32<T>(A / L);
+            } else {
+                part[h * kRec + d] = A;
+                if (d == 0) {
+                    part[h * kRec + D] = M;
+                    part[h * kRec + D + 1] = L;
+                }
+            }
+        }
+        left -= t1 - t0;
+        off = 0;
+        ++row;
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copies overwrite these records
+        __syncthreads();
+        if (!__syncthreads_and(ok)) {
+            if (threadIdx.x == 0) atomicOr(&g_attn_status, kStatusWaitTimeout);
+            break;
+        }
+    }
+}
+
+// Joins the parts of the rows that were cut: CTA = (row, K/V head chunk, head), thread = a dimension and every
+// kGroups-th part; the sums run in a fixed order.
+constexpr int kMergeThreads = 512;
+constexpr int kMaxShares = 1024;
+
+template <typename T, int D, int HC>
+__global__ void __launch_bounds__(kMergeThreads) k_kv4_merge(const Kv4Attn a, int shares) {
+    constexpr int kRec = D + 4, kGroups = kMergeThreads / D;
+    __shared__ int sm_scan[4], sm_before, sm_n, sm_total;
+    __shared__ float sm_w[kMaxShares], sm_red[kMergeThreads / 32], sm_acc[kGroups][D];
+    const int row = blockIdx.x, y = blockIdx.y, h = blockIdx.z;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    pdl_wait_primary();
+    const int share_heads = a.heads / a.c.kv_heads, chunk = y % a.chunks;
+    const int head = y / a.chunks * share_heads + chunk * HC + h;
+    if (chunk * HC + h >= share_heads) return;
+    int n[4], before, total;
+    scan_tiles(a, n, before, total, sm_scan);
+    if (threadIdx.x < 128) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (threadIdx.x * 4 + i == row) {
+                sm_before = before;
+                sm_n = n[i];
+            }
+            before += (max(n[i], 0) + kKeys - 1) / kKeys;
+        }
+        if (threadIdx.x == 0) sm_total = total;
+    }
+    __syncthreads();
+    if (sm_n <= 0) return;
+    const int share = tiles_per_share(sm_total, shares), tiles = (sm_n + kKeys - 1) / kKeys;
+    const int x0 = sm_before / share, parts = (sm_before + tiles - 1) / share - x0 + 1;
+    if (parts == 1) return;
+    // a CTA's record 0 is the row that it begins and does not end, record 1 the row that it goes on with
+    const auto rec = [&](int i) {
+        return a.part + (((size_t(y) * shares + x0 + i) * 2 + (i > 0)) * HC + h) * kRec;
+    };
+    float M = -INFINITY;
+    for (int i = threadIdx.x; i < parts; i += kMergeThreads) M = fmaxf(M, rec(i)[D]);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+    if (lane == 0) sm_red[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; ++i) M = fmaxf(M, sm_red[i]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    __syncthreads();
+    float L = 0.f;
+    for (int i = threadIdx.x; i < parts; i += kMergeThreads) {
+        const float f = exp2_approx(rec(i)[D] - ref);
+        sm_w[i] = f;
+        L = fmaf(rec(i)[D + 1], f, L);
+    }
+    L = warp_sum(L);
+    if (lane == 0) sm_red[warp] = L;
+    __syncthreads();
+    const int d = threadIdx.x % D, group = threadIdx.x / D;
+    float A = 0.f;
+#pragma unroll 8
+    for (int i = group; i < parts; i += kGroups) A = fmaf(rec(i)[d], sm_w[i], A);
+    sm_acc[group][d] = A;
+    __syncthreads();
+    if (group) return;
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < kMergeThreads / 32; ++i) L += sm_red[i];
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) A += sm_acc[i][d];
+    static_cast<T *>(a.out)[row * a.out_stride + head * D + d] = from_f32<T>(A / L);
+}
+
+// How a call is cut up: shares (CTAs) per K/V head chunk, 0 for one CTA per row.
+struct AttnPlan {
+    int heads_per_cta, chunks, ys, shares;
+    size_t scratch;
+};
+
+AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
+    AttnPlan p;
+    const int share_heads = heads / c->kv_heads;
+    p.heads_per_cta = dtype == EXL3CU_F32 ? 4 : 8;
+    p.chunks = (share_heads + p.heads_per_cta - 1) / p.heads_per_cta;
+    p.ys = c->kv_heads * p.chunks;
+    p.shares = 0;
+    p.scratch = 0;
+    if (rows > kSplitRows) return p;
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+        (void)cudaGetLastError();
+    // as many CTAs as are resident together (three per SM), no more than there can be shares
+    const long long most = (long long)rows * (c->max_len / kKeys + kMinShare - 1) / kMinShare;
+    p.shares = int(std::max(1ll, std::min((long long)std::min(3 * sms / p.ys, kMaxShares), most)));
+    p.scratch = size_t(p.ys) * p.shares * 2 * p.heads_per_cta * (c->head_dim + 4) * sizeof(float);
+    return p;
+}
+
+std::atomic<unsigned long long> g_attn_attr[6];
+
 }  // namespace
+
+cudaError_t attn_read_status(unsigned * out, bool clear) {
+    cudaError_t e = cudaMemcpyFromSymbol(out, g_attn_status, sizeof(unsigned));
+    if (e == cudaSuccess && clear && *out) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(g_attn_status, &zero, sizeof(unsigned));
+    }
+    return e;
+}
 
 }  // namespace exl3cu
 
@@ -367,10 +972,9 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
 }
 
 size_t exl3cu_kv4_attn_scratch_bytes(const exl3cu_kv4_cache * cache, int rows, int heads) {
-    (void)cache;
-    (void)rows;
-    (void)heads;
-    return 0;
+    if (!cache_ok(cache) || rows <= 0 || heads <= 0 || heads % cache->kv_heads) return 0;
+    // the larger of the two forms: f32 rows, and 16-bit rows
+    return std::max(plan_attn(cache, rows, heads, EXL3CU_F32).scratch, plan_attn(cache, rows, heads, EXL3CU_F16).scratch);
 }
 
 int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_stride, int dtype, int rows, int heads,
@@ -382,20 +986,43 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
     if (rows < 0 || n_seq < 0 || rows > 65535) return bad("kv4_attn: rows must be 0..65535 and n_seq not negative");
     if (heads <= 0 || heads % cache->kv_heads || heads > 1024)
         return bad("kv4_attn: heads must be a multiple of kv_heads, at most 1024");
+    if (!(scale > 0.f) || scale > 1e30f) return bad("kv4_attn: scale must be positive and finite");
     if (!rows || !n_seq) return EXL3CU_OK;
     const size_t width = size_t(heads) * cache->head_dim;
     if (!d_row_seq || !d_row_pos || !d_seq_slot || !rows_ok(d_q, q_stride, width, dtype) ||
         !rows_ok(d_out, out_stride, width, dtype))
         return bad("kv4_attn: null or misaligned operand, or rows closer than their width");
-    (void)d_scratch;
-    (void)scratch_bytes;
-    const Kv4 c = device_cache(cache);
+    const AttnPlan p = plan_attn(cache, rows, heads, dtype);
+    if (p.scratch && (!d_scratch || scratch_bytes < p.scratch || reinterpret_cast<uintptr_t>(d_scratch) % 16))
+        return bad("kv4_attn: scratch missing, misaligned or too small (exl3cu_kv4_attn_scratch_bytes)");
+    const Kv4Attn a{device_cache(cache), d_q, d_out, (long long)q_stride, (long long)out_stride, d_row_seq, d_row_pos,
+                    d_seq_slot, static_cast<float *>(d_scratch), rows, n_seq, heads, p.chunks, p.shares > 0,
+                    scale * 1.4426950408889634f};
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        return attn_launch(cache->head_dim == 128 ? k_kv4_attn<T, 128> : k_kv4_attn<T, 64>,
-                           dim3(unsigned(heads), unsigned(rows)), dim3(128), 0, stream, c, static_cast<const T *>(d_q),
-                           (long long)q_stride, heads, d_row_seq, d_row_pos, d_seq_slot, n_seq, scale,
-                           static_cast<T *>(d_out), (long long)out_stride);
+        constexpr bool LO = std::is_same_v<T, float>;
+        constexpr int HC = LO ? 4 : 8;
+        const auto run = [&](auto dim) {
+            constexpr int D = decltype(dim)::value;
+            constexpr int smem = kAttnWarps * kStages * Kv4Tile<D>::kBytes;
+            static_assert(size_t(HC) * (D + 4) * 4 <= kStages * Kv4Tile<D>::kBytes, "a warp's record fits its ring");
+            int dev = 0;
+            if (cudaGetDevice(&dev) != cudaSuccess) return api_cuda_fail(cudaGetLastError(), "kv4_attn");
+            auto & done = g_attn_attr[(D == 128 ? 3 : 0) + (LO ? 0 : std::is_same_v<T, __half> ? 1 : 2)];
+            const unsigned long long bit = 1ull << (dev & 63);
+            if (!(done.load() & bit)) {
+                const cudaError_t e =
+                    cudaFuncSetAttribute(k_kv4_attn<T, D, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                if (e != cudaSuccess) return api_cuda_fail(e, "kv4_attn: shared memory");
+                done.fetch_or(bit);
+            }
+            const int rc = attn_launch(k_kv4_attn<T, D, LO>, dim3(unsigned(p.shares ? p.shares : rows), unsigned(p.ys)),
+                                       dim3(128), size_t(smem), stream, a);
+            if (rc || !p.shares) return rc;
+            return attn_launch(k_kv4_merge<T, D, HC>, dim3(unsigned(rows), unsigned(p.ys), HC), dim3(kMergeThreads), 0,
+                               stream, a, p.shares);
+        };
+        return cache->head_dim == 128 ? run(std::integral_constant<int, 128>{}) : run(std::integral_constant<int, 64>{});
     });
 }
 

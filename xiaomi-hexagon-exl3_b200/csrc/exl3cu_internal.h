@@ -149,6 +149,7 @@ cudaError_t launch_get_rows(const uint32_t * lsc, const uint16_t * suh, const ui
 cudaError_t rows_read_status(unsigned * out, bool clear);
 cudaError_t peer_read_status(unsigned * out, bool clear);
 cudaError_t prompt_read_status(unsigned * out, bool clear);
+cudaError_t attn_read_status(unsigned * out, bool clear);
 // 0 when p is device (or managed) memory of `device` (-1: any device), else a failure status with the
 // thread's error text set (exl3cu_api.cu).
 int api_check_device_ptr(const void * p, int device, const char * name);
