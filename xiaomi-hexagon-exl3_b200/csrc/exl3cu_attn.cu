@@ -195,11 +195,10 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 //
 // One pass over the keys of a row in tiles of 64, on the matrix instructions, with the running maximum and sum
 // of a softmax.  Bound by the bytes of the cache (2 (D/2 + D/16) a key and K/V head) as long as a code costs about
-// one instruction; so codes are never multiplied out:
+// one instruction; so codes are never multiplied by their scales:
 //
-//   A code c of 4 bits becomes the half 1 + c/16 by a shift and one logic operation on two codes at a time: the
-//   bits go to the top of the mantissa of 1.0.  (c - 8) s = 16 s ((1 + c/16) - 1.5), and the 1.5 comes off sums:
-//   off the scores as the initial accumulator -1.5 sum q, off the result as -1.5 sum of the weights.
+//   Codes become halves by one logic operation on two at a time (into the mantissa of 1024) and one multiply-add
+//   (to c - 8, exact), after a shift for every other four.
 //   Scales stay out of the operands.  A score is sum over groups of s_g (q_g . codes_g): a group (d mod D/32) is
 //   two steps of 16 of the product, so s_g multiplies the group's sum.  On the value side the weight times s_g is the
 //   other operand, one fragment per group; the 16 dimensions of a product's rows are of one group.
@@ -209,19 +208,21 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 //   (B: the score fragment, transposed by movmatrix).
 //
 // LO (f32 rows): a column pair holds the high and the low half of one head's operand, x = hi + lo to 2^-22, so
-// 4 heads share a tile; 16-bit rows have 8 heads of one half each (weights rounded to 2^-12 of their value).  Both
-// operands are scaled by powers of two into the half's range: q by its largest element, the weights by the
-// largest value scale seen, so that nothing overflows or vanishes whatever the cache holds.  Masked keys get a
-// score of -inf and scales of zero; codes are finite whatever they are.
+// 4 heads share a tile; 16-bit rows have 8 heads of one half each (weights rounded to 2^-11 of their value, the
+// product's own precision).  Both operands are scaled by powers of two into the half's range: q by its largest
+// element, the weights by the largest value scale seen, so that nothing overflows or vanishes whatever the cache
+// holds.  Masked keys get a score of -inf and scales of zero; codes are finite whatever they are.
 //
 // The tiles of all rows form one list that is cut into equal shares, one per CTA, so that a batch of a long and
-// many short contexts fills the GPU evenly.  A CTA's part of a row that it does not hold whole goes to scratch
-// as (maximum, sum, accumulator), and k_kv4_merge joins the parts in order.
+// many short contexts fills the GPU evenly (a row counts kRowCost tiles more than it has: what taking up a row costs
+// a CTA).  A CTA's part of a row that it does not hold whole goes to scratch as (maximum, sum, accumulator), and
+// k_kv4_merge joins the parts in order.
 
 constexpr int kKeys = 64;        // keys per tile
 constexpr int kAttnWarps = 4;    // warps of a CTA, each with tiles of its own
 constexpr int kStages = 2;       // tiles in flight per warp
-constexpr int kSplitRows = 512;  // rows up to which the tiles of all rows are cut into equal shares
+constexpr int kSplitRows = 256;  // rows up to which the tiles of all rows are cut into equal shares
+constexpr int kRowCost = 2;
 constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
 
 template <int D> struct Kv4Tile {
@@ -243,26 +244,30 @@ struct Kv4Attn {
     float scale_log2;   // scale * log2(e)
 };
 
-// Visible keys of row r: -1 for a row of no sequence.
-__device__ __forceinline__ int visible(const Kv4Attn & a, int r) {
+// Visible keys of row r and its slot: -1 keys for a row of no sequence.
+__device__ __forceinline__ int visible(const Kv4Attn & a, int r, int & slot) {
     const int seq = a.row_seq[r], pos = a.row_pos[r];
+    slot = 0;
     if (seq < 0 || seq >= a.n_seq) return -1;
-    const int slot = a.seq_slot[seq];
+    slot = a.seq_slot[seq];
     return slot >= 0 && slot < a.c.n_slots ? max(0, min(pos, a.c.max_len - 1) + 1) : 0;
 }
 
-// Visible keys of rows 4 i .. 4 i + 3 for thread i of the first 128, tiles of all rows before them, and of all rows together.
-// sm: 4 ints.
-__device__ __forceinline__ void scan_tiles(const Kv4Attn & a, int (&n)[4], int & before, int & total, int * sm) {
+__device__ __forceinline__ int tiles_of(int n) { return (max(n, 0) + kKeys - 1) / kKeys; }
+__device__ __forceinline__ int list_of(int n) { return n > 0 ? tiles_of(n) + kRowCost : 0; }
+
+// Visible keys and slots of rows 2 i and 2 i + 1 for thread i of the first 128, the list before them, and the whole
+// list's length.  sm: 4 ints.
+__device__ __forceinline__ void scan_rows(const Kv4Attn & a, int (&n)[2], int (&slot)[2], int & before, int & total,
+                                          int * sm) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int mine = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = threadIdx.x * 4 + i;
-        n[i] = r < a.rows && threadIdx.x < 128 ? visible(a, r) : -1;
+    for (int i = 0; i < 2; ++i) {
+        const int r = threadIdx.x * 2 + i;
+        n[i] = -1;
+        if (r < a.rows && threadIdx.x < 128) n[i] = visible(a, r, slot[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mine += (max(n[i], 0) + kKeys - 1) / kKeys;
+    const int mine = list_of(n[0]) + list_of(n[1]);
     int upto = mine;
 #pragma unroll
     for (int x = 1; x < 32; x <<= 1) {
@@ -280,7 +285,7 @@ __device__ __forceinline__ void scan_tiles(const Kv4Attn & a, int (&n)[4], int &
     }
 }
 
-__device__ __forceinline__ int tiles_per_share(int total, int shares) {
+__device__ __forceinline__ int share_of(int total, int shares) {
     const int each = (total + shares - 1) / shares;
     return max(kMinShare, (each + kAttnWarps - 1) / kAttnWarps * kAttnWarps);
 }
@@ -291,16 +296,21 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Codes i and i + 4 of a word as halves 1 + c / 16.
-// Centred: c / 16 - 1/2, exact, one operation more.
-template <int i, bool CENTRED> __device__ __forceinline__ uint32_t codes2(uint32_t w) {
-    const uint32_t x = i == 0 ? w << 6 : i == 1 ? w << 2 : i == 2 ? w >> 2 : w >> 6;
-    uint32_t y = (x & 0x03c003c0u) | 0x3c003c00u;
-    if (CENTRED) {
-        const __half2 v = __hsub2(*reinterpret_cast<const __half2 *>(&y), __half2half2(__ushort_as_half(0x3e00)));
-        y = *reinterpret_cast<const uint32_t *>(&v);
-    }
-    return y;
+// d = a b.
+__device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Halves c - 8 of codes i and i + 4 of a word, i = 0 .. 3, from the word for i < 2 and from the word shifted right
+// by 8 for i >= 2: the code's bits in the mantissa of 1024 make 1024 + c (or, 4 bits up, 1024 + 16 c).
+template <int i> __device__ __forceinline__ uint32_t codes2(uint32_t w) {
+    const uint32_t x = (w & (i & 1 ? 0x00f000f0u : 0x000f000fu)) | 0x64006400u;
+    const __half2 v = *reinterpret_cast<const __half2 *>(&x);
+    const __half2 y = i & 1 ? __hfma2(v, __half2half2(__ushort_as_half(0x2c00)), __half2half2(__ushort_as_half(0xd480)))
+                            : __hadd2(v, __half2half2(__ushort_as_half(0xe408)));  // / 16 - 72; - 1032
+    return *reinterpret_cast<const uint32_t *>(&y);
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
@@ -321,6 +331,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
 __device__ __forceinline__ float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
@@ -329,6 +345,18 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 // on different banks as far as a row of 64 or 32 bytes allows.
 template <int D> __device__ __forceinline__ int key_of(int g) {
     return g & 1 ? 4 + ((g >> 1) ^ (D == 128 ? 1 : 2)) : g >> 1;
+}
+
+// N elements from 16-byte aligned memory.
+template <int N, typename T> __device__ __forceinline__ void load_row(const T * p, float (&x)[N]) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p + i);
+        const T * e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i + j] = to_f32(e[j]);
+    }
 }
 
 // W words of 4 bytes (1, 2 or 4) from shared memory.
@@ -350,7 +378,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
     constexpr int G = D / 32, HC = LO ? 4 : 8, H = LO ? 1 : 2;  // groups, heads of the CTA, heads of a lane's scores
     extern __shared__ __align__(128) unsigned char ring_all[];
     __shared__ uint64_t full[kAttnWarps][kStages];
-    __shared__ int sm_n[kSplitRows], sm_scan[4], sm_row, sm_off;
+    __shared__ int sm_n[kSplitRows], sm_slot[kSplitRows], sm_scan[4], sm_row, sm_off;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     unsigned char * ring = ring_all + warp * kStages * Tile::kBytes;
     const int share_heads = a.heads / a.c.kv_heads;
@@ -365,47 +393,54 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
     const auto zero_row = [&](int r) {
         for (int i = 0; i < nh * D; ++i) out[r * a.out_stride + i] = from_f32<T>(0.f);
     };
-    int row, off = 0, left;  // the next row, its first tile, tiles left of the share
+    // the next row (of the list; row0 + row of the call), where in it to begin, what is left of the share
+    int row = 0, off = 0, left;
+    const int row0 = a.split ? 0 : blockIdx.x;
     if (a.split) {
-        int n[4], before, total;
-        scan_tiles(a, n, before, total, sm_scan);
-        const int share = tiles_per_share(total, gridDim.x), begin = blockIdx.x * share;
+        int n[2], slot[2], before, total;
+        scan_rows(a, n, slot, before, total, sm_scan);
+        const int share = share_of(total, gridDim.x), begin = blockIdx.x * share;
         left = min(share, total - begin);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = threadIdx.x * 4 + i, tiles = (max(n[i], 0) + kKeys - 1) / kKeys;
-            if (r < a.rows) sm_n[r] = n[i];
+        for (int i = 0; i < 2; ++i) {
+            const int r = threadIdx.x * 2 + i, list = list_of(n[i]);
+            if (r < a.rows) {
+                sm_n[r] = n[i];
+                sm_slot[r] = slot[i];
+            }
             if (n[i] == 0 && r % gridDim.x == blockIdx.x) zero_row(r);
-            if (before <= begin && begin < before + tiles) {
+            if (before <= begin && begin < before + list) {
                 sm_row = r;
                 sm_off = begin - before;
             }
-            before += tiles;
+            before += list;
         }
         __syncthreads();
         if (left <= 0) return;
         row = sm_row;
         off = sm_off;
     } else {
-        row = blockIdx.x;
-        const int n = visible(a, row);
-        if (threadIdx.x == 0) sm_n[0] = n;
-        if (n == 0 && threadIdx.x == 0) zero_row(row);
+        int slot;
+        const int n = visible(a, row0, slot);
+        if (threadIdx.x == 0) {
+            sm_n[0] = n;
+            sm_slot[0] = slot;
+            if (n == 0) zero_row(row0);
+        }
         __syncthreads();
         if (n <= 0) return;
-        left = (n + kKeys - 1) / kKeys;
+        left = list_of(n);
     }
 
     unsigned issued = 0, used = 0;  // tiles of this warp: copies started, waited for
     bool ok = true;
     while (left > 0) {
-        const int n = sm_n[a.split ? row : 0];
-        if (n <= 0) {
-            ++row;
-            continue;
-        }
-        const int tiles = (n + kKeys - 1) / kKeys, t0 = off, t1 = min(tiles, off + left);
-        const int slot = a.seq_slot[a.row_seq[row]];
+        const int n = sm_n[row], tiles = tiles_of(n), t0 = min(off, tiles), t1 = min(tiles, off + left);
+        left -= min(left, list_of(n) - off);
+        off = 0;
+        const int call_row = row0 + row, slot = sm_slot[row];
+        ++row;
+        if (t0 >= t1) continue;
         const size_t base = (size_t(slot) * a.c.kv_heads + kvh) * a.c.max_len;
         const auto start = [&](int tile) {
             unsigned char * dst = ring + (issued % kStages) * Tile::kBytes;
@@ -426,32 +461,29 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
         // q as the B operand: column g is a head (and, with LO, its high or low half); this lane's dimensions are
         // [t D/4, +D/4), words of 8, codes i and i + 4 of a word a pair.  Scaled by 2^e to a largest element in [2^8, 2^9).
         uint32_t qb[D / 16][2];
-        float init[G][2], cs[H];
+        float cs[H];
         {
             const int col_head = LO ? g >> 1 : g;
             float x[D / 4], top = 0.f;
-            const T * src = static_cast<const T *>(a.q) + row * a.q_stride + (head0 + min(col_head, nh - 1)) * D + t * (D / 4);
+            const T * src = static_cast<const T *>(a.q) + call_row * a.q_stride + (head0 + min(col_head, nh - 1)) * D + t * (D / 4);
+            load_row<D / 4>(src, x);
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) {
-                x[i] = col_head < nh ? to_f32(src[i]) : 0.f;
+                if (col_head >= nh) x[i] = 0.f;
                 top = fmaxf(top, fabsf(x[i]));
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = int(__float_as_uint(top) >> 23);  // 255: an infinity
-            const int e = ex == 255 ? 0 : min(135 - ex, 126);
+            const int e = ex == 255 ? 0 : min(135 - ex, 60);  // below 2^-52 a query's scores are 0 but for 2^-40
             const float up = pow2(e);
-            float gs[G] = {};
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) {
                 x[i] *= up;
                 if (LO) {
                     const float hi = __half2float(__float2half_rn(x[i]));
-                    x[i] = g & 1 ? __half2float(__float2half_rn(x[i] - hi)) : hi;
-                } else {
-                    x[i] = __half2float(__float2half_rn(x[i]));
+                    x[i] = g & 1 ? x[i] - hi : hi;
                 }
-                gs[i % G] += x[i];
             }
 #pragma unroll
             for (int st = 0; st < D / 16; ++st) {
@@ -460,24 +492,18 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 qb[st][1] = pack_h2(x[8 * w + 8 + i], x[8 * w + 12 + i]);
             }
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                gs[j] += __shfl_xor_sync(0xffffffffu, gs[j], 1);
-                gs[j] += __shfl_xor_sync(0xffffffffu, gs[j], 2);
-                // the accumulator's columns are 2 t and 2 t + 1
-                init[j][0] = -1.5f * __shfl_sync(0xffffffffu, gs[j], 8 * t);
-                init[j][1] = -1.5f * __shfl_sync(0xffffffffu, gs[j], 8 * t + 4);
-            }
-#pragma unroll
-            for (int j = 0; j < H; ++j) {
+            for (int j = 0; j < H; ++j) {  // the score's columns are 2 t and 2 t + 1
                 const int eh = __shfl_sync(0xffffffffu, e, 8 * t + 4 * j);
-                cs[j] = 16.f * a.scale_log2 * pow2(-eh);
+                cs[j] = fminf(fmaxf(a.scale_log2 * pow2(-eh), 1.2e-38f), 3e38f);  // 0 or inf would meet inf or 0
             }
         }
 
-        float o[D / 16][4] = {}, ws[H][G] = {}, m[H], l[H] = {};  // accumulators, sums of the weights times scale
+        // accumulators; largest score (before cs); sum of the weights.  Weights are exp2((s - m) cs + 28 - ev),
+        // ev the exponent of the largest value scale seen: times a value scale they stay below 2^14.
+        float o[D / 16][4] = {}, m[H], l[H] = {};
 #pragma unroll
         for (int j = 0; j < H; ++j) m[j] = -INFINITY;
-        int ev = 0;  // exponent of the largest value scale seen: weights are scaled by 2^(28 - ev)
+        int ev = 0;
         for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
             const unsigned char * kc = ring + (used % kStages) * Tile::kBytes;
             const unsigned char * ks = kc + Tile::kCodes, * vc = ks + Tile::kScales, * vs = vc + Tile::kCodes;
@@ -485,95 +511,89 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
             ++used;
             if (!ok) break;
             const int keys = n - tile * kKeys;  // visible keys of the tile, >= 1
+            if (keys < kKeys) {  // what lies behind them may not be finite: scales of zero
+                uint32_t * z = reinterpret_cast<uint32_t *>(const_cast<unsigned char *>(ks));
+                for (int i = keys * (G / 2) + lane; i < kKeys * (G / 2); i += 32) {
+                    z[i] = 0;
+                    z[i + (Tile::kScales + Tile::kCodes) / 4] = 0;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the slot
+                __syncwarp();
+            }
             // scores of keys 16 x + key_of(g) (+ 8), heads t (LO) or 2 t, 2 t + 1
             float sc[4][2][H];
-            float mx[H];
-#pragma unroll
-            for (int j = 0; j < H; ++j) mx[j] = -INFINITY;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int k0 = 16 * x + key_of<D>(g);
-                uint32_t w0[D / 32], w1[D / 32], s0[G / 2], s1[G / 2];
+                uint32_t w0[D / 32], w1[D / 32], u0[D / 32], u1[D / 32], s0[G / 2], s1[G / 2];
                 lds(kc + k0 * (D / 2) + t * (D / 8), w0);
                 lds(kc + (k0 + 8) * (D / 2) + t * (D / 8), w1);
                 lds(ks + k0 * (2 * G), s0);
                 lds(ks + (k0 + 8) * (2 * G), s1);
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
+                for (int w = 0; w < D / 32; ++w) {
+                    u0[w] = w0[w] >> 8;
+                    u1[w] = w1[w] >> 8;
+                }
+                float acc[G][4];
+                const auto take = [&](auto ic) {  // codes I and I + 4 of the words: group I mod G
+                    constexpr int I = decltype(ic)::value;
 #pragma unroll
-                    for (int j = 0; j < H; ++j) sc[x][y][j] = 0.f;
+                    for (int w = 0; w < D / 32; w += 2) {
+                        const uint32_t f[4] = {codes2<I>(I < 2 ? w0[w] : u0[w]), codes2<I>(I < 2 ? w1[w] : u1[w]),
+                                               codes2<I>(I < 2 ? w0[w + 1] : u0[w + 1]), codes2<I>(I < 2 ? w1[w + 1] : u1[w + 1])};
+                        if (w == 0 && I < G) mma16816_first(acc[I % G], f, qb[2 * w + I][0], qb[2 * w + I][1]);
+                        else mma16816(acc[I % G], f, qb[2 * w + I][0], qb[2 * w + I][1]);
+                    }
+                };
+                take(std::integral_constant<int, 0>{});
+                take(std::integral_constant<int, 1>{});
+                take(std::integral_constant<int, 2>{});
+                take(std::integral_constant<int, 3>{});
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
-                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                    if (!LO) {
-                        acc[0] = acc[2] = init[j][0];
-                        acc[1] = acc[3] = init[j][1];
-                    }
-#pragma unroll
-                    for (int i = j; i < 4; i += G)  // codes of a word of group j
-#pragma unroll
-                        for (int w = 0; w < D / 32; w += 2) {
-                            const auto take = [&](auto ic) {
-                                constexpr int I = decltype(ic)::value;
-                                const uint32_t f[4] = {codes2<I, LO>(w0[w]), codes2<I, LO>(w1[w]), codes2<I, LO>(w0[w + 1]),
-                                                       codes2<I, LO>(w1[w + 1])};
-                                mma16816(acc, f, qb[2 * w + I][0], qb[2 * w + I][1]);
-                            };
-                            if (i == 0) take(std::integral_constant<int, 0>{});
-                            else if (i == 1) take(std::integral_constant<int, 1>{});
-                            else if (i == 2) take(std::integral_constant<int, 2>{});
-                            else take(std::integral_constant<int, 3>{});
-                        }
                     const float2 f0 = h2f2(s0[j / 2]), f1 = h2f2(s1[j / 2]);
                     const float a0 = j & 1 ? f0.y : f0.x, a1 = j & 1 ? f1.y : f1.x;
-                    if (LO) {
-                        sc[x][0][0] = fmaf(a0, acc[0] + acc[1], sc[x][0][0]);
-                        sc[x][1][0] = fmaf(a1, acc[2] + acc[3], sc[x][1][0]);
-                    } else {
 #pragma unroll
-                        for (int jj = 0; jj < H; ++jj) {
-                            sc[x][0][jj] = fmaf(a0, acc[jj], sc[x][0][jj]);
-                            sc[x][1][jj] = fmaf(a1, acc[2 + jj], sc[x][1][jj]);
-                        }
+                    for (int jj = 0; jj < H; ++jj) {
+                        const float v0 = LO ? acc[j][0] + acc[j][1] : acc[j][jj], v1 = LO ? acc[j][2] + acc[j][3] : acc[j][2 + jj];
+                        sc[x][0][jj] = j ? fmaf(a0, v0, sc[x][0][jj]) : a0 * v0;
+                        sc[x][1][jj] = j ? fmaf(a1, v1, sc[x][1][jj]) : a1 * v1;
                     }
                 }
-#pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int j = 0; j < H; ++j) {
-                        float v = sc[x][y][j] * cs[j];
-                        if (keys < kKeys && k0 + 8 * y >= keys) v = -INFINITY;
-                        sc[x][y][j] = v;
-                        mx[j] = fmaxf(mx[j], v);
-                    }
             }
-            // largest value scale of the visible keys: two keys a lane
+            if (keys < kKeys) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y)
+                        if (16 * x + key_of<D>(g) + 8 * y >= keys)
+#pragma unroll
+                            for (int j = 0; j < H; ++j) sc[x][y][j] = -INFINITY;
+            }
+            // exponent of the largest value scale: two keys a lane
             uint32_t top;
             {
                 uint32_t w[G];
                 lds(vs + lane * (4 * G), w);
-                uint32_t first = w[0] & 0x7fff7fffu, second = w[G / 2] & 0x7fff7fffu;
-                if (G == 4) {
-                    first = __vmaxu2(first, w[1] & 0x7fff7fffu);
-                    second = __vmaxu2(second, w[G - 1] & 0x7fff7fffu);
-                }
-                if (2 * lane >= keys) first = 0;
-                if (2 * lane + 1 >= keys) second = 0;
-                first = __vmaxu2(first, second);
-                top = __reduce_max_sync(0xffffffffu, max(first & 0xffffu, first >> 16)) >> 10;  // its exponent
+                top = w[0] & 0x7fff7fffu;
+#pragma unroll
+                for (int i = 1; i < G; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
+                top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)) >> 10;
             }
             const int grown = max(int(top) - ev, 0);
             bool moved = grown > 0;
             float corr[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) {
+                float mx = max3(m[j], sc[0][0][j], sc[0][1][j]);
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-                const float mn = fmaxf(m[j], mx[j]);
-                corr[j] = mn == m[j] ? 1.f : exp2_approx(m[j] - mn);
-                moved = moved || mn != m[j];
-                m[j] = mn;
-                l[j] *= corr[j];
+                for (int x = 1; x < 4; ++x) mx = max3(mx, sc[x][0][j], sc[x][1][j]);
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+                corr[j] = mx == m[j] ? 1.f : exp2_approx((m[j] - mx) * cs[j]);
+                moved = moved || mx != m[j];
+                m[j] = mx;
             }
             if (__any_sync(0xffffffffu, moved)) {
                 ev += grown;
@@ -581,6 +601,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
                     const float f = corr[j] * down;
+                    l[j] *= f;
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
                         o[i][j] *= f;
@@ -590,35 +611,24 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                             o[i][3] *= f;
                         }
                     }
-#pragma unroll
-                    for (int i = 0; i < G; ++i) ws[j][i] *= f;
                 }
             }
-            const float wf = pow2(28 - ev);
             float ref[H];
 #pragma unroll
-            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : m[j];
+            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : float(28 - ev) - m[j] * cs[j];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int k0 = 16 * x + key_of<D>(g);
                 uint32_t s0[G / 2], s1[G / 2];
                 lds(vs + k0 * (2 * G), s0);
                 lds(vs + (k0 + 8) * (2 * G), s1);
-                if (keys < kKeys) {
-#pragma unroll
-                    for (int j = 0; j < G / 2; ++j) {
-                        if (k0 >= keys) s0[j] = 0;
-                        if (k0 + 8 >= keys) s1[j] = 0;
-                    }
-                }
                 float p[2][H];
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
 #pragma unroll
                     for (int j = 0; j < H; ++j) {
-                        p[y][j] = exp2_approx(sc[x][y][j] - ref[j]);
+                        p[y][j] = exp2_approx(fmaf(sc[x][y][j], cs[j], ref[j]));
                         l[j] += p[y][j];
-                        p[y][j] *= wf;
                     }
                 uint32_t pb[G][2];
 #pragma unroll
@@ -626,18 +636,9 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const float2 f = h2f2(y ? s1[j / 2] : s0[j / 2]);
-                        const float sv = j & 1 ? f.y : f.x;
-                        const float v0 = p[y][0] * sv;
-                        uint32_t w;
-                        if (LO) {
-                            w = pack_h2(v0, v0 - __half2float(__float2half_rn(v0)));
-                        } else {  // the 1.5 comes off the weights as the product sees them
-                            w = pack_h2(v0, p[y][H - 1] * sv);
-                            const float2 r = h2f2(w);
-                            ws[0][j] += r.x;
-                            ws[H - 1][j] += r.y;
-                        }
-                        pb[j][y] = transpose8x8(w);
+                        const float sv = j & 1 ? f.y : f.x, v0 = p[y][0] * sv;
+                        pb[j][y] = transpose8x8(LO ? pack_h2(v0, v0 - __half2float(__float2half_rn(v0)))
+                                                   : pack_h2(v0, p[y][H - 1] * sv));
                     }
                 // values of keys 2 t, 2 t + 1 and 8 further (as the score rows count them): dimensions of word(s) g
                 uint32_t va[D / 64], vb[D / 64], vc2[D / 64], vd[D / 64];
@@ -646,23 +647,28 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 lds(vc + kb * (D / 2) + g * (D / 16), vb);
                 lds(vc + (ka + 8) * (D / 2) + g * (D / 16), vc2);
                 lds(vc + (kb + 8) * (D / 2) + g * (D / 16), vd);
-                uint32_t lo01[D / 64], hi01[D / 64], lo23[D / 64], hi23[D / 64];  // codes 0-3, 4-7 of two keys
+                // codes 0-3 and 4-7 of two keys in a word, and the same shifted for codes 2, 3 and 6, 7
+                uint32_t lo01[2][D / 64], hi01[2][D / 64], lo23[2][D / 64], hi23[2][D / 64];
 #pragma unroll
                 for (int w = 0; w < D / 64; ++w) {
-                    lo01[w] = __byte_perm(va[w], vb[w], 0x5410);
-                    hi01[w] = __byte_perm(va[w], vb[w], 0x7632);
-                    lo23[w] = __byte_perm(vc2[w], vd[w], 0x5410);
-                    hi23[w] = __byte_perm(vc2[w], vd[w], 0x7632);
+                    lo01[0][w] = __byte_perm(va[w], vb[w], 0x5410);
+                    hi01[0][w] = __byte_perm(va[w], vb[w], 0x7632);
+                    lo23[0][w] = __byte_perm(vc2[w], vd[w], 0x5410);
+                    hi23[0][w] = __byte_perm(vc2[w], vd[w], 0x7632);
+                    lo01[1][w] = lo01[0][w] >> 8;
+                    hi01[1][w] = hi01[0][w] >> 8;
+                    lo23[1][w] = lo23[0][w] >> 8;
+                    hi23[1][w] = hi23[0][w] >> 8;
                 }
                 const auto take = [&](auto ic) {
-                    constexpr int I = decltype(ic)::value;
+                    constexpr int I = decltype(ic)::value, S = I / 2;
                     if constexpr (D == 128) {  // dimensions 16 g + I, 16 g + 8 + I; then the same 4 further
-                        const uint32_t f[4] = {codes2<I, LO>(lo01[0]), codes2<I, LO>(lo01[1]), codes2<I, LO>(lo23[0]), codes2<I, LO>(lo23[1])};
-                        mma16816(o[I], f, pb[I][0], pb[I][1]);
-                        const uint32_t h[4] = {codes2<I, LO>(hi01[0]), codes2<I, LO>(hi01[1]), codes2<I, LO>(hi23[0]), codes2<I, LO>(hi23[1])};
-                        mma16816(o[I + 4], h, pb[I][0], pb[I][1]);
+                        const uint32_t f[4] = {codes2<I>(lo01[S][0]), codes2<I>(lo01[S][1]), codes2<I>(lo23[S][0]), codes2<I>(lo23[S][1])};
+                        mma16816(o[I], f, pb[I % G][0], pb[I % G][1]);
+                        const uint32_t h[4] = {codes2<I>(hi01[S][0]), codes2<I>(hi01[S][1]), codes2<I>(hi23[S][0]), codes2<I>(hi23[S][1])};
+                        mma16816(o[I + 4], h, pb[I % G][0], pb[I % G][1]);
                     } else {  // dimensions 8 g + I, 8 g + 4 + I
-                        const uint32_t f[4] = {codes2<I, LO>(lo01[0]), codes2<I, LO>(hi01[0]), codes2<I, LO>(lo23[0]), codes2<I, LO>(hi23[0])};
+                        const uint32_t f[4] = {codes2<I>(lo01[S][0]), codes2<I>(hi01[S][0]), codes2<I>(lo23[S][0]), codes2<I>(hi23[S][0])};
                         mma16816(o[I], f, pb[I % G][0], pb[I % G][1]);
                     }
                 };
@@ -680,34 +686,26 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
 
         for (; used < issued; ++used)  // after a wait that ran out: copies in flight end before their memory is used
             (void)mbar_wait(&full[warp][used % kStages], (used / kStages) & 1u);
-        // the warp's part: sums over the lanes of a head, then into the warp's own ring (its copies have landed)
-#pragma unroll
-        for (int j = 0; j < H; ++j) {
-#pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
-#pragma unroll
-                for (int i = 0; i < G; ++i) ws[j][i] += __shfl_xor_sync(0xffffffffu, ws[j][i], x);
-            }
-        }
+        // the warp's part: sums over the lanes of a head, then into the warp's own ring (its copies have landed):
+        // [HC][D + 4], accumulator, maximum (times cs), sum
         constexpr int kRec = D + 4;
-        float * const mine = reinterpret_cast<float *>(ring);  // [HC][D + 4]: accumulator, maximum, sum
+        float * const mine = reinterpret_cast<float *>(ring);
         __syncwarp();
-        const float back = 16.f * pow2(ev - 28);
+        const float back = pow2(ev - 28);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
             float * rec = mine + (LO ? t : 2 * t + j) * kRec;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-                const float w = LO ? 0.f : 1.5f * ws[j][i % G];
-                const float v0 = (LO ? o[i][0] + o[i][1] : o[i][j]) - w, v1 = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) - w;
                 const int d = D == 128 ? 16 * g + i : 8 * g + i;
-                rec[d] = v0 * back;
-                rec[d + (D == 128 ? 8 : 4)] = v1 * back;
+                rec[d] = (LO ? o[i][0] + o[i][1] : o[i][j]) * back;
+                rec[d + (D == 128 ? 8 : 4)] = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) * back;
             }
             if (g == 0) {
-                rec[D] = m[j];
-                rec[D + 1] = l[j];
+                rec[D] = m[j] * cs[j];
+                rec[D + 1] = l[j] * back;
             }
         }
         __syncthreads();
@@ -729,7 +727,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 A = fmaf(rec[w * kNext + d], f, A);
             }
             if (whole) {
-                out[row * a.out_stride + i] = from_f32<T>(A / L);
+                out[call_row * a.out_stride + i] = from_f32<T>(A / L);
             } else {
                 part[h * kRec + d] = A;
                 if (d == 0) {
@@ -738,9 +736,6 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 }
             }
         }
-        left -= t1 - t0;
-        off = 0;
-        ++row;
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copies overwrite these records
         __syncthreads();
         if (!__syncthreads_and(ok)) {
@@ -767,22 +762,22 @@ __global__ void __launch_bounds__(kMergeThreads) k_kv4_merge(const Kv4Attn a, in
     const int share_heads = a.heads / a.c.kv_heads, chunk = y % a.chunks;
     const int head = y / a.chunks * share_heads + chunk * HC + h;
     if (chunk * HC + h >= share_heads) return;
-    int n[4], before, total;
-    scan_tiles(a, n, before, total, sm_scan);
+    int n[2], slot[2], before, total;
+    scan_rows(a, n, slot, before, total, sm_scan);
     if (threadIdx.x < 128) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (threadIdx.x * 4 + i == row) {
+        for (int i = 0; i < 2; ++i) {
+            if (threadIdx.x * 2 + i == row) {
                 sm_before = before;
                 sm_n = n[i];
             }
-            before += (max(n[i], 0) + kKeys - 1) / kKeys;
+            before += list_of(n[i]);
         }
         if (threadIdx.x == 0) sm_total = total;
     }
     __syncthreads();
     if (sm_n <= 0) return;
-    const int share = tiles_per_share(sm_total, shares), tiles = (sm_n + kKeys - 1) / kKeys;
+    const int share = share_of(sm_total, shares), tiles = tiles_of(sm_n);
     const int x0 = sm_before / share, parts = (sm_before + tiles - 1) / share - x0 + 1;
     if (parts == 1) return;
     // a CTA's record 0 is the row that it begins and does not end, record 1 the row that it goes on with
@@ -842,7 +837,7 @@ AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
         (void)cudaGetLastError();
     // as many CTAs as are resident together (three per SM), no more than there can be shares
-    const long long most = (long long)rows * (c->max_len / kKeys + kMinShare - 1) / kMinShare;
+    const long long most = ((long long)rows * (c->max_len / kKeys + kRowCost) + kMinShare - 1) / kMinShare;
     p.shares = int(std::max(1ll, std::min((long long)std::min(3 * sms / p.ys, kMaxShares), most)));
     p.scratch = size_t(p.ys) * p.shares * 2 * p.heads_per_cta * (c->head_dim + 4) * sizeof(float);
     return p;
