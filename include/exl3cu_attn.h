@@ -113,6 +113,18 @@ int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void * d_k, size
                        const int32_t * d_kv_end, int n_seq, int q_rows, float scale, void * d_out, size_t out_stride,
                        int out_dtype, void * stream);
 
+/* The calls above for bindings whose conversion of arguments costs more than a launch (ctypes: 24 arguments
+ * about 6 us): `words` are the arguments of the call in order, 8 bytes each; integers and pointers as 64-bit
+ * integers, the floats as doubles. */
+enum exl3cu_attn_call {
+    EXL3CU_CALL_QK_NORM_ROPE = 0,
+    EXL3CU_CALL_KV4_APPEND = 1,
+    EXL3CU_CALL_KV4_READ = 2,
+    EXL3CU_CALL_KV4_ATTN = 3,
+    EXL3CU_CALL_PROMPT_ATTN = 4
+};
+int exl3cu_attn_words(int call, const void * words);
+
 #ifdef __cplusplus
 }
 #endif

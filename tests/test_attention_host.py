@@ -123,7 +123,7 @@ def test_python_refusals():
         A.qk_norm_rope(q, None, pos)
     with pytest.raises(ValueError):
         A.qk_norm_rope(q[0], None, pos)
-    with pytest.raises(TypeError):
+    with pytest.raises((TypeError, ValueError)):
         A.prompt_attention(q, q, q, pos, pos)
     with pytest.raises(ValueError):
         A.Kv4Cache(1, 1, 64, 96)
@@ -148,3 +148,25 @@ def test_rope_frequencies():
     assert np.all(y[turns > 40] == f[turns > 40])                       # fast ones stay
     assert np.allclose(y[turns < 0.8], f[turns < 0.8] / 16, rtol=1e-6)  # slow ones are divided
     assert np.all(np.diff(y) < 0)
+
+
+BY_WORDS = [
+    (0, "PiPiiiiiiPPPfPiifPiiPiiP", ROPE, [dict(dim=96), dict(dtype=2), dict(kot=9), dict(kv=-1), dict(rotary=24), dict(ks=511),
+                                          dict(pos=None), dict(kos=500), dict(heads=2000)]),
+    (4, "PiPiiPiiiiiiiPPPiifPiiP", PROMPT, [dict(dtype=0), dict(ot=4), dict(scale=-1.0), dict(kv_rows=-1), dict(khs=64),
+                                           dict(e=None), dict(out=None), dict(krs=1 << 40)])]
+
+
+@pytest.mark.parametrize("which,kinds,args,bad", BY_WORDS)
+def test_calls_by_words_are_the_calls(L, which, kinds, args, bad):
+    """Every word reaches the parameter of its place: what is refused is refused with the call's own text."""
+    import struct
+
+    fn = (L.exl3cu_qk_norm_rope, None, None, None, L.exl3cu_prompt_attn)[which]
+    for kw in bad + [dict(rows=0)]:
+        values = {**args, **kw}.values()
+        want, text = fn(*values), L.exl3cu_last_error()
+        words = b"".join(struct.pack("=d" if k == "f" else "=q", v or 0) for k, v in zip(kinds, values, strict=True))
+        assert L.exl3cu_attn_words(which, words) == want == (INVALID if kw != dict(rows=0) else 0)
+        assert L.exl3cu_last_error() == text
+    assert L.exl3cu_attn_words(which, None) == INVALID and L.exl3cu_attn_words(9, b"") == INVALID

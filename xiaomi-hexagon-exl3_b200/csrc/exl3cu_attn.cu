@@ -13,6 +13,8 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cstring>
+#include <tuple>
 #include <type_traits>
 
 namespace exl3cu {
@@ -21,11 +23,7 @@ static __device__ unsigned g_attn_status;
 
 namespace {
 
-__device__ __forceinline__ float warp_sum(float v) {
-#pragma unroll
-    for (int s = 16; s; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
-    return v;
-}
+constexpr int kSms = 148;  // a B200's
 
 // ---- query/key norm and rotary embedding ----------------------------------------------------------
 
@@ -54,139 +52,257 @@ __device__ __forceinline__ void rope_angle(int pos, float f, float factor, float
     sn *= factor;
 }
 
-// One warp per (row, head): lane holds dimensions [lane * D/32, +D/32).
+// Four elements, 8 or 16 bytes, as floats.
+template <typename T> __device__ __forceinline__ void load4(const T * p, float * x) {
+    if constexpr (sizeof(T) == 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        const T * e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = to_f32(e[i]);
+    }
+}
+
+__device__ __forceinline__ void store4(void * p, int dtype, long long at, const float * x) {
+    if (dtype == EXL3CU_F32) {
+        *reinterpret_cast<float4 *>(static_cast<float *>(p) + at) = make_float4(x[0], x[1], x[2], x[3]);
+    } else if (dtype == EXL3CU_F16) {
+        const __half2 lo = __floats2half2_rn(x[0], x[1]), hi = __floats2half2_rn(x[2], x[3]);
+        *reinterpret_cast<uint2 *>(static_cast<__half *>(p) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    } else {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
+        *reinterpret_cast<uint2 *>(static_cast<__nv_bfloat16 *>(p) + at) =
+            make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    }
+}
+
+// A CTA takes `rows_per_cta` rows: their angles once for all heads into shared memory, then D/8 threads a head, each
+// with two runs of four dimensions that hold both members of its pairs ((4 j, half + 4 j) or 8 consecutive ones), so
+// that the rotation needs no exchange.  Bound by the bytes of q and k in and out; a call of few rows by latency.
+constexpr int kRopeThreads = 256;
+constexpr int kRopeMaxRows = 8;
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) k_qk_norm_rope(const RopeArgs a) {
+__global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a, int rows_per_cta) {
+    constexpr int L = D / 8;  // threads of a head
+    __shared__ __align__(16) float sm_cos[kRopeMaxRows * (D / 2)], sm_sin[kRopeMaxRows * (D / 2)];
+    __shared__ int sm_pos[kRopeMaxRows];
     pdl_trigger();
+    const int half = a.rotary / 2, j = threadIdx.x % L;
+    const int row0 = blockIdx.x * rows_per_cta, rows = min(rows_per_cta, a.rows - row0);
+    // the thread's two runs of dimensions, and the first of its pairs' frequencies where it rotates
+    int d0 = 8 * j, d1 = 8 * j + 4, f0 = a.interleaved ? 4 * j : -1;
+    if (!a.interleaved && 4 * j < half) d0 = f0 = 4 * j, d1 = half + 4 * j;
+    const bool turns = a.interleaved ? d0 < a.rotary : f0 >= 0;
     pdl_wait_primary();
-    constexpr int E = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    const int per_row = a.heads + a.kv_heads;
-    if (item >= (long long)a.rows * per_row) return;
-    const int r = int(item / per_row), h = int(item % per_row);
-    const int pos = a.row_pos[r];
-    if (pos < 0) return;
-    const bool is_q = h < a.heads;
-    const T * x = static_cast<const T *>(is_q ? a.q : a.k) +
-                  (is_q ? r * a.q_stride + h * D : r * a.k_stride + (h - a.heads) * D);
-    const float * w = is_q ? a.q_w : a.k_w;
-    float v[E];
+    float wq[8], wk[8];
 #pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = to_f32(x[lane * E + i]);
-    if (w) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) ss = fmaf(v[i], v[i], ss);
-        const float inv = rsqrtf(warp_sum(ss) / float(D) + a.eps);
-#pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = v[i] * inv * w[lane * E + i];
+    for (int i = 0; i < 8; ++i) {  // any alignment
+        wq[i] = a.q_w ? a.q_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
+        wk[i] = a.k_w && a.kv_heads ? a.k_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
     }
-    const int half = a.rotary / 2;
-    if (a.interleaved) {
+    for (int i = threadIdx.x; i < rows * half; i += kRopeThreads) {
+        const int r = i / half, f = i - r * half, pos = a.row_pos[row0 + r];
+        float cs, sn;
+        rope_angle(max(pos, 0), a.inv_freq[f], a.factor, cs, sn);
+        sm_cos[r * (D / 2) + f] = cs;
+        sm_sin[r * (D / 2) + f] = sn;
+    }
+    if (threadIdx.x < rows) sm_pos[threadIdx.x] = a.row_pos[row0 + threadIdx.x];
+    __syncthreads();
+    const int per_row = a.heads + a.kv_heads, items = rows * per_row;
+    for (int item = threadIdx.x / L; item < items; item += kRopeThreads / L) {
+        const int r = item / per_row, h = item - r * per_row;
+        const bool is_q = h < a.heads, live = sm_pos[r] >= 0;
+        const long long row = row0 + r;
+        const T * x = is_q ? static_cast<const T *>(a.q) + row * a.q_stride + h * D
+                           : static_cast<const T *>(a.k) + row * a.k_stride + (h - a.heads) * D;
+        float v[8];
+        load4(x + d0, v);
+        load4(x + d1, v + 4);
+        if (is_q ? a.q_w != nullptr : a.k_w != nullptr) {
+            float ss = 0.f;
 #pragma unroll
-        for (int i = 0; i < E; i += 2) {
-            const int d = lane * E + i;
-            if (d < a.rotary) {
-                float cs, sn;
-                rope_angle(pos, a.inv_freq[d >> 1], a.factor, cs, sn);
-                const float x0 = v[i], x1 = v[i + 1];
-                v[i] = x0 * cs - x1 * sn;
-                v[i + 1] = x1 * cs + x0 * sn;
+            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+            const unsigned mask = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1)));
+#pragma unroll
+            for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
+            const float inv = rsqrtf(ss / float(D) + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (is_q ? wq[i] : wk[i]);
+        }
+        if (!live) continue;
+        if (turns) {
+            float cs[4], sn[4];
+            load4(sm_cos + r * (D / 2) + f0, cs);
+            load4(sm_sin + r * (D / 2) + f0, sn);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // interleaved is the same for the whole grid: both forms keep v in registers
+                const float x0 = a.interleaved ? v[2 * i] : v[i], x1 = a.interleaved ? v[2 * i + 1] : v[i + 4];
+                const float y0 = x0 * cs[i] - x1 * sn[i], y1 = x1 * cs[i] + x0 * sn[i];
+                if (a.interleaved) {
+                    v[2 * i] = y0;
+                    v[2 * i + 1] = y1;
+                } else {
+                    v[i] = y0;
+                    v[i + 4] = y1;
+                }
             }
         }
-    } else if (half) {
-        // the partner of dimension d < half is d + half: half / E lanes further on
-        const int shift = half / E;
-        const bool first = lane < shift, second = lane >= shift && lane < 2 * shift;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float up = __shfl_sync(0xffffffffu, v[i], (lane + shift) & 31);
-            const float down = __shfl_sync(0xffffffffu, v[i], (lane - shift) & 31);
-            if (first || second) {
-                const int j = (first ? lane : lane - shift) * E + i;
-                float cs, sn;
-                rope_angle(pos, a.inv_freq[j], a.factor, cs, sn);
-                v[i] = first ? v[i] * cs - up * sn : v[i] * cs + down * sn;
-            }
-        }
-    }
-    const long long at = is_q ? r * a.q_out_stride + h * D : r * a.k_out_stride + (h - a.heads) * D;
-    void * out = is_q ? a.q_out : a.k_out;
-    const int dt = is_q ? a.q_out_dtype : a.k_out_dtype;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const long long p = at + lane * E + i;
-        if (dt == EXL3CU_F32) static_cast<float *>(out)[p] = v[i];
-        else if (dt == EXL3CU_F16) static_cast<__half *>(out)[p] = __float2half_rn(v[i]);
-        else static_cast<__nv_bfloat16 *>(out)[p] = __float2bfloat16_rn(v[i]);
+        void * out = is_q ? a.q_out : a.k_out;
+        const int dt = is_q ? a.q_out_dtype : a.k_out_dtype;
+        const long long at = is_q ? row * a.q_out_stride + h * D : row * a.k_out_stride + (h - a.heads) * D;
+        store4(out, dt, at + d0, v);
+        store4(out, dt, at + d1, v + 4);
     }
 }
 
 // ---- the 4-bit cache -------------------------------------------------------------------------------
 
-// One warp per (row, K or V, head): lane holds dimensions [lane * D/32, +D/32); dimension d is of group
-// d mod G, G = D / 32, so a lane holds one element of every group.
+constexpr int kCacheThreads = 256;
+
+// D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value: one word of codes each.
+// Dimension d is of group d mod G, so a thread holds 8 / G elements of every group, and the largest of a group is
+// taken over the threads by halving the groups that a thread carries.  Bound by the bytes of the rows.
 template <typename T, int D>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kCacheThreads)
 k_kv4_append(const Kv4 c, const T * k, long long k_stride, const T * v, long long v_stride, int rows,
              const int32_t * row_seq, const int32_t * row_pos, const int32_t * seq_slot, int n_seq) {
+    constexpr int G = D / 32, L = D / 8;
     pdl_trigger();
+    const long long item = blockIdx.x * (long long)(kCacheThreads / L) + threadIdx.x / L;
+    const int j = threadIdx.x % L;
+    const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
     pdl_wait_primary();
-    constexpr int G = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    const int per_row = 2 * c.kv_heads;
-    if (item >= (long long)rows * per_row) return;
-    const int r = int(item / per_row), j = int(item % per_row);
-    const bool is_v = j >= c.kv_heads;
-    const int h = is_v ? j - c.kv_heads : j;
-    const int seq = row_seq[r];
-    if (seq < 0 || seq >= n_seq) return;
-    const int slot = seq_slot[seq], pos = row_pos[r];
-    if (slot < 0 || slot >= c.n_slots || pos < 0 || pos >= c.max_len) return;
-    const T * x = (is_v ? v + r * v_stride : k + r * k_stride) + h * D + lane * G;
-    const size_t at = (size_t(slot) * c.kv_heads + h) * c.max_len + pos;
-    uint32_t code[G];
-#pragma unroll
-    for (int g = 0; g < G; ++g) {
-        const float xv = to_f32(x[g]);
-        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(xv) & 0x7fffffffu);
-        const __half s = kv4_scale(most);
-        code[g] = kv4_code(xv, __half2float(s));
-        if (lane == 0) (is_v ? c.v_scales : c.k_scales)[at * G + g] = __half_as_ushort(s);
-    }
-    uint8_t * out = (is_v ? c.v_codes : c.k_codes) + at * (D / 2) + lane * (G / 2);
-#pragma unroll
-    for (int g = 0; g < G; g += 2) out[g / 2] = uint8_t(code[g] | code[g + 1] << 4);
-}
-
-// One warp per (row, head): lane holds dimensions [lane * G, +G) of the key and of the value.
-template <typename T, int D>
-__global__ void __launch_bounds__(128)
-k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n_seq, int total, T * k,
-           long long k_stride, T * v, long long v_stride) {
-    pdl_trigger();
-    pdl_wait_primary();
-    constexpr int G = D / 32;
-    const int lane = threadIdx.x & 31;
-    const long long item = blockIdx.x * 4ll + (threadIdx.x >> 5);
-    if (item >= (long long)total * c.kv_heads) return;
-    const int r = int(item / c.kv_heads), h = int(item % c.kv_heads);
-    const int seq = find_segment(offsets, n_seq, r);
-    if (seq < 0) return;
-    const int slot = seq_slot[seq], pos = r - offsets[seq];
-    const bool ok = slot >= 0 && slot < c.n_slots && pos < c.max_len;
-    const size_t at = ok ? (size_t(slot) * c.kv_heads + h) * c.max_len + pos : 0;
+    if (item >= (long long)rows * c.kv_heads) return;
+    const int r = int(item / c.kv_heads), h = int(item - (long long)r * c.kv_heads);
+    float x[2][8];
+    const T * src[2] = {k + r * k_stride + h * D + 8 * j, v + r * v_stride + h * D + 8 * j};
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        const uint8_t * codes = (w ? c.v_codes : c.k_codes) + at * (D / 2) + lane * (G / 2);
-        const uint16_t * scales = (w ? c.v_scales : c.k_scales) + at * G;
-        T * out = (w ? v + r * v_stride : k + r * k_stride) + h * D + lane * G;
+        load4(src[w], x[w]);
+        load4(src[w] + 4, x[w] + 4);
+    }
+    const int seq = row_seq[r], pos = row_pos[r];
+    if (seq < 0 || seq >= n_seq) return;
+    const int slot = seq_slot[seq];
+    if (slot < 0 || slot >= c.n_slots || pos < 0 || pos >= c.max_len) return;
+    const size_t at = (size_t(slot) * c.kv_heads + h) * c.max_len + pos;
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
-            const int code = (codes[g / 2] >> (4 * (g & 1))) & 15;
-            out[g] = from_f32<T>(ok ? float(code - 8) * __half2float(__ushort_as_half(scales[g])) : 0.f);
+    for (int w = 0; w < 2; ++w) {
+        uint32_t most[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) most[g] = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most[i % G] = max(most[i % G], __float_as_uint(x[w][i]) & 0x7fffffffu);
+        // exchange: after it this thread carries group `mine` over all threads
+        int mine = 0;
+        if constexpr (G == 4) {
+            const bool up = j & (L / 2);
+            const uint32_t a0 = up ? most[0] : most[2], a1 = up ? most[1] : most[3];
+            most[0] = max(up ? most[2] : most[0], __shfl_xor_sync(mask, a0, L / 2));
+            most[1] = max(up ? most[3] : most[1], __shfl_xor_sync(mask, a1, L / 2));
+            mine = up ? 2 : 0;
+        }
+        constexpr int S = G == 4 ? L / 4 : L / 2;
+        const bool up = j & S;
+        uint32_t m = max(up ? most[1] : most[0], __shfl_xor_sync(mask, up ? most[0] : most[1], S));
+        mine += up ? 1 : 0;
+#pragma unroll
+        for (int s = S / 2; s; s >>= 1) m = max(m, __shfl_xor_sync(mask, m, s));
+        const __half half_scale = kv4_scale(m);
+        const float own = __half2float(half_scale);
+        if (!(j & (S - 1))) (w ? c.v_scales : c.k_scales)[at * G + mine] = __half_as_ushort(half_scale);
+        float s[G], inv[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {  // thread g * S of the head carries group g in the order of the halvings
+            s[g] = __shfl_sync(mask, own, g * S, L);
+            inv[g] = __fdividef(1.f, s[g]);
+        }
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= kv4_code(x[w][i], s[i % G], inv[i % G]) << (4 * i);
+        reinterpret_cast<uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j] = word;
+    }
+}
+
+// D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value; kReadRows rows a thread,
+// whose loads are under way together.  Bound by the bytes written.
+constexpr int kReadRows = 4;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kCacheThreads)
+k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n_seq, int total, T * k,
+           long long k_stride, T * v, long long v_stride) {
+    constexpr int G = D / 32, L = D / 8, kDtype = std::is_same_v<T, float> ? EXL3CU_F32 : std::is_same_v<T, __half> ? EXL3CU_F16 : EXL3CU_BF16;
+    pdl_trigger();
+    const int j = threadIdx.x % L;
+    // items of the CTA: (row, head), heads first; a thread's are kCacheThreads / L apart
+    const long long items = (long long)total * c.kv_heads;
+    const long long first = blockIdx.x * (long long)(kReadRows * kCacheThreads / L) + threadIdx.x / L;
+    pdl_wait_primary();
+    if (first >= items) return;
+    int seq = find_segment(offsets, n_seq, int(first / c.kv_heads));
+    const int end = offsets[n_seq];
+    uint32_t codes[kReadRows][2], scales[kReadRows][2][G / 2];
+    int rows[kReadRows], heads[kReadRows];
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+        const long long item = first + u * (kCacheThreads / L);
+        const int r = int(item / c.kv_heads), h = int(item - (long long)r * c.kv_heads);
+        rows[u] = -1;
+        heads[u] = h;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            codes[u][w] = 0x88888888u;
+#pragma unroll
+            for (int g = 0; g < G / 2; ++g) scales[u][w][g] = 0;
+        }
+        if (item >= items || r >= end) continue;
+        if (seq < 0) seq = find_segment(offsets, n_seq, r);
+        if (seq < 0) continue;
+        while (r >= offsets[seq + 1]) ++seq;  // ends: r < offsets[n_seq]
+        rows[u] = r;
+        const int slot = seq_slot[seq], pos = r - offsets[seq];
+        if (slot < 0 || slot >= c.n_slots || pos >= c.max_len) continue;  // zeros
+        const size_t at = (size_t(slot) * c.kv_heads + h) * c.max_len + pos;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            codes[u][w] = reinterpret_cast<const uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j];
+            const uint32_t * s = reinterpret_cast<const uint32_t *>((w ? c.v_scales : c.k_scales) + at * G);
+#pragma unroll
+            for (int g = 0; g < G / 2; ++g) scales[u][w][g] = s[g];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+        if (rows[u] < 0) continue;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            float s[G], x[8];
+#pragma unroll
+            for (int g = 0; g < G; g += 2) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&scales[u][w][g / 2]));
+                s[g] = f.x;
+                s[g + 1] = f.y;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = float(int(codes[u][w] >> (4 * i) & 15u) - 8) * s[i % G];
+            T * out = (w ? v + rows[u] * v_stride : k + rows[u] * k_stride) + heads[u] * D + 8 * j;
+            if constexpr (sizeof(T) == 4) {
+                store4(out, kDtype, 0, x);
+                store4(out, kDtype, 4, x + 4);
+            } else {
+                uint4 q;
+                T * e = reinterpret_cast<T *>(&q);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
+                *reinterpret_cast<uint4 *>(out) = q;
+            }
         }
     }
 }
@@ -785,19 +901,36 @@ __global__ void __launch_bounds__(kMergeThreads) k_kv4_merge(const Kv4Attn a, in
     if constexpr (WIDE) {
         const int h = blockIdx.z, d = threadIdx.x % D, group = threadIdx.x / D;
         if (h >= nh) return;
+        // loads of eight parts at a time, all under way together
         float M = -INFINITY;
-#pragma unroll 8
-        for (int i = threadIdx.x & 31; i < plan.y; i += 32) M = fmaxf(M, rec(i, h)[D]);
+        for (int i0 = threadIdx.x & 31; i0 < plan.y; i0 += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < plan.y ? rec(i0 + 32 * u, h)[D] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) M = fmaxf(M, v[u]);
+        }
 #pragma unroll
         for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
         const float ref = M == -INFINITY ? 0.f : M;
         float L = 0.f, A = 0.f;
-#pragma unroll 8
-        for (int i = group; i < plan.y; i += kGroups) {
-            const float * r = rec(i, h);
-            const float f = exp2_approx(r[D] - ref);
-            L = fmaf(r[D + 1], f, L);
-            A = fmaf(r[d], f, A);
+        for (int i0 = group; i0 < plan.y; i0 += 8 * kGroups) {
+            float vm[8], vl[8], va[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + kGroups * u;
+                const float * r = rec(min(i, plan.y - 1), h);
+                vm[u] = i < plan.y ? r[D] : -INFINITY;
+                vl[u] = r[D + 1];
+                va[u] = r[d];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (i0 + kGroups * u < plan.y) {
+                    const float f = exp2_approx(vm[u] - ref);
+                    L = fmaf(vl[u], f, L);
+                    A = fmaf(va[u], f, A);
+                }
         }
         sm_acc[group][d] = A;
         if (d == 0) sm_l[group] = L;
@@ -813,16 +946,31 @@ __global__ void __launch_bounds__(kMergeThreads) k_kv4_merge(const Kv4Attn a, in
     } else {
         for (int i = threadIdx.x; i < nh * D; i += kMergeThreads) {
             const int h = i / D, d = i % D;
+            // one pass over the parts, four under way together
             float M = -INFINITY, L = 0.f, A = 0.f;
-#pragma unroll 4
-            for (int x = 0; x < plan.y; ++x) M = fmaxf(M, rec(x, h)[D]);
-            const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-            for (int x = 0; x < plan.y; ++x) {
-                const float * r = rec(x, h);
-                const float f = exp2_approx(r[D] - ref);
-                L = fmaf(r[D + 1], f, L);
-                A = fmaf(r[d], f, A);
+            for (int x0 = 0; x0 < plan.y; x0 += 4) {
+                float vm[4], vl[4], va[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float * r = rec(min(x0 + u, plan.y - 1), h);
+                    vm[u] = r[D];
+                    vl[u] = r[D + 1];
+                    va[u] = r[d];
+                }
+                float mn = M;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) mn = fmaxf(mn, vm[u]);
+                const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_approx(M - ref);
+                L *= f0;
+                A *= f0;
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (x0 + u < plan.y) {
+                        const float f = exp2_approx(vm[u] - ref);
+                        L = fmaf(vl[u], f, L);
+                        A = fmaf(va[u], f, A);
+                    }
+                M = mn;
             }
             out[i] = from_f32<T>(A / L);
         }
@@ -844,12 +992,9 @@ AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     p.shares = 0;
     p.scratch = 0;
     if (rows > kSplitRows) return p;
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-        (void)cudaGetLastError();
     // as many CTAs as are resident together (three per SM), no more than there can be shares
     const long long most = ((long long)rows * (c->max_len / kKeys + kRowCost) + kMinShare - 1) / kMinShare;
-    p.shares = int(std::max(1ll, std::min((long long)(3 * sms / p.ys), most)));
+    p.shares = int(std::max(1ll, std::min((long long)(3 * kSms / p.ys), most)));
     p.scratch = kPlanFloats * sizeof(float) + size_t(p.ys) * p.shares * 2 * p.heads_per_cta * (c->head_dim + 4) * sizeof(float);
     return p;
 }
@@ -895,6 +1040,27 @@ Kv4 device_cache(const exl3cu_kv4_cache * c) {
     return Kv4{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->n_slots, c->kv_heads, c->max_len};
 }
 
+// Words of 8 bytes, each read as the kind of the parameter that it becomes.
+struct Words {
+    const char * at;
+    template <typename P> P next() {
+        P v;
+        memcpy(&v, at, 8);
+        at += 8;
+        return v;
+    }
+    operator int() { return int(next<long long>()); }
+    operator size_t() { return next<size_t>(); }
+    operator float() { return float(next<double>()); }
+    template <typename P> operator P *() { return next<P *>(); }
+};
+
+template <typename... A> int call_with_words(int (*f)(A...), const void * words) {
+    Words w{static_cast<const char *>(words)};
+    const std::tuple<A...> args{static_cast<A>(w)...};  // braces: evaluated in order
+    return std::apply(f, args);
+}
+
 constexpr const char * kBadCache =
     "kv4: bad cache (four 16-byte aligned arrays, head_dim 64 or 128, max_len a multiple of 64)";
 
@@ -923,12 +1089,12 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
     const RopeArgs a{d_q, d_k, d_q_out, d_k_out, (long long)q_stride, (long long)k_stride, (long long)q_out_stride,
                      (long long)k_out_stride, d_row_pos, d_q_w, d_k_w, d_inv_freq, eps, attn_factor, rows, heads,
                      kv_heads, rotary_dim, interleaved != 0, q_out_dtype, k_out_dtype};
-    const long long items = (long long)rows * (heads + kv_heads);
-    if (items > (1ll << 32)) return bad("qk_norm_rope: too many rows");
+    // rows of a CTA: one while that leaves SMs without work, then as many as keep eight CTAs an SM
+    const int per_cta = std::max(1, std::min(kRopeMaxRows, rows / (8 * kSms)));
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(head_dim == 128 ? k_qk_norm_rope<T, 128> : k_qk_norm_rope<T, 64>,
-                           dim3(unsigned((items + 3) / 4)), dim3(128), 0, stream, a);
+                           dim3(unsigned((rows + per_cta - 1) / per_cta)), dim3(kRopeThreads), 0, stream, a, per_cta);
     });
 }
 
@@ -944,12 +1110,13 @@ int exl3cu_kv4_append(const exl3cu_kv4_cache * cache, const void * d_k, size_t k
         !rows_ok(d_v, v_stride, width, dtype))
         return bad("kv4_append: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
-    const long long items = 2ll * rows * cache->kv_heads;
-    if (items > (1ll << 32)) return bad("kv4_append: too many rows");
+    const long long per_cta = kCacheThreads / (cache->head_dim / 8);
+    const long long ctas = ((long long)rows * cache->kv_heads + per_cta - 1) / per_cta;
+    if (ctas > 0x7fffffffll) return bad("kv4_append: too many rows");
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_append<T, 128> : k_kv4_append<T, 64>,
-                           dim3(unsigned((items + 3) / 4)), dim3(128), 0, stream, c, static_cast<const T *>(d_k),
+                           dim3(unsigned(ctas)), dim3(kCacheThreads), 0, stream, c, static_cast<const T *>(d_k),
                            (long long)k_stride, static_cast<const T *>(d_v), (long long)v_stride, rows, d_row_seq,
                            d_row_pos, d_seq_slot, n_seq);
     });
@@ -966,12 +1133,13 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
     if (!d_seq_slot || !d_kv_offsets || !rows_ok(d_k, k_stride, width, dtype) || !rows_ok(d_v, v_stride, width, dtype))
         return bad("kv4_read: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
-    const long long items = (long long)total_rows * cache->kv_heads;
-    if (items > (1ll << 32)) return bad("kv4_read: too many rows");
+    const long long per_cta = kReadRows * (kCacheThreads / (cache->head_dim / 8));
+    const long long ctas = ((long long)total_rows * cache->kv_heads + per_cta - 1) / per_cta;
+    if (ctas > 0x7fffffffll) return bad("kv4_read: too many rows");
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_read<T, 128> : k_kv4_read<T, 64>,
-                           dim3(unsigned((items + 3) / 4)), dim3(128), 0, stream, c, d_seq_slot, d_kv_offsets, n_seq,
+                           dim3(unsigned(ctas)), dim3(kCacheThreads), 0, stream, c, d_seq_slot, d_kv_offsets, n_seq,
                            total_rows, static_cast<T *>(d_k), (long long)k_stride, static_cast<T *>(d_v),
                            (long long)v_stride);
     });
@@ -1035,6 +1203,18 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
         };
         return cache->head_dim == 128 ? run(std::integral_constant<int, 128>{}) : run(std::integral_constant<int, 64>{});
     });
+}
+
+int exl3cu_attn_words(int call, const void * words) {
+    if (!words) return bad("attn_words: words is NULL");
+    switch (call) {
+        case EXL3CU_CALL_QK_NORM_ROPE: return call_with_words(exl3cu_qk_norm_rope, words);
+        case EXL3CU_CALL_KV4_APPEND: return call_with_words(exl3cu_kv4_append, words);
+        case EXL3CU_CALL_KV4_READ: return call_with_words(exl3cu_kv4_read, words);
+        case EXL3CU_CALL_KV4_ATTN: return call_with_words(exl3cu_kv4_attn, words);
+        case EXL3CU_CALL_PROMPT_ATTN: return call_with_words(exl3cu_prompt_attn, words);
+        default: return bad("attn_words: unknown call");
+    }
 }
 
 }  // extern "C"

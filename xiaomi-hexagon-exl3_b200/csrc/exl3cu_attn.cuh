@@ -37,12 +37,12 @@ __device__ __forceinline__ __half kv4_scale(uint32_t most_bits) {
     return s > 65504.0f ? __ushort_as_half(0x7bff) : __float2half_ru(s);
 }
 
-// 8 + x / s rounded to the nearest integer, ties to even, from -7 to 7.  The approximate quotient is at
+// 8 + x / s rounded to the nearest integer, ties to even, from -7 to 7; inv about 1 / s.  The approximate quotient is at
 // most one step off; x - t s is exact (t s has 15 bits at most, and t s and x are within a factor of
 // two of one another where t is not zero), and so is its comparison with s / 2.
-__device__ __forceinline__ uint32_t kv4_code(float x, float s) {
+__device__ __forceinline__ uint32_t kv4_code(float x, float s, float inv) {
     if (!(s > 0.f)) return 8u;  // a group of zeros, or a NaN scale
-    float t = rintf(__fdividef(x, s));
+    float t = rintf(x * inv);
     t = fminf(fmaxf(t, -8.f), 8.f);  // saturated groups
     const float d = fmaf(-t, s, x), h = 0.5f * s;
     const bool odd = (int(t) & 1) != 0;

@@ -18,9 +18,9 @@ arguments raise ValueError, TypeError or Exl3InvalidArgument (a ValueError).
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
+import struct
 
 import numpy as np
 import torch
@@ -57,85 +57,129 @@ def _lib():
         for name in ("exl3cu_qk_norm_rope", "exl3cu_kv4_append", "exl3cu_kv4_read", "exl3cu_kv4_attn",
                      "exl3cu_prompt_attn"):
             getattr(L, name).restype = _I
+        L.exl3cu_attn_words.restype = _I
+        L.exl3cu_attn_words.argtypes = [_I, ctypes.c_char_p]
         _L = L
     return _L
 
 
-_HERE = contextlib.nullcontext()
+def _call(which, types):
+    """A call by exl3cu_attn_words: arguments of the given kinds (P: address or None, i: integer, f: float) are
+    packed into words, which takes ctypes a fraction of the time that converting them one by one does."""
+    pack = struct.Struct("=" + "".join("d" if t == "f" else "q" for t in types)).pack
+    entry = None
+
+    def call(*args):
+        nonlocal entry
+        if entry is None:
+            entry = _lib().exl3cu_attn_words
+        status = entry(which, pack(*args))
+        if status:
+            check(status)
+
+    return call
 
 
-def _on(device):
-    """Context in which `device` is the current one."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+_rope_call = _call(0, "PiPiiiiiiPPPfPiifPiiPiiP")
+_append_call = _call(1, "PPiPiiiPPPiP")
+_read_call = _call(2, "PPPiiPiPiiP")
+_attn_call = _call(3, "PPiiiiPPPifPiPiP")
+_prompt_call = _call(4, "PiPiiPiiiiiiiPPPiifPiiP")
 
 
-def _on_stream(call):
-    """A call with stream=s runs as if s were the current stream: what it copies and allocates on the way
-    is ordered with what it launches, and its memory belongs to s."""
+_current_device = torch.cuda.current_device
+if hasattr(torch._C, "_cuda_getDevice"):  # the same without the check that CUDA is initialised: a CUDA tensor exists
+    _current_device = torch._C._cuda_getDevice
+_i32, _f32t, _packed = torch.int32, torch.float32, torch.contiguous_format
+
+
+def _op(call):
+    """An operator's entry.  It runs on the device of its first tensor argument (or of the cache that it is a
+    method of), whatever the current one is.  With stream=s it runs as if s were the current stream: what it
+    copies and allocates on the way is ordered with what it launches, and its memory belongs to s."""
 
     @functools.wraps(call)
-    def wrapper(*args, stream=None, **kw):
-        if stream is None:
-            return call(*args, **kw)
-        if not hasattr(stream, "cuda_stream"):
-            stream = torch.cuda.ExternalStream(int(stream))
-        with torch.cuda.stream(stream):
-            return call(*args, **kw)
+    def wrapper(first, *args, stream=None, **kw):
+        if stream is not None:
+            if not hasattr(stream, "cuda_stream"):
+                stream = torch.cuda.ExternalStream(int(stream))
+            with torch.cuda.stream(stream):
+                return wrapper(first, *args, **kw)
+        index = first.get_device()
+        if index < 0:
+            raise ValueError("operands must be on a CUDA device")
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return call(first, *args, **kw)
+        return call(first, *args, **kw)
 
     return wrapper
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
 
 
-def _heads(name, t, device=None, dtype=None):
-    """`t` as [rows, heads, head_dim] with contiguous heads and 16-byte aligned rows; its row stride."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [rows, heads, head_dim]")
-    if t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype):
-        raise TypeError(f"{name} must be float32, float16 or bfloat16, and q, k and v of one type")
-    if not t.is_cuda or (device is not None and t.device != device):
-        raise ValueError(f"{name} must be on the CUDA device of the other operands")
+if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a Stream object around it
+    _stream = torch._C._cuda_getCurrentRawStream
+
+
+def _heads(name, t, index, dtype):
+    """`t` as [rows, heads, head_dim] with contiguous heads and 16-byte aligned rows: the tensor (a copy where
+    that is needed, to be kept until the launch), its address and its row stride."""
+    if t.dtype is not dtype or t.dim() != 3 or t.get_device() != index:
+        if t.dim() != 3:
+            raise ValueError(f"{name} must be [rows, heads, head_dim]")
+        if t.get_device() != index:
+            raise ValueError(f"{name} must be on the CUDA device of the other operands")
+        raise TypeError(f"{name} must be of the other operands' type")
     rows, heads, dim = t.shape
-    s = t.stride()
-    if (s[2] != 1 or (s[1] != dim and heads != 1) or (rows > 1 and s[0] < heads * dim)
-            or (rows > 1 and s[0] * t.element_size() % 16) or t.data_ptr() % 16):
+    s0, s1, s2 = t.stride()
+    ptr, width = t.data_ptr(), heads * dim
+    if rows <= 1:
+        s0 = width
+    if s2 != 1 or (s1 != dim and heads != 1) or s0 < width or s0 * t.element_size() % 16 or ptr % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        s = t.stride()
-    return t, (s[0] if rows > 1 else heads * dim)
+        ptr, s0 = t.data_ptr(), width
+    return t, ptr, s0
 
 
-def _into(name, t, rows, heads, dim, device, dtypes):
+def _into(name, t, rows, heads, dim, index, dtypes):
     """A caller's output: [rows, heads, dim] with contiguous heads, never copied; its row stride."""
-    if tuple(t.shape) != (rows, heads, dim) or t.device != device:
-        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}] on {device}")
+    if t.shape != (rows, heads, dim) or t.get_device() != index:
+        raise ValueError(f"{name} must be [{rows}, {heads}, {dim}] on the device of the other operands")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has an unsupported type {t.dtype}")
-    s = t.stride()
-    if rows and (s[2] != 1 or (s[1] != dim and heads != 1) or (rows > 1 and s[0] < heads * dim)):
+    s0, s1, s2 = t.stride()
+    if rows <= 1:
+        s0 = heads * dim
+    if rows and (s2 != 1 or (s1 != dim and heads != 1) or s0 < heads * dim):
         raise ValueError(f"{name} must have contiguous heads and rows that do not overlap")
-    return s[0] if rows > 1 else heads * dim
+    return s0
 
 
-def _index(name, t, count, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.device != device:
-        raise ValueError(f"{name} must be a 1-D int32 tensor on {device}")
-    if count is not None and t.shape[0] != count:
-        raise ValueError(f"{name} must have {count} entries")
-    if t.shape[0] > 1 and t.stride(0) != 1:
-        raise ValueError(f"{name} must be contiguous")
+def _index(name, t, count, index):
+    """Address of a contiguous int32 tensor of `count` entries."""
+    if t.dtype is not _i32 or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {count} on the device of the other operands")
     return t.data_ptr()
 
 
-def _f32(name, t, count, device):
+def _f32(name, t, count, index):
     if t is None:
-        return None
-    if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != count or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous float32 tensor of {count} on {device}")
+        return 0
+    if t.dtype is not _f32t or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous float32 tensor of {count} on the device of the other operands")
     return t.data_ptr()
+
+
+def _known(name, dtype):
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16")
+    return code
 
 
 def rope_frequencies(rotary_dim: int, theta: float = 1e4, factor: float = 1.0, original_len: int = 0,
@@ -162,7 +206,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e4, factor: float = 1.0, o
     return (f / factor * ramp + f * (1 - ramp)).astype(np.float32), float(0.1 * np.log(factor) + 1.0)
 
 
-@_on_stream
+@_op
 def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, *, eps: float = 1e-6,
                  interleaved: bool = False, attention_factor: float = 1.0, q_out=None, k_out=None, out_dtype=None):
     """Per-head RMSNorm (where weights are given) and rotary embedding of q [rows, heads, D] and k
@@ -171,32 +215,36 @@ def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, *
     positions: int32 [rows]; rows of a negative position are not written.  inv_freq: float32
     [rotary_dim / 2] (rope_frequencies), or None for no rotation.  q_out / k_out may be q / k
     themselves, or of another of the three types; out_dtype is the type of outputs allocated here."""
-    L = _lib()
-    dev = q.device
-    q, qs = _heads("q", q)
+    index, dtype = q.get_device(), q.dtype
+    code = _known("q", dtype)
+    q, qp, qs = _heads("q", q, index, dtype)
     rows, heads, dim = q.shape
+    kv, kp, ks, kop, kos, kcode = 0, 0, 0, 0, 0, 0
     if k is not None:
-        k, ks = _heads("k", k, dev, q.dtype)
-        if k.shape[0] != rows or k.shape[2] != dim:
-            raise ValueError("k must have q's rows and head_dim")
+        k, kp, ks = _heads("k", k, index, dtype)
         kv = k.shape[1]
-    else:
-        kv, ks = 0, 0
-    pos = _index("positions", positions, rows, dev)
+        if k.shape != (rows, kv, dim):
+            raise ValueError("k must have q's rows and head_dim")
     rotary = 0 if inv_freq is None else 2 * inv_freq.shape[0]
-    freq = _f32("inv_freq", inv_freq, rotary // 2, dev)
-    qw, kw = _f32("q_weight", q_weight, dim, dev), _f32("k_weight", k_weight, dim, dev)
     if q_out is None:
-        q_out = torch.empty((rows, heads, dim), dtype=out_dtype or q.dtype, device=dev)
-    qos = _into("q_out", q_out, rows, heads, dim, dev, _DTYPES)
-    if kv and k_out is None:
-        k_out = torch.empty((rows, kv, dim), dtype=out_dtype or q.dtype, device=dev)
-    kos = _into("k_out", k_out, rows, kv, dim, dev, _DTYPES) if kv else 0
-    with _on(dev):
-        check(L.exl3cu_qk_norm_rope(q.data_ptr(), qs, k.data_ptr() if kv else None, ks, _DTYPES[q.dtype], rows, heads,
-                                    kv, dim, pos, qw, kw, eps, freq, rotary, int(interleaved), attention_factor,
-                                    q_out.data_ptr(), qos, _DTYPES[q_out.dtype], k_out.data_ptr() if kv else None, kos,
-                                    _DTYPES[k_out.dtype] if kv else 0, _stream(dev)))
+        q_out = torch.empty_like(q, dtype=out_dtype, memory_format=_packed)
+        qos = heads * dim
+        qcode = _known("out_dtype", q_out.dtype)
+    else:
+        qos = _into("q_out", q_out, rows, heads, dim, index, _DTYPES)
+        qcode = _DTYPES[q_out.dtype]
+    if kv:
+        if k_out is None:
+            k_out = torch.empty_like(k, dtype=out_dtype, memory_format=_packed)
+            kos = kv * dim
+        else:
+            kos = _into("k_out", k_out, rows, kv, dim, index, _DTYPES)
+        kop, kcode = k_out.data_ptr(), _known("k_out", k_out.dtype)
+    _rope_call(qp, qs, kp, ks, code, rows, heads, kv, dim,
+               _index("positions", positions, rows, index), _f32("q_weight", q_weight, dim, index),
+               _f32("k_weight", k_weight, dim, index), eps,
+               _f32("inv_freq", inv_freq, rotary // 2, index), rotary, bool(interleaved),
+               attention_factor, q_out.data_ptr(), qos, qcode, kop, kos, kcode, _stream(index))
     return q_out, k_out
 
 
@@ -238,101 +286,117 @@ class Kv4Cache:
         self._c = _Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), slots, kv,
                          max_len, 2 * half)
         self._ref = ctypes.pointer(self._c)
+        self._at = ctypes.addressof(self._c)
+        self._index = k_codes.get_device()
+        self._scratch = {}  # attend()'s scratch bytes by (rows, heads): a function of the cache's shape
 
-    @_on_stream
+    def get_device(self) -> int:
+        """Index of the cache's CUDA device."""
+        return self._index
+
+    @_op
     def append(self, k, v, row_seq, row_pos, seq_slot) -> None:
         """Quantise rows k, v [rows, kv_heads, D] into (seq_slot[row_seq], row_pos) (exl3cu_kv4_append).
         Rows outside the cache (a position, slot or sequence out of range) are skipped."""
-        L = _lib()
-        dev = self.device
-        k, ks = _heads("k", k, dev)
-        v, vs = _heads("v", v, dev, k.dtype)
-        rows = k.shape[0]
-        if tuple(k.shape[1:]) != (self.kv_heads, self.head_dim) or v.shape != k.shape:
+        index, dtype = self._index, k.dtype
+        code = _known("k", dtype)
+        k, kp, ks = _heads("k", k, index, dtype)
+        v, vp, vs = _heads("v", v, index, dtype)
+        rows, n = k.shape[0], seq_slot.shape[0]
+        if k.shape != (rows, self.kv_heads, self.head_dim) or v.shape != k.shape:
             raise ValueError(f"k and v must be [rows, {self.kv_heads}, {self.head_dim}]")
-        with _on(dev):
-            check(L.exl3cu_kv4_append(self._ref, k.data_ptr(), ks, v.data_ptr(), vs, _DTYPES[k.dtype], rows,
-                                      _index("row_seq", row_seq, rows, dev), _index("row_pos", row_pos, rows, dev),
-                                      _index("seq_slot", seq_slot, None, dev), seq_slot.shape[0], _stream(dev)))
+        _append_call(self._at, kp, ks, vp, vs, code, rows, _index("row_seq", row_seq, rows, index),
+                     _index("row_pos", row_pos, rows, index),
+                     _index("seq_slot", seq_slot, n, index), n, _stream(index))
 
-    @_on_stream
+    @_op
     def read(self, seq_slot, kv_offsets, total_rows: int, dtype=torch.float16, k_out=None, v_out=None):
         """Positions 0 .. kv_offsets[s+1] - kv_offsets[s] of each sequence's slot as packed rows
         [total_rows, kv_heads, D] of `dtype` (exl3cu_kv4_read); returns (k, v).  Rows from kv_offsets[-1]
         on are left as they were (undefined where allocated here)."""
-        L = _lib()
-        dev = self.device
-        n = seq_slot.shape[0]
+        index, n = self._index, seq_slot.shape[0]
         if k_out is None or v_out is None:
-            if dtype not in _DTYPES:
-                raise TypeError("dtype must be float32, float16 or bfloat16")
+            for t in (k_out, v_out):
+                dtype = dtype if t is None else t.dtype
+            _known("dtype", dtype)
             shape = (total_rows, self.kv_heads, self.head_dim)
-            if k_out is None:
-                k_out = torch.empty(shape, dtype=dtype if v_out is None else v_out.dtype, device=dev)
-            if v_out is None:
-                v_out = torch.empty(shape, dtype=k_out.dtype, device=dev)
-        ks = _into("k_out", k_out, total_rows, self.kv_heads, self.head_dim, dev, _DTYPES)
-        vs = _into("v_out", v_out, total_rows, self.kv_heads, self.head_dim, dev, (k_out.dtype,))
-        with _on(dev):
-            check(L.exl3cu_kv4_read(self._ref, _index("seq_slot", seq_slot, None, dev),
-                                    _index("kv_offsets", kv_offsets, n + 1, dev), n, total_rows, k_out.data_ptr(), ks,
-                                    v_out.data_ptr(), vs, _DTYPES[k_out.dtype], _stream(dev)))
+            k_out = torch.empty(shape, dtype=dtype, device=self.device) if k_out is None else k_out
+            v_out = torch.empty(shape, dtype=dtype, device=self.device) if v_out is None else v_out
+        ks = _into("k_out", k_out, total_rows, self.kv_heads, self.head_dim, index, _DTYPES)
+        vs = _into("v_out", v_out, total_rows, self.kv_heads, self.head_dim, index, (k_out.dtype,))
+        _read_call(self._at, _index("seq_slot", seq_slot, n, index),
+                   _index("kv_offsets", kv_offsets, n + 1, index), n, total_rows,
+                   k_out.data_ptr(), ks, v_out.data_ptr(), vs, _DTYPES[k_out.dtype],
+                   _stream(index))
         return k_out, v_out
 
+    @_op
     def scratch_bytes(self, rows: int, heads: int) -> int:
         """Scratch that attend() needs for `rows` rows of `heads` query heads."""
-        with _on(self.device):
-            return _lib().exl3cu_kv4_attn_scratch_bytes(self._ref, rows, heads)
+        key = (rows, heads)
+        need = self._scratch.get(key)
+        if need is None:
+            need = self._scratch[key] = _lib().exl3cu_kv4_attn_scratch_bytes(self._ref, rows, heads)
+        return need
 
-    @_on_stream
+    @_op
     def attend(self, q, row_seq, row_pos, seq_slot, scale: float | None = None, out=None, scratch=None):
         """Attention of rows q [rows, heads, D] over positions 0 .. row_pos of their slots
         (exl3cu_kv4_attn); scale defaults to 1/sqrt(D).  scratch: a uint8 tensor of scratch_bytes() that
         no other call uses at the same time; allocated per call when not given."""
-        L = _lib()
-        dev = self.device
-        q, qs = _heads("q", q, dev)
+        index, dtype = self._index, q.dtype
+        code = _known("q", dtype)
+        q, qp, qs = _heads("q", q, index, dtype)
         rows, heads, dim = q.shape
+        n = seq_slot.shape[0]
         if dim != self.head_dim or heads % self.kv_heads:
             raise ValueError(f"q must be [rows, a multiple of {self.kv_heads}, {self.head_dim}]")
         if out is None:
-            out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-        os_ = _into("out", out, rows, heads, dim, dev, (q.dtype,))
-        with _on(dev):
-            if scratch is None:
-                need = L.exl3cu_kv4_attn_scratch_bytes(self._ref, rows, heads)
-                if need:
-                    scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-            elif scratch.device != dev or not scratch.is_contiguous():
-                raise ValueError(f"scratch must be contiguous memory of {dev}")
-            check(L.exl3cu_kv4_attn(self._ref, q.data_ptr(), qs, _DTYPES[q.dtype], rows, heads,
-                                    _index("row_seq", row_seq, rows, dev), _index("row_pos", row_pos, rows, dev),
-                                    _index("seq_slot", seq_slot, None, dev), seq_slot.shape[0],
-                                    dim ** -0.5 if scale is None else scale, out.data_ptr(), os_,
-                                    scratch.data_ptr() if scratch is not None else None,
-                                    scratch.numel() * scratch.element_size() if scratch is not None else 0,
-                                    _stream(dev)))
+            out, os_ = torch.empty_like(q, memory_format=_packed), heads * dim
+        else:
+            os_ = _into("out", out, rows, heads, dim, index, (dtype,))
+        if scratch is None:
+            need = self._scratch.get((rows, heads))
+            if need is None:
+                need = self.scratch_bytes(rows, heads)
+            if need:
+                scratch = self.k_codes.new_empty(need)
+            held = need
+        else:
+            held = scratch.numel() * scratch.element_size()
+            if scratch.get_device() != index or not scratch.is_contiguous():
+                raise ValueError("scratch must be contiguous memory of the cache's device")
+        _attn_call(self._at, qp, qs, code, rows, heads, _index("row_seq", row_seq, rows, index),
+                   _index("row_pos", row_pos, rows, index),
+                   _index("seq_slot", seq_slot, n, index), n,
+                   dim ** -0.5 if scale is None else scale, out.data_ptr(), os_,
+                   scratch.data_ptr() if held else 0, held, _stream(index))
         return out
 
 
-def _kv(name, t, device, dtype, shape):
-    """k or v [rows, kv_heads, D] with any row and head strides that are multiples of 16 bytes."""
-    if t.dim() != 3 or t.shape[2] != shape[2] or (shape[1] and t.shape[1] != shape[1]):
-        raise ValueError(f"{name} must be [rows, kv_heads, head_dim], k and v alike")
-    if t.dtype != dtype or t.device != device:
+def _kv(name, t, index, dtype, dim):
+    """k or v [rows, kv_heads, D] with any row and head strides that are multiples of 16 bytes: the tensor (or
+    its copy), address, row and head strides."""
+    if t.dim() != 3 or t.shape[2] != dim:
+        raise ValueError(f"{name} must be [rows, kv_heads, {dim}]")
+    if t.dtype is not dtype or t.get_device() != index:
         raise TypeError(f"{name} must have q's type and device")
+    rows, heads, _ = t.shape
     rs, hs, ds = t.stride()
-    dim = t.shape[2]
-    rs, hs = rs if t.shape[0] > 1 else t.shape[1] * dim, hs if t.shape[1] > 1 else dim
-    if ds != 1 or rs % 8 or hs % 8 or rs < dim or hs < dim or t.data_ptr() % 16:
+    ptr = t.data_ptr()
+    if rows <= 1:
+        rs = heads * dim
+    if heads <= 1:
+        hs = dim
+    if ds != 1 or rs % 8 or hs % 8 or rs < dim or hs < dim or ptr % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        rs, hs = t.shape[1] * dim, dim
-    return t, rs, hs
+        ptr, rs, hs = t.data_ptr(), heads * dim, dim
+    return t, ptr, rs, hs
 
 
-@_on_stream
+@_op
 def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_end=None, scale: float | None = None,
                      out=None):
     """Causal attention of packed sequences (exl3cu_prompt_attn): q [q_rows, heads, D], k and v
@@ -341,36 +405,34 @@ def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_e
     slot cache).  Its last query sees all of its keys, the one before all but the last, and so on; a query
     that sees none becomes zero.  out may be float32 or of q's type; query rows outside every sequence are
     left as they were (undefined where out is allocated here)."""
-    L = _lib()
-    dev = q.device
-    if q.dtype == torch.float32:
+    index, dtype = q.get_device(), q.dtype
+    if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError("q, k and v must be float16 or bfloat16")
-    q, qs = _heads("q", q)
+    q, qp, qs = _heads("q", q, index, dtype)
     rows, heads, dim = q.shape
-    k, krs, khs = _kv("k", k, dev, q.dtype, (0, 0, dim))
-    v, vrs, vhs = _kv("v", v, dev, q.dtype, k.shape)
-    if v.shape[0] != k.shape[0]:
-        raise ValueError("k and v must have the same rows")
+    k, kp, krs, khs = _kv("k", k, index, dtype, dim)
+    v, vp, vrs, vhs = _kv("v", v, index, dtype, dim)
+    if v.shape != k.shape:
+        raise ValueError("k and v must have the same shape")
     if kv_offsets is not None:
         if kv_begin is not None or kv_end is not None:
             raise ValueError("give kv_offsets, or kv_begin and kv_end")
-        n = kv_offsets.shape[0] - 1
-        begin = _index("kv_offsets", kv_offsets, None, dev)
+        n = q_offsets.shape[0] - 1
+        begin = _index("kv_offsets", kv_offsets, n + 1, index)
         end = begin + 4
     else:
         if kv_begin is None or kv_end is None:
             raise ValueError("give kv_offsets, or kv_begin and kv_end")
         n = kv_begin.shape[0]
-        begin, end = _index("kv_begin", kv_begin, None, dev), _index("kv_end", kv_end, n, dev)
+        begin, end = _index("kv_begin", kv_begin, n, index), _index("kv_end", kv_end, n, index)
     if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=dev)
-    os_ = _into("out", out, rows, heads, dim, dev, (q.dtype, torch.float32))
-    with _on(dev):
-        check(L.exl3cu_prompt_attn(q.data_ptr(), qs, k.data_ptr(), krs, khs, v.data_ptr(), vrs, vhs, k.shape[0],
-                                   _DTYPES[q.dtype], heads, k.shape[1], dim,
-                                   _index("q_offsets", q_offsets, n + 1, dev), begin, end, n, rows,
-                                   dim ** -0.5 if scale is None else scale, out.data_ptr(), os_, _DTYPES[out.dtype],
-                                   _stream(dev)))
+        out, os_ = torch.empty_like(q, memory_format=_packed), heads * dim
+    else:
+        os_ = _into("out", out, rows, heads, dim, index, (dtype, torch.float32))
+    _prompt_call(qp, qs, kp, krs, khs, vp, vrs, vhs, k.shape[0], _DTYPES[dtype], heads,
+                 k.shape[1], dim, _index("q_offsets", q_offsets, n + 1, index), begin, end, n,
+                 rows, dim ** -0.5 if scale is None else scale, out.data_ptr(), os_,
+                 _DTYPES[out.dtype], _stream(index))
     return out
 
 
