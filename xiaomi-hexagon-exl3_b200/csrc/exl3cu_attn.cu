@@ -25,6 +25,60 @@ namespace {
 
 constexpr int kSms = 148;  // a B200's
 
+// The largest of three, a NaN if one is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+
+// Constants of codes2 in registers: an instruction takes one immediate, and these need two.
+struct CodeConst {
+    uint32_t magic, sixteenth, minus72;
+    __device__ __forceinline__ CodeConst() {
+        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
+        asm volatile("mov.b32 %0, 0x2c002c00;" : "=r"(sixteenth));
+        asm volatile("mov.b32 %0, 0xd480d480;" : "=r"(minus72));
+    }
+};
+
+// Halves c - 8 of codes i and i + 4 of a word, i = 0 .. 3, from the word for i < 2 and from the word shifted right
+// by 8 for i >= 2: the code's bits in the mantissa of 1024 make 1024 + c (or, 4 bits up, 1024 + 16 c).
+template <int i> __device__ __forceinline__ uint32_t codes2(uint32_t w, const CodeConst & k) {
+    uint32_t x, y;
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "r"(i & 1 ? 0x00f000f0u : 0x000f000fu), "r"(k.magic));
+    if (i & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(k.sixteenth), "r"(k.minus72));
+    else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));  // - 1032
+    return y;
+}
+
+__device__ __forceinline__ float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+
+// N elements from 16-byte aligned memory.
+template <int N, typename T> __device__ __forceinline__ void load_row(const T * p, float (&x)[N]) {
+    constexpr int V = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; i += V) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p + i);
+        const T * e = reinterpret_cast<const T *>(&v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[i + j] = to_f32(e[j]);
+    }
+}
+
+// W words of 4 bytes (1, 2 or 4) from shared memory.
+template <int W> __device__ __forceinline__ void lds(const unsigned char * p, uint32_t (&w)[W]) {
+    if constexpr (W == 4) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2 *>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
 // ---- query/key norm and rotary embedding ----------------------------------------------------------
 
 struct RopeArgs {
@@ -81,13 +135,16 @@ __device__ __forceinline__ void store4(void * p, int dtype, long long at, const 
 
 // A CTA takes `rows_per_cta` rows: their angles once for all heads into shared memory, then D/8 threads a head, each
 // with two runs of four dimensions that hold both members of its pairs ((4 j, half + 4 j) or 8 consecutive ones), so
-// that the rotation needs no exchange.  Bound by the bytes of q and k in and out; a call of few rows by latency.
-constexpr int kRopeThreads = 256;
-constexpr int kRopeMaxRows = 8;
+// that the rotation needs no exchange; a thread's next head is loaded while it works on one.  Bound by the bytes of q
+// and k in and out; a call of few rows by latency.
+constexpr int kRopeThreads = 128;
+constexpr int kRopeMaxRows = 4;
 
-template <typename T, int D>
+// SAME: the outputs are of the inputs' type.
+template <typename T, int D, bool SAME>
 __global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a, int rows_per_cta) {
-    constexpr int L = D / 8;  // threads of a head
+    constexpr int L = D / 8, kStep = kRopeThreads / L;  // threads of a head, heads at a time
+    constexpr int kType = std::is_same_v<T, float> ? EXL3CU_F32 : std::is_same_v<T, __half> ? EXL3CU_F16 : EXL3CU_BF16;
     __shared__ __align__(16) float sm_cos[kRopeMaxRows * (D / 2)], sm_sin[kRopeMaxRows * (D / 2)];
     __shared__ int sm_pos[kRopeMaxRows];
     pdl_trigger();
@@ -97,65 +154,85 @@ __global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a,
     int d0 = 8 * j, d1 = 8 * j + 4, f0 = a.interleaved ? 4 * j : -1;
     if (!a.interleaved && 4 * j < half) d0 = f0 = 4 * j, d1 = half + 4 * j;
     const bool turns = a.interleaved ? d0 < a.rotary : f0 >= 0;
+    const int per_row = a.heads + a.kv_heads;
+    int r = 0, h = threadIdx.x / L;  // h < per_row after this
+    const auto settle = [&] {
+        while (h >= per_row) {
+            h -= per_row;
+            ++r;
+        }
+    };
+    const auto load = [&](float * v) {
+        const long long row = row0 + r;
+        const T * x = h < a.heads ? static_cast<const T *>(a.q) + row * a.q_stride + h * D
+                                  : static_cast<const T *>(a.k) + row * a.k_stride + (h - a.heads) * D;
+        load4(x + d0, v);
+        load4(x + d1, v + 4);
+    };
+    settle();
     pdl_wait_primary();
+    float next[8];
+    if (r < rows) load(next);
+    if (threadIdx.x < rows) sm_pos[threadIdx.x] = a.row_pos[row0 + threadIdx.x];
+    for (int i = threadIdx.x; i < rows * half; i += kRopeThreads) {
+        const int ar = i / half, f = i - ar * half, pos = a.row_pos[row0 + ar];
+        float cs, sn;
+        rope_angle(max(pos, 0), a.inv_freq[f], a.factor, cs, sn);
+        sm_cos[ar * (D / 2) + f] = cs;
+        sm_sin[ar * (D / 2) + f] = sn;
+    }
     float wq[8], wk[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {  // any alignment
         wq[i] = a.q_w ? a.q_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
         wk[i] = a.k_w && a.kv_heads ? a.k_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
     }
-    for (int i = threadIdx.x; i < rows * half; i += kRopeThreads) {
-        const int r = i / half, f = i - r * half, pos = a.row_pos[row0 + r];
-        float cs, sn;
-        rope_angle(max(pos, 0), a.inv_freq[f], a.factor, cs, sn);
-        sm_cos[r * (D / 2) + f] = cs;
-        sm_sin[r * (D / 2) + f] = sn;
-    }
-    if (threadIdx.x < rows) sm_pos[threadIdx.x] = a.row_pos[row0 + threadIdx.x];
+    const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
     __syncthreads();
-    const int per_row = a.heads + a.kv_heads, items = rows * per_row;
-    for (int item = threadIdx.x / L; item < items; item += kRopeThreads / L) {
-        const int r = item / per_row, h = item - r * per_row;
-        const bool is_q = h < a.heads, live = sm_pos[r] >= 0;
-        const long long row = row0 + r;
-        const T * x = is_q ? static_cast<const T *>(a.q) + row * a.q_stride + h * D
-                           : static_cast<const T *>(a.k) + row * a.k_stride + (h - a.heads) * D;
+    while (r < rows) {
+        const int now_r = r, now_h = h;
         float v[8];
-        load4(x + d0, v);
-        load4(x + d1, v + 4);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = next[i];
+        h += kStep;
+        settle();
+        if (r < rows) load(next);
+        const bool is_q = now_h < a.heads;
         if (is_q ? a.q_w != nullptr : a.k_w != nullptr) {
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-            const unsigned mask = (L == 32 ? 0xffffffffu : ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1)));
 #pragma unroll
             for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
-            const float inv = rsqrtf(ss / float(D) + a.eps);
+            const float inv = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (is_q ? wq[i] : wk[i]);
         }
-        if (!live) continue;
         if (turns) {
             float cs[4], sn[4];
-            load4(sm_cos + r * (D / 2) + f0, cs);
-            load4(sm_sin + r * (D / 2) + f0, sn);
+            load4(sm_cos + now_r * (D / 2) + f0, cs);
+            load4(sm_sin + now_r * (D / 2) + f0, sn);
+            if (a.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // interleaved is the same for the whole grid: both forms keep v in registers
-                const float x0 = a.interleaved ? v[2 * i] : v[i], x1 = a.interleaved ? v[2 * i + 1] : v[i + 4];
-                const float y0 = x0 * cs[i] - x1 * sn[i], y1 = x1 * cs[i] + x0 * sn[i];
-                if (a.interleaved) {
-                    v[2 * i] = y0;
-                    v[2 * i + 1] = y1;
-                } else {
-                    v[i] = y0;
-                    v[i + 4] = y1;
+                for (int i = 0; i < 4; ++i) {
+                    const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                    v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                    v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float x0 = v[i], x1 = v[i + 4];
+                    v[i] = x0 * cs[i] - x1 * sn[i];
+                    v[i + 4] = x1 * cs[i] + x0 * sn[i];
                 }
             }
         }
+        if (sm_pos[now_r] < 0) continue;
+        const long long row = row0 + now_r;
         void * out = is_q ? a.q_out : a.k_out;
-        const int dt = is_q ? a.q_out_dtype : a.k_out_dtype;
-        const long long at = is_q ? row * a.q_out_stride + h * D : row * a.k_out_stride + (h - a.heads) * D;
+        const int dt = SAME ? kType : is_q ? a.q_out_dtype : a.k_out_dtype;
+        const long long at = is_q ? row * a.q_out_stride + now_h * D : row * a.k_out_stride + (now_h - a.heads) * D;
         store4(out, dt, at + d0, v);
         store4(out, dt, at + d1, v + 4);
     }
@@ -165,29 +242,60 @@ __global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a,
 
 constexpr int kCacheThreads = 256;
 
+// Scaled codes of one thread's 8 dimensions (dimension i of group i mod G) as a word; inv = 1 / s within an ulp or two,
+// 0 where s is 0.  A sum with 1.5 * 2^23 + 8 rounds to the nearest integer, ties to even, and leaves the code in its low
+// bits; the constant high bits come off the assembled word at once.
+//   x of 16 bits: x / s differs from a tie (n + 1/2) by at least 2^-16 unless it is one, since x has 11 bits and
+//   (n + 1/2) s at most 15; rounding the approximate quotient (off by 2^-20 at most) to multiples of 2^-18 first, by a
+//   sum with 48, makes ties exact and moves nothing else across one.
+//   f32: the remainder x - t s is exact; where it reaches half a step (a tie, or the quotient's error) the exact
+//   comparison of kv4_code decides.
+template <typename T, int G>
+__device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], const float (&s)[G], const float (&inv)[G]) {
+    constexpr float kMagic = 12582912.f + 8.f;
+    constexpr uint32_t kHigh = 0x4b400000u;  // the bits of 1.5 * 2^23
+    uint32_t word = 0, taken = 0;
+    bool close = false;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+        float w;
+        if constexpr (sizeof(T) == 4) {
+            w = fmaf(x[i], inv[i % G], kMagic);
+            close = close || fabsf(fmaf(kMagic - w, s[i % G], x[i])) >= 0.5f * s[i % G];
+        } else {
+            w = (fmaf(x[i], inv[i % G], 48.f) - 48.f) + kMagic;
+        }
+        word = word * 16u + __float_as_uint(w);
+        taken = taken * 16u + kHigh;
+    }
+    word -= taken;
+    if (sizeof(T) == 4 && close) {
+        word = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) word |= kv4_code(x[i], s[i % G], inv[i % G]) << (4 * i);
+    }
+    return word;
+}
+
 // D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value: one word of codes each.
 // Dimension d is of group d mod G, so a thread holds 8 / G elements of every group, and the largest of a group is
-// taken over the threads by halving the groups that a thread carries.  Bound by the bytes of the rows.
+// taken over the threads by halving the groups that a thread carries.  Bound by the bytes of the rows.  blockIdx.y is
+// the head: the CTA's rows, consecutive positions of a prompt, are one piece of the cache.
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads)
 k_kv4_append(const Kv4 c, const T * k, long long k_stride, const T * v, long long v_stride, int rows,
              const int32_t * row_seq, const int32_t * row_pos, const int32_t * seq_slot, int n_seq) {
     constexpr int G = D / 32, L = D / 8;
     pdl_trigger();
-    const long long item = blockIdx.x * (long long)(kCacheThreads / L) + threadIdx.x / L;
-    const int j = threadIdx.x % L;
+    const int r = blockIdx.x * (kCacheThreads / L) + threadIdx.x / L, h = blockIdx.y, j = threadIdx.x % L;
     const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
     pdl_wait_primary();
-    if (item >= (long long)rows * c.kv_heads) return;
-    const int r = int(item / c.kv_heads), h = int(item - (long long)r * c.kv_heads);
+    if (r >= rows) return;
+    const int seq = row_seq[r], pos = row_pos[r];
     float x[2][8];
     const T * src[2] = {k + r * k_stride + h * D + 8 * j, v + r * v_stride + h * D + 8 * j};
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        load4(src[w], x[w]);
-        load4(src[w] + 4, x[w] + 4);
-    }
-    const int seq = row_seq[r], pos = row_pos[r];
+    for (int w = 0; w < 2; ++w) load_row<8>(src[w], x[w]);
     if (seq < 0 || seq >= n_seq) return;
     const int slot = seq_slot[seq];
     if (slot < 0 || slot >= c.n_slots || pos < 0 || pos >= c.max_len) return;
@@ -196,9 +304,12 @@ k_kv4_append(const Kv4 c, const T * k, long long k_stride, const T * v, long lon
     for (int w = 0; w < 2; ++w) {
         uint32_t most[G];
 #pragma unroll
-        for (int g = 0; g < G; ++g) most[g] = 0;
+        for (int g = 0; g < G; ++g) {
+            float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most[i % G] = max(most[i % G], __float_as_uint(x[w][i]) & 0x7fffffffu);
+            for (int i = g; i < 8; i += 2 * G) m = max3_nan(m, fabsf(x[w][i]), fabsf(x[w][i + G]));
+            most[g] = __float_as_uint(m);  // a NaN is the largest as an integer
+        }
         // exchange: after it this thread carries group `mine` over all threads
         int mine = 0;
         if constexpr (G == 4) {
@@ -214,88 +325,96 @@ k_kv4_append(const Kv4 c, const T * k, long long k_stride, const T * v, long lon
         mine += up ? 1 : 0;
 #pragma unroll
         for (int s = S / 2; s; s >>= 1) m = max(m, __shfl_xor_sync(mask, m, s));
-        const __half half_scale = kv4_scale(m);
-        const float own = __half2float(half_scale);
-        if (!(j & (S - 1))) (w ? c.v_scales : c.k_scales)[at * G + mine] = __half_as_ushort(half_scale);
+        const __half scale = kv4_scale(m);
+        const float own = __half2float(scale), own_inv = own > 0.f ? __fdividef(1.f, own) : 0.f;
+        if (!(j & (S - 1))) (w ? c.v_scales : c.k_scales)[at * G + mine] = __half_as_ushort(scale);
         float s[G], inv[G];
+        // thread g * S of the head carries group g in the order of the halvings
 #pragma unroll
-        for (int g = 0; g < G; ++g) {  // thread g * S of the head carries group g in the order of the halvings
+        for (int g = 0; g < G; ++g) {
             s[g] = __shfl_sync(mask, own, g * S, L);
-            inv[g] = __fdividef(1.f, s[g]);
+            inv[g] = __shfl_sync(mask, own_inv, g * S, L);
         }
-        uint32_t word = 0;
+        // a group beyond the largest scale saturates; one that is not finite has codes of zero
+        if (__any_sync(mask, m > __float_as_uint(7.f * 65504.f))) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= kv4_code(x[w][i], s[i % G], inv[i % G]) << (4 * i);
-        reinterpret_cast<uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j] = word;
+            for (int i = 0; i < 8; ++i) {
+                const float most_x = 7.f * s[i % G];
+                x[w][i] = inv[i % G] > 0.f ? fminf(fmaxf(x[w][i], -most_x), most_x) : 0.f;
+            }
+        }
+        reinterpret_cast<uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j] = kv4_word<T, G>(x[w], s, inv);
     }
 }
 
 // D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value; kReadRows rows a thread,
-// whose loads are under way together.  Bound by the bytes written.
+// whose loads are under way together.  Bound by the bytes written.  blockIdx.y is the head.
 constexpr int kReadRows = 4;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads)
 k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n_seq, int total, T * k,
            long long k_stride, T * v, long long v_stride) {
-    constexpr int G = D / 32, L = D / 8, kDtype = std::is_same_v<T, float> ? EXL3CU_F32 : std::is_same_v<T, __half> ? EXL3CU_F16 : EXL3CU_BF16;
+    constexpr int G = D / 32, L = D / 8, kStep = kCacheThreads / L;
     pdl_trigger();
-    const int j = threadIdx.x % L;
-    // items of the CTA: (row, head), heads first; a thread's are kCacheThreads / L apart
-    const long long items = (long long)total * c.kv_heads;
-    const long long first = blockIdx.x * (long long)(kReadRows * kCacheThreads / L) + threadIdx.x / L;
+    const int j = threadIdx.x % L, h = blockIdx.y;
+    const int first = blockIdx.x * (kReadRows * kStep) + threadIdx.x / L;  // rows first, first + kStep, ...
+    const CodeConst kc2;
     pdl_wait_primary();
-    if (first >= items) return;
-    int seq = find_segment(offsets, n_seq, int(first / c.kv_heads));
-    const int end = offsets[n_seq];
+    if (first >= total) return;
+    int seq = find_segment(offsets, n_seq, first);
+    const int end = min(offsets[n_seq], total);
     uint32_t codes[kReadRows][2], scales[kReadRows][2][G / 2];
-    int rows[kReadRows], heads[kReadRows];
+    bool live[kReadRows];
 #pragma unroll
     for (int u = 0; u < kReadRows; ++u) {
-        const long long item = first + u * (kCacheThreads / L);
-        const int r = int(item / c.kv_heads), h = int(item - (long long)r * c.kv_heads);
-        rows[u] = -1;
-        heads[u] = h;
+        const int r = first + u * kStep;
+        live[u] = false;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             codes[u][w] = 0x88888888u;
 #pragma unroll
             for (int g = 0; g < G / 2; ++g) scales[u][w][g] = 0;
         }
-        if (item >= items || r >= end) continue;
+        if (r >= end) continue;
         if (seq < 0) seq = find_segment(offsets, n_seq, r);
         if (seq < 0) continue;
         while (r >= offsets[seq + 1]) ++seq;  // ends: r < offsets[n_seq]
-        rows[u] = r;
+        live[u] = true;
         const int slot = seq_slot[seq], pos = r - offsets[seq];
         if (slot < 0 || slot >= c.n_slots || pos >= c.max_len) continue;  // zeros
         const size_t at = (size_t(slot) * c.kv_heads + h) * c.max_len + pos;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             codes[u][w] = reinterpret_cast<const uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j];
-            const uint32_t * s = reinterpret_cast<const uint32_t *>((w ? c.v_scales : c.k_scales) + at * G);
-#pragma unroll
-            for (int g = 0; g < G / 2; ++g) scales[u][w][g] = s[g];
+            lds(reinterpret_cast<const unsigned char *>((w ? c.v_scales : c.k_scales) + at * G), scales[u][w]);
         }
     }
 #pragma unroll
     for (int u = 0; u < kReadRows; ++u) {
-        if (rows[u] < 0) continue;
+        if (!live[u]) continue;
+        const long long r = first + u * kStep;
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             float s[G], x[8];
 #pragma unroll
             for (int g = 0; g < G; g += 2) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&scales[u][w][g / 2]));
+                const float2 f = h2f2(scales[u][w][g / 2]);
                 s[g] = f.x;
                 s[g + 1] = f.y;
             }
+            const uint32_t lo = codes[u][w], hi = lo >> 8;
+            const uint32_t pairs[4] = {codes2<0>(lo, kc2), codes2<1>(lo, kc2), codes2<2>(hi, kc2), codes2<3>(hi, kc2)};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = float(int(codes[u][w] >> (4 * i) & 15u) - 8) * s[i % G];
-            T * out = (w ? v + rows[u] * v_stride : k + rows[u] * k_stride) + heads[u] * D + 8 * j;
+            for (int i = 0; i < 4; ++i) {  // codes i and i + 4, less 8
+                const float2 f = h2f2(pairs[i]);
+                x[i] = f.x * s[i % G];
+                x[i + 4] = f.y * s[i % G];
+            }
+            T * out = (w ? v + r * v_stride : k + r * k_stride) + h * D + 8 * j;
             if constexpr (sizeof(T) == 4) {
-                store4(out, kDtype, 0, x);
-                store4(out, kDtype, 4, x + 4);
+                store4(out, EXL3CU_F32, 0, x);
+                store4(out, EXL3CU_F32, 4, x + 4);
             } else {
                 uint4 q;
                 T * e = reinterpret_cast<T *>(&q);
@@ -421,26 +540,6 @@ __device__ __forceinline__ void mma16816_first(float (&d)[4], const uint32_t (&a
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Constants of codes2 in registers: an instruction takes one immediate, and these need two.
-struct CodeConst {
-    uint32_t magic, sixteenth, minus72;
-    __device__ __forceinline__ CodeConst() {
-        asm volatile("mov.b32 %0, 0x64006400;" : "=r"(magic));
-        asm volatile("mov.b32 %0, 0x2c002c00;" : "=r"(sixteenth));
-        asm volatile("mov.b32 %0, 0xd480d480;" : "=r"(minus72));
-    }
-};
-
-// Halves c - 8 of codes i and i + 4 of a word, i = 0 .. 3, from the word for i < 2 and from the word shifted right
-// by 8 for i >= 2: the code's bits in the mantissa of 1024 make 1024 + c (or, 4 bits up, 1024 + 16 c).
-template <int i> __device__ __forceinline__ uint32_t codes2(uint32_t w, const CodeConst & k) {
-    uint32_t x, y;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w), "r"(i & 1 ? 0x00f000f0u : 0x000f000fu), "r"(k.magic));
-    if (i & 1) asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(y) : "r"(x), "r"(k.sixteenth), "r"(k.minus72));
-    else asm("add.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0xe408e408u));  // - 1032
-    return y;
-}
-
 __device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
     uint32_t y;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
@@ -465,7 +564,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
-__device__ __forceinline__ float2 h2f2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 .. 127
 
 // The key of a 16-key step that row g (and, 8 further, row g + 8) of the score fragment stands for.  Chosen so
@@ -473,31 +571,6 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 // on different banks as far as a row of 64 or 32 bytes allows.
 template <int D> __device__ __forceinline__ int key_of(int g) {
     return g & 1 ? 4 + ((g >> 1) ^ (D == 128 ? 1 : 2)) : g >> 1;
-}
-
-// N elements from 16-byte aligned memory.
-template <int N, typename T> __device__ __forceinline__ void load_row(const T * p, float (&x)[N]) {
-    constexpr int V = 16 / sizeof(T);
-#pragma unroll
-    for (int i = 0; i < N; i += V) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p + i);
-        const T * e = reinterpret_cast<const T *>(&v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) x[i + j] = to_f32(e[j]);
-    }
-}
-
-// W words of 4 bytes (1, 2 or 4) from shared memory.
-template <int W> __device__ __forceinline__ void lds(const unsigned char * p, uint32_t (&w)[W]) {
-    if constexpr (W == 4) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-    } else if constexpr (W == 2) {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        w[0] = v.x, w[1] = v.y;
-    } else {
-        w[0] = *reinterpret_cast<const uint32_t *>(p);
-    }
 }
 
 template <typename T, int D, bool LO>
@@ -1031,7 +1104,7 @@ bool rows_ok(const void * p, size_t stride, size_t width, int dtype) {
 
 bool cache_ok(const exl3cu_kv4_cache * c) {
     return c && c->k_codes && c->k_scales && c->v_codes && c->v_scales && c->n_slots > 0 && c->kv_heads > 0 &&
-           c->max_len > 0 && c->max_len % 64 == 0 && (c->head_dim == 64 || c->head_dim == 128) &&
+           c->kv_heads <= 1024 && c->max_len > 0 && c->max_len % 64 == 0 && (c->head_dim == 64 || c->head_dim == 128) &&
            (reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->k_scales) |
             reinterpret_cast<uintptr_t>(c->v_codes) | reinterpret_cast<uintptr_t>(c->v_scales)) % 16 == 0;
 }
@@ -1089,12 +1162,18 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
     const RopeArgs a{d_q, d_k, d_q_out, d_k_out, (long long)q_stride, (long long)k_stride, (long long)q_out_stride,
                      (long long)k_out_stride, d_row_pos, d_q_w, d_k_w, d_inv_freq, eps, attn_factor, rows, heads,
                      kv_heads, rotary_dim, interleaved != 0, q_out_dtype, k_out_dtype};
-    // rows of a CTA: one while that leaves SMs without work, then as many as keep eight CTAs an SM
-    const int per_cta = std::max(1, std::min(kRopeMaxRows, rows / (8 * kSms)));
+    // rows of a CTA: one while that leaves SMs idle; with more the angles are shared by fewer threads, and the last
+    // CTAs leave the GPU emptier (8191 rows: 2 rows TIME2, 4 rows TIME4 us)
+    const int per_cta = std::max(1, std::min(2, rows / (8 * kSms)));
+    const bool same = q_out_dtype == dtype && (!kv_heads || k_out_dtype == dtype);
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        return attn_launch(head_dim == 128 ? k_qk_norm_rope<T, 128> : k_qk_norm_rope<T, 64>,
-                           dim3(unsigned((rows + per_cta - 1) / per_cta)), dim3(kRopeThreads), 0, stream, a, per_cta);
+        const dim3 grid(unsigned((rows + per_cta - 1) / per_cta));
+        if (head_dim == 128)
+            return attn_launch(same ? k_qk_norm_rope<T, 128, true> : k_qk_norm_rope<T, 128, false>, grid,
+                               dim3(kRopeThreads), 0, stream, a, per_cta);
+        return attn_launch(same ? k_qk_norm_rope<T, 64, true> : k_qk_norm_rope<T, 64, false>, grid, dim3(kRopeThreads), 0,
+                           stream, a, per_cta);
     });
 }
 
@@ -1110,13 +1189,12 @@ int exl3cu_kv4_append(const exl3cu_kv4_cache * cache, const void * d_k, size_t k
         !rows_ok(d_v, v_stride, width, dtype))
         return bad("kv4_append: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
-    const long long per_cta = kCacheThreads / (cache->head_dim / 8);
-    const long long ctas = ((long long)rows * cache->kv_heads + per_cta - 1) / per_cta;
-    if (ctas > 0x7fffffffll) return bad("kv4_append: too many rows");
+    const int per_cta = kCacheThreads / (cache->head_dim / 8);
+    const dim3 grid(unsigned((rows - 1) / per_cta + 1), unsigned(cache->kv_heads));
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_append<T, 128> : k_kv4_append<T, 64>,
-                           dim3(unsigned(ctas)), dim3(kCacheThreads), 0, stream, c, static_cast<const T *>(d_k),
+                           grid, dim3(kCacheThreads), 0, stream, c, static_cast<const T *>(d_k),
                            (long long)k_stride, static_cast<const T *>(d_v), (long long)v_stride, rows, d_row_seq,
                            d_row_pos, d_seq_slot, n_seq);
     });
@@ -1133,13 +1211,12 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
     if (!d_seq_slot || !d_kv_offsets || !rows_ok(d_k, k_stride, width, dtype) || !rows_ok(d_v, v_stride, width, dtype))
         return bad("kv4_read: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
-    const long long per_cta = kReadRows * (kCacheThreads / (cache->head_dim / 8));
-    const long long ctas = ((long long)total_rows * cache->kv_heads + per_cta - 1) / per_cta;
-    if (ctas > 0x7fffffffll) return bad("kv4_read: too many rows");
+    const int per_cta = kReadRows * (kCacheThreads / (cache->head_dim / 8));
+    const dim3 grid(unsigned((total_rows - 1) / per_cta + 1), unsigned(cache->kv_heads));
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_read<T, 128> : k_kv4_read<T, 64>,
-                           dim3(unsigned(ctas)), dim3(kCacheThreads), 0, stream, c, d_seq_slot, d_kv_offsets, n_seq,
+                           grid, dim3(kCacheThreads), 0, stream, c, d_seq_slot, d_kv_offsets, n_seq,
                            total_rows, static_cast<T *>(d_k), (long long)k_stride, static_cast<T *>(d_v),
                            (long long)v_stride);
     });
