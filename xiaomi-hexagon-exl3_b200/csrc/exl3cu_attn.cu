@@ -154,25 +154,27 @@ __global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a,
     int d0 = 8 * j, d1 = 8 * j + 4, f0 = a.interleaved ? 4 * j : -1;
     if (!a.interleaved && 4 * j < half) d0 = f0 = 4 * j, d1 = half + 4 * j;
     const bool turns = a.interleaved ? d0 < a.rotary : f0 >= 0;
-    const int per_row = a.heads + a.kv_heads;
-    int r = 0, h = threadIdx.x / L;  // h < per_row after this
-    const auto settle = [&] {
-        while (h >= per_row) {
-            h -= per_row;
-            ++r;
-        }
-    };
-    const auto load = [&](float * v) {
-        const long long row = row0 + r;
-        const T * x = h < a.heads ? static_cast<const T *>(a.q) + row * a.q_stride + h * D
-                                  : static_cast<const T *>(a.k) + row * a.k_stride + (h - a.heads) * D;
-        load4(x + d0, v);
-        load4(x + d1, v + 4);
-    };
-    settle();
     pdl_wait_primary();
+    // the heads of q, then those of k: item = (row, head), this thread's kStep apart
+    struct Items {
+        const T * x;
+        long long stride;
+        int heads, r, h;
+        __device__ __forceinline__ void settle() {
+            while (h >= heads) {
+                h -= heads;
+                ++r;
+            }
+        }
+        __device__ __forceinline__ const T * at(int row0) const { return x + (row0 + r) * stride + h * D; }
+    };
+    Items q{static_cast<const T *>(a.q), a.q_stride, a.heads, 0, int(threadIdx.x / L)};
+    q.settle();
     float next[8];
-    if (r < rows) load(next);
+    if (q.r < rows) {
+        load4(q.at(row0) + d0, next);
+        load4(q.at(row0) + d1, next + 4);
+    }
     if (threadIdx.x < rows) sm_pos[threadIdx.x] = a.row_pos[row0 + threadIdx.x];
     for (int i = threadIdx.x; i < rows * half; i += kRopeThreads) {
         const int ar = i / half, f = i - ar * half, pos = a.row_pos[row0 + ar];
@@ -181,61 +183,67 @@ __global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a,
         sm_cos[ar * (D / 2) + f] = cs;
         sm_sin[ar * (D / 2) + f] = sn;
     }
-    float wq[8], wk[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {  // any alignment
-        wq[i] = a.q_w ? a.q_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
-        wk[i] = a.k_w && a.kv_heads ? a.k_w[(i < 4 ? d0 : d1 - 4) + i] : 1.f;
-    }
     const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
-    __syncthreads();
-    while (r < rows) {
-        const int now_r = r, now_h = h;
-        float v[8];
+    const auto run = [&](Items it, const float * weights, void * out, long long out_stride, int out_dtype) {
+        float w[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = next[i];
-        h += kStep;
-        settle();
-        if (r < rows) load(next);
-        const bool is_q = now_h < a.heads;
-        if (is_q ? a.q_w != nullptr : a.k_w != nullptr) {
-            float ss = 0.f;
+        for (int i = 0; i < 8; ++i) w[i] = weights ? weights[(i < 4 ? d0 : d1 - 4) + i] : 1.f;  // any alignment
+        while (it.r < rows) {
+            const int r = it.r, h = it.h;
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+            for (int i = 0; i < 8; ++i) v[i] = next[i];
+            it.h += kStep;
+            it.settle();
+            if (it.r < rows) {
+                load4(it.at(row0) + d0, next);
+                load4(it.at(row0) + d1, next + 4);
+            }
+            if (weights) {
+                float ss = 0.f;
 #pragma unroll
-            for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
-            const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+                for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * (is_q ? wq[i] : wk[i]);
-        }
-        if (turns) {
-            float cs[4], sn[4];
-            load4(sm_cos + now_r * (D / 2) + f0, cs);
-            load4(sm_sin + now_r * (D / 2) + f0, sn);
-            if (a.interleaved) {
+                for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
+                const float inv = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x0 = v[2 * i], x1 = v[2 * i + 1];
-                    v[2 * i] = x0 * cs[i] - x1 * sn[i];
-                    v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
-                }
-            } else {
+                for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+            }
+            if (turns) {
+                float cs[4], sn[4];
+                load4(sm_cos + r * (D / 2) + f0, cs);
+                load4(sm_sin + r * (D / 2) + f0, sn);
+                if (a.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float x0 = v[i], x1 = v[i + 4];
-                    v[i] = x0 * cs[i] - x1 * sn[i];
-                    v[i + 4] = x1 * cs[i] + x0 * sn[i];
+                    for (int i = 0; i < 4; ++i) {
+                        const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                        v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                        v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x0 = v[i], x1 = v[i + 4];
+                        v[i] = x0 * cs[i] - x1 * sn[i];
+                        v[i + 4] = x1 * cs[i] + x0 * sn[i];
+                    }
                 }
             }
+            if (sm_pos[r] < 0) continue;
+            const long long at = (row0 + r) * out_stride + h * D;
+            store4(out, SAME ? kType : out_dtype, at + d0, v);
+            store4(out, SAME ? kType : out_dtype, at + d1, v + 4);
         }
-        if (sm_pos[now_r] < 0) continue;
-        const long long row = row0 + now_r;
-        void * out = is_q ? a.q_out : a.k_out;
-        const int dt = SAME ? kType : is_q ? a.q_out_dtype : a.k_out_dtype;
-        const long long at = is_q ? row * a.q_out_stride + now_h * D : row * a.k_out_stride + (now_h - a.heads) * D;
-        store4(out, dt, at + d0, v);
-        store4(out, dt, at + d1, v + 4);
+    };
+    Items k{static_cast<const T *>(a.k), a.k_stride, max(a.kv_heads, 1), a.kv_heads ? 0 : rows, int(threadIdx.x / L)};
+    k.settle();
+    __syncthreads();
+    run(q, a.q_w, a.q_out, a.q_out_stride, a.q_out_dtype);
+    if (k.r < rows) {
+        load4(k.at(row0) + d0, next);
+        load4(k.at(row0) + d1, next + 4);
     }
+    run(k, a.k_w, a.k_out, a.k_out_stride, a.k_out_dtype);
 }
 
 // ---- the 4-bit cache -------------------------------------------------------------------------------

@@ -29,12 +29,14 @@ struct Kv4 {
 };
 
 // The scale of a group from the bits of its largest |x| (compared as integers, so that a NaN is the
-// largest): the smallest half with 7 * scale >= |x|.  Rounding up twice, the quotient to float and that to
-// half, is the half above the exact quotient, since every half is a float.
+// largest): the smallest half with 7 * scale >= |x|, at most 65504.  The half nearest to the quotient is that one
+// or the one below it, and 7 times a half is exact.
 __device__ __forceinline__ __half kv4_scale(uint32_t most_bits) {
-    if (most_bits >= 0x7f800000u) return __ushort_as_half(0x7fff);  // an infinity or a NaN in the group
-    const float s = __fdiv_ru(__uint_as_float(most_bits), 7.0f);
-    return s > 65504.0f ? __ushort_as_half(0x7bff) : __float2half_ru(s);
+    const float most = __uint_as_float(most_bits);
+    const __half near = __float2half_rn(fminf(most * (1.f / 7.f), 65504.f));
+    uint32_t bits = __half_as_ushort(near);
+    if (7.f * __half2float(near) < most && bits < 0x7bffu) ++bits;
+    return __ushort_as_half(most_bits >= 0x7f800000u ? 0x7fff : bits);  // an infinity or a NaN in the group
 }
 
 // 8 + x / s rounded to the nearest integer, ties to even, from -7 to 7; inv about 1 / s.  The approximate quotient is at
