@@ -133,117 +133,110 @@ __device__ __forceinline__ void store4(void * p, int dtype, long long at, const 
     }
 }
 
-// A CTA takes `rows_per_cta` rows: their angles once for all heads into shared memory, then D/8 threads a head, each
-// with two runs of four dimensions that hold both members of its pairs ((4 j, half + 4 j) or 8 consecutive ones), so
-// that the rotation needs no exchange; a thread's next head is loaded while it works on one.  Bound by the bytes of q
-// and k in and out; a call of few rows by latency.
-constexpr int kRopeThreads = 128;
-constexpr int kRopeMaxRows = 4;
+// D/8 threads to a head, each with two runs of four dimensions that hold both members of its pairs ((4 j, half + 4 j)
+// or 8 consecutive ones), so that the rotation needs no exchange.  A thread keeps its head (with its weights and
+// addresses) and goes through the CTA's rows, the next row's loads under way; the rows' angles are computed once for
+// all heads, kRopeRows rows at a time, into shared memory.  Bound by the bytes of q and k in and out; a call of few
+// rows by latency.  The CTAs of a call are resident together, each with an equal number of rows.
+constexpr int kRopeThreads = 512;    // at most: heads beyond kRopeThreads / (D / 8) are taken in turn
+constexpr int kRopeRows = 8;
+constexpr int kRopePerSm = 1024;     // threads resident on an SM
 
 // SAME: the outputs are of the inputs' type.
 template <typename T, int D, bool SAME>
-__global__ void __launch_bounds__(kRopeThreads) k_qk_norm_rope(const RopeArgs a, int rows_per_cta) {
-    constexpr int L = D / 8, kStep = kRopeThreads / L;  // threads of a head, heads at a time
+__global__ void __launch_bounds__(kRopeThreads, 2) k_qk_norm_rope(const RopeArgs a) {
+    constexpr int L = D / 8;
     constexpr int kType = std::is_same_v<T, float> ? EXL3CU_F32 : std::is_same_v<T, __half> ? EXL3CU_F16 : EXL3CU_BF16;
-    __shared__ __align__(16) float sm_cos[kRopeMaxRows * (D / 2)], sm_sin[kRopeMaxRows * (D / 2)];
-    __shared__ int sm_pos[kRopeMaxRows];
+    __shared__ __align__(16) float sm_cos[2][kRopeRows * (D / 2)], sm_sin[2][kRopeRows * (D / 2)];
+    __shared__ int sm_pos[2][kRopeRows];
     pdl_trigger();
-    const int half = a.rotary / 2, j = threadIdx.x % L;
-    const int row0 = blockIdx.x * rows_per_cta, rows = min(rows_per_cta, a.rows - row0);
+    const int half = a.rotary / 2, j = threadIdx.x % L, per_row = a.heads + a.kv_heads, step = blockDim.x / L;
+    // the CTA's rows: an equal share
+    const int first = int((long long)a.rows * blockIdx.x / gridDim.x), last = int((long long)a.rows * (blockIdx.x + 1) / gridDim.x);
     // the thread's two runs of dimensions, and the first of its pairs' frequencies where it rotates
     int d0 = 8 * j, d1 = 8 * j + 4, f0 = a.interleaved ? 4 * j : -1;
     if (!a.interleaved && 4 * j < half) d0 = f0 = 4 * j, d1 = half + 4 * j;
     const bool turns = a.interleaved ? d0 < a.rotary : f0 >= 0;
-    pdl_wait_primary();
-    // the heads of q, then those of k: item = (row, head), this thread's kStep apart
-    struct Items {
-        const T * x;
-        long long stride;
-        int heads, r, h;
-        __device__ __forceinline__ void settle() {
-            while (h >= heads) {
-                h -= heads;
-                ++r;
-            }
-        }
-        __device__ __forceinline__ const T * at(int row0) const { return x + (row0 + r) * stride + h * D; }
-    };
-    Items q{static_cast<const T *>(a.q), a.q_stride, a.heads, 0, int(threadIdx.x / L)};
-    q.settle();
-    float next[8];
-    if (q.r < rows) {
-        load4(q.at(row0) + d0, next);
-        load4(q.at(row0) + d1, next + 4);
-    }
-    if (threadIdx.x < rows) sm_pos[threadIdx.x] = a.row_pos[row0 + threadIdx.x];
-    for (int i = threadIdx.x; i < rows * half; i += kRopeThreads) {
-        const int ar = i / half, f = i - ar * half, pos = a.row_pos[row0 + ar];
-        float cs, sn;
-        rope_angle(max(pos, 0), a.inv_freq[f], a.factor, cs, sn);
-        sm_cos[ar * (D / 2) + f] = cs;
-        sm_sin[ar * (D / 2) + f] = sn;
-    }
+    f0 = max(f0, 0);
     const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
-    const auto run = [&](Items it, const float * weights, void * out, long long out_stride, int out_dtype) {
-        float w[8];
+    pdl_wait_primary();
+    for (int row0 = first, buf = 0; row0 < last; row0 += kRopeRows, buf ^= 1) {
+        const int rows = min(kRopeRows, last - row0);
+        if (threadIdx.x < rows) sm_pos[buf][threadIdx.x] = a.row_pos[row0 + threadIdx.x];
+        for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
+            const int ar = i / half, f = i - ar * half, pos = a.row_pos[row0 + ar];
+            float cs, sn;
+            rope_angle(max(pos, 0), a.inv_freq[f], a.factor, cs, sn);
+            sm_cos[buf][ar * (D / 2) + f] = cs;
+            sm_sin[buf][ar * (D / 2) + f] = sn;
+        }
+        bool ready = false;
+        for (int h = threadIdx.x / L; h < per_row || !ready; h += step) {
+            const bool is_q = h < a.heads, any = h < per_row;
+            const int kh = h - a.heads;
+            const T * x = is_q ? static_cast<const T *>(a.q) + row0 * a.q_stride + h * D
+                               : static_cast<const T *>(a.k) + row0 * a.k_stride + kh * D;
+            const long long stride = is_q ? a.q_stride : a.k_stride, out_stride = is_q ? a.q_out_stride : a.k_out_stride;
+            const float * weights = is_q ? a.q_w : a.k_w;
+            void * out = is_q ? a.q_out : a.k_out;
+            const int dt = SAME ? kType : is_q ? a.q_out_dtype : a.k_out_dtype;
+            long long at = row0 * out_stride + (is_q ? h : kh) * D;
+            float next[8], w[8];
+            if (any) {
+                load4(x + d0, next);
+                load4(x + d1, next + 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = weights ? weights[(i < 4 ? d0 : d1 - 4) + i] : 1.f;  // any alignment
-        while (it.r < rows) {
-            const int r = it.r, h = it.h;
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = next[i];
-            it.h += kStep;
-            it.settle();
-            if (it.r < rows) {
-                load4(it.at(row0) + d0, next);
-                load4(it.at(row0) + d1, next + 4);
+                for (int i = 0; i < 8; ++i) w[i] = weights ? weights[(i < 4 ? d0 : d1 - 4) + i] : 1.f;  // any alignment
             }
-            if (weights) {
-                float ss = 0.f;
+            if (!ready) __syncthreads();  // the angles; with two buffers the next chunk's are not those still in use
+            ready = true;
+            if (!any) break;
+            const float * cos_at = sm_cos[buf] + f0, * sin_at = sm_sin[buf] + f0;
+            for (int r = 0; r < rows; ++r, at += out_stride, cos_at += D / 2, sin_at += D / 2) {
+                float v[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+                for (int i = 0; i < 8; ++i) v[i] = next[i];
+                if (r + 1 < rows) {
+                    x += stride;
+                    load4(x + d0, next);
+                    load4(x + d1, next + 4);
+                }
+                if (weights) {
+                    float ss = 0.f;
 #pragma unroll
-                for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
-                const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+                    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
-            }
-            if (turns) {
-                float cs[4], sn[4];
-                load4(sm_cos + r * (D / 2) + f0, cs);
-                load4(sm_sin + r * (D / 2) + f0, sn);
-                if (a.interleaved) {
+                    for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
+                    const float inv = rsqrtf(ss * (1.f / D) + a.eps);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x0 = v[2 * i], x1 = v[2 * i + 1];
-                        v[2 * i] = x0 * cs[i] - x1 * sn[i];
-                        v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
-                    }
-                } else {
+                    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+                }
+                if (turns) {
+                    float cs[4], sn[4];
+                    load4(cos_at, cs);
+                    load4(sin_at, sn);
+                    if (a.interleaved) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x0 = v[i], x1 = v[i + 4];
-                        v[i] = x0 * cs[i] - x1 * sn[i];
-                        v[i + 4] = x1 * cs[i] + x0 * sn[i];
+                        for (int i = 0; i < 4; ++i) {
+                            const float x0 = v[2 * i], x1 = v[2 * i + 1];
+                            v[2 * i] = x0 * cs[i] - x1 * sn[i];
+                            v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x0 = v[i], x1 = v[i + 4];
+                            v[i] = x0 * cs[i] - x1 * sn[i];
+                            v[i + 4] = x1 * cs[i] + x0 * sn[i];
+                        }
                     }
                 }
+                if (sm_pos[buf][r] < 0) continue;
+                store4(out, dt, at + d0, v);
+                store4(out, dt, at + d1, v + 4);
             }
-            if (sm_pos[r] < 0) continue;
-            const long long at = (row0 + r) * out_stride + h * D;
-            store4(out, SAME ? kType : out_dtype, at + d0, v);
-            store4(out, SAME ? kType : out_dtype, at + d1, v + 4);
         }
-    };
-    Items k{static_cast<const T *>(a.k), a.k_stride, max(a.kv_heads, 1), a.kv_heads ? 0 : rows, int(threadIdx.x / L)};
-    k.settle();
-    __syncthreads();
-    run(q, a.q_w, a.q_out, a.q_out_stride, a.q_out_dtype);
-    if (k.r < rows) {
-        load4(k.at(row0) + d0, next);
-        load4(k.at(row0) + d1, next + 4);
     }
-    run(k, a.k_w, a.k_out, a.k_out_stride, a.k_out_dtype);
 }
 
 // ---- the 4-bit cache -------------------------------------------------------------------------------
@@ -1170,18 +1163,15 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
     const RopeArgs a{d_q, d_k, d_q_out, d_k_out, (long long)q_stride, (long long)k_stride, (long long)q_out_stride,
                      (long long)k_out_stride, d_row_pos, d_q_w, d_k_w, d_inv_freq, eps, attn_factor, rows, heads,
                      kv_heads, rotary_dim, interleaved != 0, q_out_dtype, k_out_dtype};
-    // rows of a CTA: one while that leaves SMs idle; with more the angles are shared by fewer threads, and the last
-    // CTAs leave the GPU emptier (8191 rows: 2 rows TIME2, 4 rows TIME4 us)
-    const int per_cta = std::max(1, std::min(2, rows / (8 * kSms)));
     const bool same = q_out_dtype == dtype && (!kv_heads || k_out_dtype == dtype);
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const dim3 grid(unsigned((rows + per_cta - 1) / per_cta));
+        const int lanes = head_dim / 8;
+        const int threads = (std::min((heads + kv_heads) * lanes, kRopeThreads) + 31) / 32 * 32;
+        const dim3 grid(unsigned(std::min(rows, kRopePerSm / threads * kSms))), block{unsigned(threads)};
         if (head_dim == 128)
-            return attn_launch(same ? k_qk_norm_rope<T, 128, true> : k_qk_norm_rope<T, 128, false>, grid,
-                               dim3(kRopeThreads), 0, stream, a, per_cta);
-        return attn_launch(same ? k_qk_norm_rope<T, 64, true> : k_qk_norm_rope<T, 64, false>, grid, dim3(kRopeThreads), 0,
-                           stream, a, per_cta);
+            return attn_launch(same ? k_qk_norm_rope<T, 128, true> : k_qk_norm_rope<T, 128, false>, grid, block, 0, stream, a);
+        return attn_launch(same ? k_qk_norm_rope<T, 64, true> : k_qk_norm_rope<T, 64, false>, grid, block, 0, stream, a);
     });
 }
 
