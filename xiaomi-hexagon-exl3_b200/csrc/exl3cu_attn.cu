@@ -443,11 +443,13 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 //   O^T [16 dimensions x 8] += V codes (A: pairs of keys brought together by a byte permutation) times weights
 //   (B: the score fragment, transposed by movmatrix).
 //
-// LO (f32 rows): a column pair holds the high and the low half of one head's operand, x = hi + lo to 2^-22, so
-// 4 heads share a tile; 16-bit rows have 8 heads of one half each (weights rounded to 2^-11 of their value, the
-// product's own precision).  Both operands are scaled by powers of two into the half's range: q by its largest
-// element, the weights by the largest value scale seen, so that nothing overflows or vanishes whatever the cache
-// holds.  Masked keys get a score of -inf and scales of zero; codes are finite whatever they are.
+// Columns: 8 heads of 16-bit rows, or, where no more than 4 share a K/V head, one head to a pair of columns, which
+// halves what a lane computes around the products; of f32 rows the pair's second column holds the low half of the
+// operand, x = hi + lo to 2^-22.  (16-bit rows: weights rounded to 2^-11 of their value, the result's own precision.)
+// Both operands are scaled by powers of two into the half's range: q by its largest element, the weights by the largest
+// value scale seen, so that nothing overflows or vanishes whatever the cache holds.  The maximum that the weights
+// refer to follows the true one when it has grown by more than 2^kLazy.  Masked keys get a score of -inf and scales of
+// zero; codes are finite whatever they are.
 //
 // The tiles of all rows form one list that is cut into equal shares, one per CTA, so that a batch of a long and
 // many short contexts fills the GPU evenly (a row counts kRowCost tiles more than it has: what taking up a row costs
@@ -461,6 +463,7 @@ constexpr int kSplitRows = 256;  // rows up to which the tiles of all rows are c
 constexpr int kRowCost = 2;
 constexpr int kPlanFloats = 2 * kSplitRows;  // scratch begins with (first share, shares) of every row
 constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
+constexpr int kLazy = 6, kTop = 14 - kLazy;  // weights times value scales are up to 2^kTop, 2^14 before m moves
 
 template <int D> struct Kv4Tile {
     static constexpr int kCodes = kKeys * D / 2, kScales = kKeys * D / 16;  // bytes of one of K and V
@@ -574,10 +577,12 @@ template <int D> __device__ __forceinline__ int key_of(int g) {
     return g & 1 ? 4 + ((g >> 1) ^ (D == 128 ? 1 : 2)) : g >> 1;
 }
 
-template <typename T, int D, bool LO>
+template <typename T, int D, int HC>
 __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
     using Tile = Kv4Tile<D>;
-    constexpr int G = D / 32, HC = LO ? 4 : 8, H = LO ? 1 : 2;  // groups, heads of the CTA, heads of a lane's scores
+    constexpr int G = D / 32, H = HC / 4;  // groups, heads of a lane's scores
+    constexpr bool PAIR = HC == 4, LO = sizeof(T) == 4;  // a head to two columns; the second one its low halves
+    static_assert(!LO || PAIR, "f32 rows take two columns a head");
     extern __shared__ __align__(128) unsigned char ring_all[];
     __shared__ uint64_t full[kAttnWarps][kStages];
     __shared__ int sm_n[kSplitRows], sm_slot[kSplitRows], sm_scan[4], sm_row, sm_off;
@@ -665,12 +670,12 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
         int next = t0 + warp;
         for (int i = 0; i < kStages && next < t1; ++i, next += kAttnWarps) start(next);
 
-        // q as the B operand: column g is a head (and, with LO, its high or low half); this lane's dimensions are
+        // q as the B operand: column g is a head (PAIR: half of one); this lane's dimensions are
         // [t D/4, +D/4), words of 8, codes i and i + 4 of a word a pair.  Scaled by 2^e to a largest element in [2^8, 2^9).
         uint32_t qb[D / 16][2];
         float cs[H];
         {
-            const int col_head = LO ? g >> 1 : g;
+            const int col_head = PAIR ? g >> 1 : g;
             float x[D / 4], top = 0.f;
             const T * src = static_cast<const T *>(a.q) + call_row * a.q_stride + (head0 + min(col_head, nh - 1)) * D + t * (D / 4);
             load_row<D / 4>(src, x);
@@ -690,6 +695,8 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 if (LO) {
                     const float hi = __half2float(__float2half_rn(x[i]));
                     x[i] = g & 1 ? x[i] - hi : hi;
+                } else if (PAIR && (g & 1)) {
+                    x[i] = 0.f;
                 }
             }
 #pragma unroll
@@ -705,8 +712,8 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
             }
         }
 
-        // accumulators; largest score (before cs); sum of the weights.  Weights are exp2((s - m) cs + 28 - ev),
-        // ev the exponent of the largest value scale seen: times a value scale they stay below 2^14.
+        // accumulators; the score that weights refer to (before cs); sum of the weights.  Weights are
+        // exp2((s - m) cs + 14 + kTop - ev), ev the exponent of the largest value scale seen, which is below 2^(ev - 14).
         float o[D / 16][4] = {}, m[H], l[H] = {};
 #pragma unroll
         for (int j = 0; j < H; ++j) m[j] = -INFINITY;
@@ -727,7 +734,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the next copy into the slot
                 __syncwarp();
             }
-            // scores of keys 16 x + key_of(g) (+ 8), heads t (LO) or 2 t, 2 t + 1
+            // scores of keys 16 x + key_of(g) (+ 8), heads t (PAIR) or 2 t, 2 t + 1
             float sc[4][2][H];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
@@ -763,7 +770,8 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                     const float a0 = j & 1 ? f0.y : f0.x, a1 = j & 1 ? f1.y : f1.x;
 #pragma unroll
                     for (int jj = 0; jj < H; ++jj) {
-                        const float v0 = LO ? acc[j][0] + acc[j][1] : acc[j][jj], v1 = LO ? acc[j][2] + acc[j][3] : acc[j][2 + jj];
+                        const float v0 = LO ? acc[j][0] + acc[j][1] : acc[j][jj];
+                        const float v1 = LO ? acc[j][2] + acc[j][3] : acc[j][2 + jj];
                         sc[x][0][jj] = j ? fmaf(a0, v0, sc[x][0][jj]) : a0 * v0;
                         sc[x][1][jj] = j ? fmaf(a1, v1, sc[x][1][jj]) : a1 * v1;
                     }
@@ -790,24 +798,23 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
             }
             const int grown = max(int(top) - ev, 0);
             bool moved = grown > 0;
-            float corr[H];
+            float mx[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) {
-                float mx = max3(m[j], sc[0][0][j], sc[0][1][j]);
+                mx[j] = max3(m[j], sc[0][0][j], sc[0][1][j]);
 #pragma unroll
-                for (int x = 1; x < 4; ++x) mx = max3(mx, sc[x][0][j], sc[x][1][j]);
+                for (int x = 1; x < 4; ++x) mx[j] = max3(mx[j], sc[x][0][j], sc[x][1][j]);
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-                corr[j] = mx == m[j] ? 1.f : exp2_approx((m[j] - mx) * cs[j]);
-                moved = moved || mx != m[j];
-                m[j] = mx;
+                for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
+                moved = moved || (mx[j] - m[j]) * cs[j] > float(kLazy);  // no: both -inf
             }
             if (__any_sync(0xffffffffu, moved)) {
                 ev += grown;
                 const float down = pow2(-grown);
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
-                    const float f = corr[j] * down;
+                    const float f = (mx[j] == m[j] ? 1.f : exp2_approx((m[j] - mx[j]) * cs[j])) * down;
+                    m[j] = mx[j];
                     l[j] *= f;
 #pragma unroll
                     for (int i = 0; i < D / 16; ++i) {
@@ -822,7 +829,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
             }
             float ref[H];
 #pragma unroll
-            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : float(28 - ev) - m[j] * cs[j];
+            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : float(14 + kTop - ev) - m[j] * cs[j];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int k0 = 16 * x + key_of<D>(g);
@@ -845,7 +852,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                         const float2 f = h2f2(y ? s1[j / 2] : s0[j / 2]);
                         const float sv = j & 1 ? f.y : f.x, v0 = p[y][0] * sv;
                         pb[j][y] = transpose8x8(LO ? pack_h2(v0, v0 - __half2float(__float2half_rn(v0)))
-                                                   : pack_h2(v0, p[y][H - 1] * sv));
+                                                   : pack_h2(v0, PAIR ? 0.f : p[y][H - 1] * sv));
                     }
                 // values of keys 2 t, 2 t + 1 and 8 further (as the score rows count them): dimensions of word(s) g
                 uint32_t va[D / 64], vb[D / 64], vc2[D / 64], vd[D / 64];
@@ -898,12 +905,12 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
         constexpr int kRec = D + 4;
         float * const mine = reinterpret_cast<float *>(ring);
         __syncwarp();
-        const float back = pow2(ev - 28);
+        const float back = pow2(ev - 14 - kTop);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], x);
-            float * rec = mine + (LO ? t : 2 * t + j) * kRec;
+            float * rec = mine + (PAIR ? t : 2 * t + j) * kRec;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const int d = D == 128 ? 16 * g + i : 8 * g + i;
@@ -954,101 +961,69 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
 
 // Joins the parts of the rows that were cut, in a fixed order.  WIDE (few rows, so many parts to each): a CTA per
 // (row, K/V head chunk, head), a thread per dimension and kGroups-th part.  Otherwise a CTA per (row, K/V head chunk),
-// a thread per output.
-constexpr int kMergeThreads = 512;
+// a thread per output.  Bound by latency: the parts' loads go out together, kBatch to a thread.
+constexpr int kMergeThreads = 1024;
 
 template <typename T, int D, int HC, bool WIDE>
-__global__ void __launch_bounds__(kMergeThreads) k_kv4_merge(const Kv4Attn a, int shares) {
-    constexpr int kRec = D + 4, kGroups = kMergeThreads / D;
-    __shared__ float sm_acc[WIDE ? kGroups : 1][D], sm_l[WIDE ? kGroups : 1];
+__global__ void __launch_bounds__(WIDE ? kMergeThreads : HC * D) k_kv4_merge(const Kv4Attn a, int shares) {
+    constexpr int kRec = D + 4, kGroups = WIDE ? kMergeThreads / D : 1, kBatch = WIDE ? 14 : 4;
+    __shared__ float sm_a[kGroups][D], sm_m[kGroups], sm_l[kGroups];
     const int row = blockIdx.x, y = blockIdx.y;
     pdl_trigger();
     pdl_wait_primary();
     const int2 plan = reinterpret_cast<const int2 *>(a.part)[row];  // first share, shares
     if (plan.y <= 1) return;
     const int share_heads = a.heads / a.c.kv_heads, chunk = y % a.chunks;
-    const int nh = min(HC, share_heads - chunk * HC);
-    const float * const base = a.part + kPlanFloats + ((size_t(y) * shares + plan.x) * 2) * (HC * kRec);
-    // a CTA's record 0 is the row that it begins and does not end, record 1 the row that it goes on with
-    const auto rec = [&](int i, int h) { return base + (size_t(i) * 2 * HC + (i > 0 ? HC : 0) + h) * kRec; };
-    T * const out = static_cast<T *>(a.out) + row * a.out_stride + (y / a.chunks * share_heads + chunk * HC) * D;
-    if constexpr (WIDE) {
-        const int h = blockIdx.z, d = threadIdx.x % D, group = threadIdx.x / D;
-        if (h >= nh) return;
-        // loads of eight parts at a time, all under way together
-        float M = -INFINITY;
-        for (int i0 = threadIdx.x & 31; i0 < plan.y; i0 += 8 * 32) {
-            float v[8];
+    const int h = WIDE ? blockIdx.z : threadIdx.x / D, d = threadIdx.x % D, group = WIDE ? threadIdx.x / D : 0;
+    if (h >= min(HC, share_heads - chunk * HC)) return;
+    const float * const base = a.part + kPlanFloats + ((size_t(y) * shares + plan.x) * 2 * HC + h) * kRec;
+    float M = -INFINITY, L = 0.f, A = 0.f;
+    for (int i0 = group; i0 < plan.y; i0 += kBatch * kGroups) {
+        float vm[kBatch], vl[kBatch], va[kBatch];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = i0 + 32 * u < plan.y ? rec(i0 + 32 * u, h)[D] : -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) M = fmaxf(M, v[u]);
+        for (int u = 0; u < kBatch; ++u) {
+            const int i = min(i0 + kGroups * u, plan.y - 1);
+            // a CTA's record 0 is the row that it begins and does not end, record 1 the row that it goes on with
+            const float * r = base + (size_t(i) * 2 + (i > 0)) * HC * kRec;
+            vm[u] = r[D];
+            vl[u] = r[D + 1];
+            va[u] = r[d];
         }
+        float mn = M;
 #pragma unroll
-        for (int x = 16; x; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-        const float ref = M == -INFINITY ? 0.f : M;
-        float L = 0.f, A = 0.f;
-        for (int i0 = group; i0 < plan.y; i0 += 8 * kGroups) {
-            float vm[8], vl[8], va[8];
+        for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, vm[u]);
+        const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_approx(M - ref);
+        L *= f0;
+        A *= f0;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = i0 + kGroups * u;
-                const float * r = rec(min(i, plan.y - 1), h);
-                vm[u] = i < plan.y ? r[D] : -INFINITY;
-                vl[u] = r[D + 1];
-                va[u] = r[d];
+        for (int u = 0; u < kBatch; ++u)
+            if (i0 + kGroups * u < plan.y) {
+                const float f = exp2_approx(vm[u] - ref);
+                L = fmaf(vl[u], f, L);
+                A = fmaf(va[u], f, A);
             }
-#pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (i0 + kGroups * u < plan.y) {
-                    const float f = exp2_approx(vm[u] - ref);
-                    L = fmaf(vl[u], f, L);
-                    A = fmaf(va[u], f, A);
-                }
+        M = mn;
+    }
+    if constexpr (WIDE) {
+        sm_a[group][d] = A;
+        if (d == 0) {
+            sm_m[group] = M;
+            sm_l[group] = L;
         }
-        sm_acc[group][d] = A;
-        if (d == 0) sm_l[group] = L;
         __syncthreads();
         if (group) return;
-        L = sm_l[0];
 #pragma unroll
-        for (int i = 1; i < kGroups; ++i) {
-            L += sm_l[i];
-            A += sm_acc[i][d];
-        }
-        out[h * D + d] = from_f32<T>(A / L);
-    } else {
-        for (int i = threadIdx.x; i < nh * D; i += kMergeThreads) {
-            const int h = i / D, d = i % D;
-            // one pass over the parts, four under way together
-            float M = -INFINITY, L = 0.f, A = 0.f;
-            for (int x0 = 0; x0 < plan.y; x0 += 4) {
-                float vm[4], vl[4], va[4];
+        for (int i = 0; i < kGroups; ++i) M = fmaxf(M, sm_m[i]);
+        const float ref = M == -INFINITY ? 0.f : M;
+        L = A = 0.f;
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const float * r = rec(min(x0 + u, plan.y - 1), h);
-                    vm[u] = r[D];
-                    vl[u] = r[D + 1];
-                    va[u] = r[d];
-                }
-                float mn = M;
-#pragma unroll
-                for (int u = 0; u < 4; ++u) mn = fmaxf(mn, vm[u]);
-                const float ref = mn == -INFINITY ? 0.f : mn, f0 = exp2_approx(M - ref);
-                L *= f0;
-                A *= f0;
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (x0 + u < plan.y) {
-                        const float f = exp2_approx(vm[u] - ref);
-                        L = fmaf(vl[u], f, L);
-                        A = fmaf(va[u], f, A);
-                    }
-                M = mn;
-            }
-            out[i] = from_f32<T>(A / L);
+        for (int i = 0; i < kGroups; ++i) {
+            const float f = exp2_approx(sm_m[i] - ref);
+            L = fmaf(sm_l[i], f, L);
+            A = fmaf(sm_a[i][d], f, A);
         }
     }
+    static_cast<T *>(a.out)[row * a.out_stride + (y / a.chunks * share_heads + chunk * HC + h) * D + d] = from_f32<T>(A / L);
 }
 
 // How a call is cut up: shares (CTAs) per K/V head chunk, 0 for one CTA per row.
@@ -1060,7 +1035,7 @@ struct AttnPlan {
 AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     AttnPlan p;
     const int share_heads = heads / c->kv_heads;
-    p.heads_per_cta = dtype == EXL3CU_F32 ? 4 : 8;
+    p.heads_per_cta = dtype == EXL3CU_F32 || share_heads <= 4 ? 4 : 8;
     p.chunks = (share_heads + p.heads_per_cta - 1) / p.heads_per_cta;
     p.ys = c->kv_heads * p.chunks;
     p.shares = 0;
@@ -1072,8 +1047,6 @@ AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     p.scratch = kPlanFloats * sizeof(float) + size_t(p.ys) * p.shares * 2 * p.heads_per_cta * (c->head_dim + 4) * sizeof(float);
     return p;
 }
-
-std::atomic<unsigned long long> g_attn_attr[6];
 
 }  // namespace
 
@@ -1249,34 +1222,38 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
                     scale * 1.4426950408889634f};
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        constexpr bool LO = std::is_same_v<T, float>;
-        constexpr int HC = LO ? 4 : 8;
-        const auto run = [&](auto dim) {
-            constexpr int D = decltype(dim)::value;
+        const auto run = [&](auto dim, auto heads_per_cta) {
+            constexpr int D = decltype(dim)::value, HC = decltype(heads_per_cta)::value;
             constexpr int smem = kAttnWarps * kStages * Kv4Tile<D>::kBytes;
             static_assert(size_t(HC) * (D + 4) * 4 <= kStages * Kv4Tile<D>::kBytes, "a warp's record fits its ring");
             int dev = 0;
             if (cudaGetDevice(&dev) != cudaSuccess) return api_cuda_fail(cudaGetLastError(), "kv4_attn");
-            auto & done = g_attn_attr[(D == 128 ? 3 : 0) + (LO ? 0 : std::is_same_v<T, __half> ? 1 : 2)];
+            static std::atomic<unsigned long long> done{0};  // devices whose kernel may use that much shared memory
             const unsigned long long bit = 1ull << (dev & 63);
             if (!(done.load() & bit)) {
                 const cudaError_t e =
-                    cudaFuncSetAttribute(k_kv4_attn<T, D, LO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                    cudaFuncSetAttribute(k_kv4_attn<T, D, HC>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
                 if (e != cudaSuccess) return api_cuda_fail(e, "kv4_attn: shared memory");
                 done.fetch_or(bit);
             }
-            const int rc = attn_launch(k_kv4_attn<T, D, LO>, dim3(unsigned(p.shares ? p.shares : rows), unsigned(p.ys)),
+            const int rc = attn_launch(k_kv4_attn<T, D, HC>, dim3(unsigned(p.shares ? p.shares : rows), unsigned(p.ys)),
                                        dim3(128), size_t(smem), stream, a);
             if (rc || !p.shares) return rc;
-            // a row has about shares / rows parts: above 8, a CTA per head (one row of 131071 positions, 103 parts:
-            // 10.0 against 4.1 us); below, one for all heads (64 rows: 17.9 against 3 us)
+            // a row has about shares / rows parts: above 8, a CTA per head, below, one for all heads of a K/V head
             if (p.shares > 8 * rows)
                 return attn_launch(k_kv4_merge<T, D, HC, true>, dim3(unsigned(rows), unsigned(p.ys), HC),
                                    dim3(kMergeThreads), 0, stream, a, p.shares);
-            return attn_launch(k_kv4_merge<T, D, HC, false>, dim3(unsigned(rows), unsigned(p.ys)), dim3(kMergeThreads), 0,
+            return attn_launch(k_kv4_merge<T, D, HC, false>, dim3(unsigned(rows), unsigned(p.ys)), dim3(HC * D), 0,
                                stream, a, p.shares);
         };
-        return cache->head_dim == 128 ? run(std::integral_constant<int, 128>{}) : run(std::integral_constant<int, 64>{});
+        constexpr std::integral_constant<int, 64> d64;
+        constexpr std::integral_constant<int, 128> d128;
+        constexpr std::integral_constant<int, 4> h4;
+        if constexpr (sizeof(T) == 2) {
+            constexpr std::integral_constant<int, 8> h8;
+            if (p.heads_per_cta == 8) return cache->head_dim == 128 ? run(d128, h8) : run(d64, h8);
+        }
+        return cache->head_dim == 128 ? run(d128, h4) : run(d64, h4);
     });
 }
 
