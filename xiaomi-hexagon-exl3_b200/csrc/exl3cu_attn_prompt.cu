@@ -11,10 +11,10 @@
 // blocks of a sequence are launched longest first.
 //
 // Per tile of keys:  S = Q K^T (tcgen05, operands in shared memory by TMA, 128-byte swizzle), S in TMEM;
-// a thread owns a row of S: maximum, P = exp2(scale log2e (S - m)), row sum in f32, P rounded to the 16-bit
-// type (half a step each, as the library of any such kernel does: the product needs 16-bit operands) and
-// stored over S in TMEM;  O += P V with P from TMEM, V from shared memory as it lies (MN-major), O in TMEM.  The
-// maximum that the weights refer to follows the true one only when it has grown by more than 2^8, so O is
+// a thread owns a row of S: maximum, P = exp2(scale log2e (S - m)), a quarter of them on the multiply-add pipe,
+// row sum in f32, P rounded to the 16-bit type (half a step each: the product takes 16-bit operands) and stored over S
+// in TMEM;  O += P V, begun when half of P is there, with P from TMEM, V from shared memory as it lies (MN-major), O in
+// TMEM.  The maximum that the weights refer to follows the true one only when it has grown by more than 2^8, so O is
 // rescaled rarely; weights stay at or below 256.
 //
 // Warps: 0-3 and 4-7 the rows of the two tiles; 8 loads; 9 issues the products and owns TMEM.  While one
@@ -75,10 +75,18 @@ struct PromptArgs {
     float scale_log2; // scale * log2(e)
 };
 
-__device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo) {
-    return uint64_t((saddr >> 4) & 0x3fffu) | uint64_t((lbo >> 4) & 0x3fffu) << 16 | uint64_t((sbo >> 4) & 0x3fffu) << 32 |
-           uint64_t(1) << 46 |  // descriptor version for sm_100
-           uint64_t(2) << 61;   // 128-byte swizzle
+// A shared-memory operand's descriptor: the low word (address and leading offset) moves with the operand, the high
+// word (stride of 8 rows 1024 bytes, descriptor version for sm_100, 128-byte swizzle) is the same for all here.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo) {
+    return ((saddr >> 4) & 0x3fffu) | ((lbo >> 4) & 0x3fffu) << 16;
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+    return p != 0;
 }
 
 __device__ __forceinline__ void commit(uint64_t * bar) {
@@ -91,18 +99,18 @@ __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D = A B (+ D): both operands in shared memory / A in TMEM.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 x, {%1, %4};\n\tmov.b64 y, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(uint32_t(acc))
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0u)
+        "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %5, 0;\n\tmov.b64 y, {%2, %4};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}"
+        ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(kDescHigh), "r"(uint32_t(acc))
         : "memory");
 }
 
@@ -141,10 +149,51 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The largest of three, a NaN if one is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+
+// Two floats side by side, the operands of the two-wide instructions.
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
+    return y;
+}
+__device__ __forceinline__ float2 of_two(uint64_t x) {
+    float2 y;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
+    return y;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t y;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
+    return y;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t y;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
+    return y;
+}
+
+// 2^x of two x from -126 to 127 on the multiply-add pipe (the exponential unit does 16 a clock and SM, which is as
+// long as the products take): x = n + f, |f| <= 1/2, by a sum with 1.5 * 2^23; 2^f by a polynomial of degree 4 fitted
+// for the least relative error on [-1/2, 1/2], 2.6e-6 at most; n goes into the exponent.
+__device__ __forceinline__ float2 exp2_two(uint64_t x) {
+    const float2 v = of_two(x);
+    x = two(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+    const uint64_t magic = two(12582912.f, 12582912.f);
+    const uint64_t t = add2(x, magic);
+    const uint64_t f = add2(x, fma2(t, two(-1.f, -1.f), magic));  // x - n
+    uint64_t y = fma2(f, two(9.570096619e-3f, 9.570096619e-3f), two(5.591785908e-2f, 5.591785908e-2f));
+    y = fma2(y, f, two(0.2402474433f, 0.2402474433f));
+    y = fma2(y, f, two(0.6931217909f, 0.6931217909f));
+    y = fma2(y, f, two(0.9999992847f, 0.9999992847f));
+    const float2 n = of_two(t), r = of_two(y);
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(n.x) << 23)),
+                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(n.y) << 23)));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
     uint32_t y;
@@ -154,7 +203,7 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
 }
 
 struct Bars {
-    uint64_t full[8], empty[8], q_full, clean[kMasked], s_full[2], p_full[2], o_done[2];
+    uint64_t full[8], empty[8], q_full, clean[kMasked], s_full[2], p_full[2][2], o_done[2];
     uint32_t tmem, dirty;
     int seq, q0, q1, k0, k1, p0;  // the CTA's work; q1 <= q0: none
 };
@@ -232,7 +281,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             for (int i = 0; i < kMasked; ++i) mbar_init(&bars.clean[i], 1);
             for (int t = 0; t < 2; ++t) {
                 mbar_init(&bars.s_full[t], 1);
-                mbar_init(&bars.p_full[t], 4);  // the tile's warps
+                for (int i = 0; i < 2; ++i) mbar_init(&bars.p_full[t][i], 4);  // the tile's warps
                 mbar_init(&bars.o_done[t], 1);
             }
             bars.dirty = 0;
@@ -349,67 +398,88 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         }
         __syncwarp();
     } else if (warp == 9) {
-        // ---- products (one thread) ----
-        if (lane == 0 && n > 0) {
-            constexpr uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
-            constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | 8u << 24;  // f32 sums, M = 128
-            constexpr uint32_t idesc_s = common | uint32_t(kTile >> 3) << 17;
-            constexpr uint32_t idesc_o = common | uint32_t(D >> 3) << 17 | 1u << 16;  // V: MN-major
-            const uint64_t desc_q = smem_desc(smem_addr(sq), 16, 1024);
-            const uint64_t desc_k = smem_desc(smem_addr(ring), 16, 1024);
-            const uint64_t desc_v = smem_desc(smem_addr(ring), kBlockBytes, 1024);
-            constexpr uint64_t tile16 = Sh::kTileBytes >> 4;
-            const auto product_s = [&](int t, int slot) {
+        // ---- products ----
+        // The warp stays together and one lane issues, so that addresses and descriptors live in uniform registers:
+        // a lone thread spends more time on preparing the instructions than the tensor cores on carrying them out.
+        constexpr uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
+        constexpr uint32_t common = 1u << 4 | type << 7 | type << 10 | 8u << 24;  // f32 sums, M = 128
+        constexpr uint32_t idesc_s = common | uint32_t(kTile >> 3) << 17;
+        constexpr uint32_t idesc_o = common | uint32_t(D >> 3) << 17 | 1u << 16;  // V: MN-major
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const int n0 = __shfl_sync(0xffffffffu, nt[0], 0), n1 = __shfl_sync(0xffffffffu, nt[1], 0), nn = max(n0, n1);
+        const int first_masked = __shfl_sync(0xffffffffu, masked0, 0);
+        const uint32_t desc_q = desc_low(smem_addr(sq), 16), desc_k = desc_low(smem_addr(ring), 16);
+        const uint32_t desc_v = desc_low(smem_addr(ring), kBlockBytes);
+        constexpr uint32_t tile16 = Sh::kTileBytes >> 4;
+        const auto product_s = [&](int t, int slot) {
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint64_t at = uint64_t((kk / 4) * kBlockBytes + (kk % 4) * 32) >> 4;
-                    mma_ss(tmem + t * 128, desc_q + t * tile16 + at, desc_k + slot * tile16 + at, idesc_s, kk > 0);
-                }
-            };
-            const auto product_o = [&](int t, int slot, bool add) {
+            for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t at = uint32_t((kk / 4) * kBlockBytes + (kk % 4) * 32) >> 4;
+                mma_ss(tm + t * 128, desc_q + t * tile16 + at, desc_k + slot * tile16 + at, idesc_s, kk > 0);
+            }
+        };
+        const auto product_o = [&](int t, int slot, int part, bool add) {  // one half of the tile's keys
 #pragma unroll
-                for (int kk = 0; kk < kTile / 16; ++kk)
-                    mma_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, desc_v + slot * tile16 + kk * (2048 >> 4), idesc_o,
-                           add || kk > 0);
-            };
-            bool ok = mbar_wait(&bars.q_full, 0) && mbar_wait(&bars.full[0], 0);
-            if (ok) {
+            for (int kk = 4 * part; kk < 4 * part + 4; ++kk)
+                mma_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, desc_v + slot * tile16 + kk * (2048 >> 4), idesc_o, add || kk > 0);
+        };
+        bool ok = true;
+        // every lane has seen the phase, or none goes on
+        const auto wait = [&](uint64_t & bar, unsigned parity) {
+            ok = ok && __all_sync(0xffffffffu, mbar_wait(&bar, parity));
+        };
+        // a slot is handed back only where a later load waits for it: no arrival outlives the CTA
+        const auto returns = [&](int item) { return item + Sh::kSlots < 2 * nn; };
+        if (nn > 0) {
+            wait(bars.q_full, 0);
+            wait(bars.full[0], 0);
+            if (ok && elect()) {
                 for (int t = 0; t < 2; ++t)
-                    if (nt[t] > 0) {
+                    if ((t ? n1 : n0) > 0) {
                         product_s(t, 0);
                         commit(&bars.s_full[t]);
                     }
+                if (returns(0)) commit(&bars.empty[0]);
             }
-            // a slot is handed back only where a later load waits for it: no arrival outlives the CTA
-            const auto hand_back = [&](int item) {
-                if (item + Sh::kSlots < 2 * n) commit(&bars.empty[item % Sh::kSlots]);
-            };
-            if (ok) hand_back(0);
-            for (int j = 0; j < n && ok; ++j) {
-                const int vi = 2 * j + 1, ki = 2 * j + 2;
-                const int vs = vi % Sh::kSlots, ks = ki % Sh::kSlots;
-                ok = mbar_wait(&bars.full[vs], unsigned(vi / Sh::kSlots) & 1u);
-                if (ok && j >= masked0) ok = mbar_wait(&bars.clean[j - masked0], 0);
-                if (ok && j + 1 < n) ok = mbar_wait(&bars.full[ks], unsigned(ki / Sh::kSlots) & 1u);
-                for (int t = 0; t < 2 && ok; ++t) {
-                    if (j < nt[t]) {
-                        ok = mbar_wait(&bars.p_full[t], unsigned(j) & 1u);
-                        if (!ok) break;
-                        fence_after();
-                        product_o(t, vs, j > 0);
-                        if (j + 1 == nt[t]) commit(&bars.o_done[t]);
-                    }
-                    if (t == 1 || nt[1] <= j) hand_back(vi);
-                    if (j + 1 < nt[t]) {
-                        product_s(t, ks);
-                        commit(&bars.s_full[t]);
-                    }
-                    if (t == 0 && nt[1] <= j) break;  // the second tile has no more
-                }
-                if (ok && j + 1 < n) hand_back(ki);
-            }
-            if (!ok) atomicOr(&g_prompt_status, kStatusWaitTimeout);
+            __syncwarp();
         }
+        int vs = 1, ks = 2;               // slots of this tile's values and the next one's keys
+        unsigned vphase = 0, kphase = 0;  // and their barriers' phases
+        for (int j = 0; j < nn && ok; ++j) {
+            wait(bars.full[vs], vphase);
+            if (j >= first_masked) wait(bars.clean[j - first_masked], 0);
+            if (j + 1 < nn) wait(bars.full[ks], kphase);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int mine = t ? n1 : n0, other = t ? n0 : n1;
+                if (j < mine) {
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        wait(bars.p_full[t][part], unsigned(j) & 1u);
+                        fence_after();
+                        if (ok && elect()) {
+                            product_o(t, vs, part, part || j > 0);
+                            if (part) {
+                                if (j + 1 == mine) commit(&bars.o_done[t]);
+                                // the tile's last user of the values, and of the next keys
+                                if ((t || j >= other) && returns(2 * j + 1)) commit(&bars.empty[vs]);
+                                if (j + 1 < mine) {
+                                    product_s(t, ks);
+                                    commit(&bars.s_full[t]);
+                                    if ((t || j + 1 >= other) && returns(2 * j + 2)) commit(&bars.empty[ks]);
+                                }
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            vs += 2;
+            if (vs >= Sh::kSlots) vs -= Sh::kSlots, vphase ^= 1u;
+            ks += 2;
+            if (ks >= Sh::kSlots) ks -= Sh::kSlots, kphase ^= 1u;
+        }
+        if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
         __syncwarp();
     }
     } else {
@@ -430,22 +500,29 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             if (!ok) break;
             fence_after();
             uint32_t s[kTile];
+            const bool edge = (j + 1) * kTile > tile_sees;  // some row does not see all of the tile
+            const int left = lim - j * kTile;
+            // four chains of maxima over 32 columns at a time, the next columns on their way
+            float mx[4] = {m, m, m, m};
+            tmem_ld(ts, s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tmem_ld(ts + 32 * i, s + 32 * i);
-            wait_ld();
-            if ((j + 1) * kTile > tile_sees) {
-                const int left = lim - j * kTile;
+            for (int i = 0; i < 4; ++i) {
+                wait_ld();
+                if (i < 3) tmem_ld(ts + 32 * (i + 1), s + 32 * (i + 1));
+                if (edge) {
 #pragma unroll
-                for (int i = 0; i < kTile; ++i) s[i] = i < left ? s[i] : 0xff800000u;
+                    for (int x = 32 * i; x < 32 * i + 32; ++x) s[x] = x < left ? s[x] : 0xff800000u;
+                }
+#pragma unroll
+                for (int x = 0; x < 32; x += 2)
+                    mx[x / 2 % 4] = max3(mx[x / 2 % 4], __uint_as_float(s[32 * i + x]), __uint_as_float(s[32 * i + x + 1]));
             }
-            float mx = m;
-#pragma unroll
-            for (int i = 0; i < kTile; i += 2) mx = max3(mx, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+            const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
             // m: what the weights refer to.  It moves with the first tile, and when the true maximum is more
-            // than 2^8 above; then the sums so far are scaled down.  (mx - m is NaN where both are -inf.)
-            if (__any_sync(0xffffffffu, (mx - m) * c > 8.f)) {
-                const float f = mx == m ? 1.f : exp2_fast((m - mx) * c);
-                m = mx;
+            // than 2^8 above (or a NaN, which then stays); then the sums so far are scaled down.
+            if (__any_sync(0xffffffffu, !((top - m) * c <= 8.f))) {
+                const float f = top == m ? 1.f : exp2_fast((m - top) * c);
+                m = top;
                 sum *= f;
                 if (j > 0) {  // every product up to the tile before is complete: S of this tile came after them
                     for (int i = 0; i < D; i += 32) {
@@ -458,23 +535,39 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     }
                 }
             }
-            const float mc = m == -INFINITY ? 0.f : m * c;  // a row that has seen nothing: all weights are 0
-            float add0 = 0.f, add1 = 0.f;
+            // a row that has seen nothing: all weights 0; +inf among the scores: all NaN, as inf - inf is
+            const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : m * c;
+            const uint64_t c2 = two(c, c), mc2 = two(-mc, -mc);
+            uint64_t add[2] = {0, 0};
+            // masked scores have to become 0: at a view's end the polynomial is not used
+            const auto weights = [&](auto polynomial) {
 #pragma unroll
-            for (int i = 0; i < kTile; i += 2) {
-                const float e0 = exp2_fast(fmaf(__uint_as_float(s[i]), c, -mc));
-                const float e1 = exp2_fast(fmaf(__uint_as_float(s[i + 1]), c, -mc));
-                add0 += e0;
-                add1 += e1;
-                s[i / 2] = pack2<T>(e0, e1);
-            }
-            sum += add0 + add1;
-            tmem_st(ts, s);
-            tmem_st(ts + 32, s + 32);
-            wait_st();
-            fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.p_full[t]);
+                for (int part = 0; part < 2; ++part) {
+#pragma unroll
+                    for (int i = kTile / 2 * part; i < kTile / 2 * (part + 1); i += 2) {
+                        const uint64_t x = fma2(two(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, mc2);
+                        float2 e;
+                        if (decltype(polynomial)::value && i / 2 % 4 == 3) {
+                            e = exp2_two(x);
+                        } else {
+                            e = of_two(x);
+                            e.x = exp2_fast(e.x);
+                            e.y = exp2_fast(e.y);
+                        }
+                        add[i / 2 % 2] = add2(add[i / 2 % 2], two(e.x, e.y));
+                        s[i / 2] = pack2<T>(e.x, e.y);
+                    }
+                    tmem_st(ts + 32 * part, s + 32 * part);
+                    wait_st();
+                    fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars.p_full[t][part]);
+                }
+            };
+            if (edge) weights(std::false_type{});
+            else weights(std::true_type{});
+            const float2 added = of_two(add2(add[0], add[1]));
+            sum += added.x + added.y;
         }
         if (ok && tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[t], 0));
         if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
