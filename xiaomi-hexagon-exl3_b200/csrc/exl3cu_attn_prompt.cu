@@ -13,9 +13,12 @@
 // Per tile of keys:  S = Q K^T (tcgen05, operands in shared memory by TMA, 128-byte swizzle), S in TMEM;
 // a thread owns a row of S: maximum, P = exp2(scale log2e (S - m)), a quarter of them on the multiply-add pipe,
 // row sum in f32, P rounded to the 16-bit type (half a step each: the product takes 16-bit operands) and stored over S
-// in TMEM;  O += P V, begun when half of P is there, with P from TMEM, V from shared memory as it lies (MN-major), O in
+// in TMEM;  O += P V, begun when three quarters of P are there, with P from TMEM, V from shared memory as it lies (MN-major), O in
 // TMEM.  The maximum that the weights refer to follows the true one only when it has grown by more than 2^8, so O is
 // rescaled rarely; weights stay at or below 256.
+//
+// (Two threads a row instead of one: the exponentials of a tile take no less time, 1235 against 877 us at 16384
+// tokens.)
 //
 // Warps: 0-3 and 4-7 the rows of the two tiles; 8 loads; 9 issues the products and owns TMEM.  While one
 // tile's rows work on their exponentials, the other tile's products run.
@@ -51,6 +54,7 @@ constexpr int kThreads = 384;   // 8 warps of rows, load warp, product warp, two
 constexpr int kRegs = 168, kRegsRows = 216, kRegsRest = 72;
 static_assert(8 * kRegsRows + 4 * kRegsRest <= 12 * kRegs, "more registers than the launch has would wait forever");
 constexpr int kBlockBytes = kTile * 128;  // 64 dimensions of 128 rows
+constexpr int kEarly = 96;      // keys of a tile whose weights are handed to the products before the others are computed
 constexpr uint32_t kNever = 0x7fffffffu;
 // Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
 // at most three tiles.
@@ -133,6 +137,14 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t * r) {
           "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t * r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+        ::"r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
 
@@ -418,10 +430,11 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                 mma_ss(tm + t * 128, desc_q + t * tile16 + at, desc_k + slot * tile16 + at, idesc_s, kk > 0);
             }
         };
-        const auto product_o = [&](int t, int slot, int part, bool add) {  // one half of the tile's keys
+        const auto product_o = [&](int t, int slot, int part, bool add) {
 #pragma unroll
-            for (int kk = 4 * part; kk < 4 * part + 4; ++kk)
-                mma_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, desc_v + slot * tile16 + kk * (2048 >> 4), idesc_o, add || kk > 0);
+            for (int kk = 0; kk < kTile / 16; ++kk)
+                if ((kk >= kEarly / 16) == (part != 0))
+                    mma_ts(tm + 256 + t * 128, tm + t * 128 + kk * 8, desc_v + slot * tile16 + kk * (2048 >> 4), idesc_o, add || kk > 0);
         };
         bool ok = true;
         // every lane has seen the phase, or none goes on
@@ -502,21 +515,17 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             uint32_t s[kTile];
             const bool edge = (j + 1) * kTile > tile_sees;  // some row does not see all of the tile
             const int left = lim - j * kTile;
-            // four chains of maxima over 32 columns at a time, the next columns on their way
-            float mx[4] = {m, m, m, m};
-            tmem_ld(ts, s);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                wait_ld();
-                if (i < 3) tmem_ld(ts + 32 * (i + 1), s + 32 * (i + 1));
-                if (edge) {
+            for (int i = 0; i < 4; ++i) tmem_ld(ts + 32 * i, s + 32 * i);
+            wait_ld();
+            if (edge) {
 #pragma unroll
-                    for (int x = 32 * i; x < 32 * i + 32; ++x) s[x] = x < left ? s[x] : 0xff800000u;
-                }
-#pragma unroll
-                for (int x = 0; x < 32; x += 2)
-                    mx[x / 2 % 4] = max3(mx[x / 2 % 4], __uint_as_float(s[32 * i + x]), __uint_as_float(s[32 * i + x + 1]));
+                for (int x = 0; x < kTile; ++x) s[x] = x < left ? s[x] : 0xff800000u;
             }
+            float mx[4] = {m, m, m, m};
+#pragma unroll
+            for (int x = 0; x < kTile; x += 2)
+                mx[x / 2 % 4] = max3(mx[x / 2 % 4], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
             const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
             // m: what the weights refer to.  It moves with the first tile, and when the true maximum is more
             // than 2^8 above (or a NaN, which then stays); then the sums so far are scaled down.
@@ -541,10 +550,9 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             uint64_t add[2] = {0, 0};
             // masked scores have to become 0: at a view's end the polynomial is not used
             const auto weights = [&](auto polynomial) {
+                const auto some = [&](auto from, auto to_key) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part) {
-#pragma unroll
-                    for (int i = kTile / 2 * part; i < kTile / 2 * (part + 1); i += 2) {
+                    for (int i = decltype(from)::value; i < decltype(to_key)::value; i += 2) {
                         const uint64_t x = fma2(two(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), c2, mc2);
                         float2 e;
                         if (decltype(polynomial)::value && i / 2 % 4 == 3) {
@@ -557,12 +565,20 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                         add[i / 2 % 2] = add2(add[i / 2 % 2], two(e.x, e.y));
                         s[i / 2] = pack2<T>(e.x, e.y);
                     }
-                    tmem_st(ts + 32 * part, s + 32 * part);
+                };
+                const auto hand_over = [&](int part) {
                     wait_st();
                     fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_full[t][part]);
-                }
+                };
+                some(std::integral_constant<int, 0>{}, std::integral_constant<int, kEarly>{});
+                tmem_st(ts, s);
+                tmem_st16(ts + 32, s + 32);
+                hand_over(0);
+                some(std::integral_constant<int, kEarly>{}, std::integral_constant<int, kTile>{});
+                tmem_st16(ts + 48, s + 48);
+                hand_over(1);
             };
             if (edge) weights(std::false_type{});
             else weights(std::true_type{});
