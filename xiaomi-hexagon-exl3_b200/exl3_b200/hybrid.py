@@ -23,6 +23,13 @@ RMSNorm and SwiGLU on load, residual adds in the epilogue) and the final
 RMSNorm into the head, which then is one launch; a layer is 4 operator
 launches plus its mixer.
 
+With kv_bits=4 the engine keeps its K/V caches in 4 bits (exl3_b200.attention): full-attention layers run
+        q, k = norm + RoPE                                exl3cu_qk_norm_rope
+        K, V quantised into the caches                    exl3cu_kv4_append
+        decode steps: attention over the 4-bit caches     exl3cu_kv4_attn
+        steps with prompt rows: the contexts read back    exl3cu_kv4_read
+                         and causal prompt attention      exl3cu_prompt_attn
+
 The model is synthetic (no checkpoints offline): random-init parameters with
 the stated shapes; each linear layer is an EXL3 matrix with a seeded random
 trellis bitstream, +-1 input signs and U(0.01, 0.03) output scales (the same
@@ -181,17 +188,20 @@ def one_row_each(row_offsets) -> bool:
 
 class StepMeta:
     """Device int32 row metadata of one step, filled from one pinned host buffer by one copy:
-    [tokens R | row_seq R | row_pos R | row_offsets n_seq+1 | seq_slot n_seq | logit_rows nout]."""
+    [tokens R | row_seq R | row_pos R | row_offsets n_seq+1 | seq_slot n_seq | logit_rows nout |
+    kv_offsets n_seq+1], kv_offsets the running total of the sequences' positions after the step."""
 
     def __init__(self, torch, device, max_rows: int, max_seq: int, max_out: int):
         self.cap = (max_rows, max_seq, max_out)
-        n = 3 * max_rows + 2 * max_seq + 1 + max_out
+        n = 3 * max_rows + 3 * max_seq + 2 + max_out
         self.host = torch.zeros(n, dtype=torch.int32, pin_memory=True)
         self.dev = torch.zeros(n, dtype=torch.int32, device=device)
         R, Q, O = max_rows, max_seq, max_out
         self.off = {"tokens": 0, "row_seq": R, "row_pos": 2 * R, "row_offsets": 3 * R, "seq_slot": 3 * R + Q + 1,
-                    "logit_rows": 3 * R + 2 * Q + 1}
-        self.len = {"tokens": R, "row_seq": R, "row_pos": R, "row_offsets": Q + 1, "seq_slot": Q, "logit_rows": O}
+                    "logit_rows": 3 * R + 2 * Q + 1, "kv_offsets": 3 * R + 2 * Q + 1 + O}
+        self.len = {"tokens": R, "row_seq": R, "row_pos": R, "row_offsets": Q + 1, "seq_slot": Q, "logit_rows": O,
+                    "kv_offsets": Q + 1}
+        self.kv_total = 0  # positions of the filled step's sequences together
         self.one_row_each = False  # every sequence of the filled step has exactly one row (a decode step)
 
     def view(self, name):
@@ -200,8 +210,14 @@ class StepMeta:
 
     def fill(self, tokens, row_seq, row_pos, row_offsets, seq_slot, logit_rows):
         h = self.host.numpy()
+        offs, pos = np.asarray(row_offsets, np.int64), np.asarray(row_pos, np.int64)
+        last = offs[1:] - 1  # each sequence's last row
+        kv = np.where(np.diff(offs) > 0, pos[np.clip(last, 0, max(pos.size - 1, 0))] + 1, 0) if pos.size else 0 * last
+        kv_offsets = np.concatenate([[0], np.cumsum(kv)])
+        self.kv_total = int(kv_offsets[-1])
         for name, arr in (("tokens", tokens), ("row_seq", row_seq), ("row_pos", row_pos),
-                          ("row_offsets", row_offsets), ("seq_slot", seq_slot), ("logit_rows", logit_rows)):
+                          ("row_offsets", row_offsets), ("seq_slot", seq_slot), ("logit_rows", logit_rows),
+                          ("kv_offsets", kv_offsets)):
             a = np.asarray(arr, np.int32)
             if a.size > self.len[name]:
                 raise ValueError(f"{name}: {a.size} entries, capacity {self.len[name]}")
@@ -213,18 +229,22 @@ class StepMeta:
 
 
 class HybridEngine:
-    """The hybrid decoder resident on one GPU: EXL3 weights, fp16 embedding/head, fp16 KV caches and
-    fp32 delta-rule states for `slots` concurrent sequences of up to `max_len` positions."""
+    """The hybrid decoder resident on one GPU: EXL3 weights, fp16 embedding/head, KV caches and
+    fp32 delta-rule states for `slots` concurrent sequences of up to `max_len` positions.  kv_bits: 16 (fp16
+    caches) or 4 (4.5 bits a value, 9/32 of the memory, for contexts that fp16 has no room for)."""
 
     def __init__(self, weights: HybridWeights, device: int = 0, slots: int = 8, max_len: int = 1536,
-                 max_rows: int = 512):
+                 max_rows: int = 512, kv_bits: int = 16):
         import torch
 
         from .ops import Exl3Weight
 
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits must be 16 or 4")
         self.torch = torch
         self.cfg = cfg = weights.cfg
         self.device = device
+        self.kv_bits = kv_bits
         dev = f"cuda:{device}"
         self.dev = dev
         self.slots, self.max_len, self.max_rows = slots, max_len, max_rows
@@ -258,8 +278,20 @@ class HybridEngine:
         self.down = torch.zeros((R, H), dtype=f32, device=dev)
         n_full = sum(1 for d in self.layers if d["kind"] == "full")
         n_gdn = len(self.layers) - n_full
-        self.kc = torch.zeros((max(n_full, 1), slots, cfg.kv_heads, max_len, cfg.head_dim), dtype=f16, device=dev)
-        self.vc = torch.zeros_like(self.kc)
+        if kv_bits == 16:
+            self.kc = torch.zeros((max(n_full, 1), slots, cfg.kv_heads, max_len, cfg.head_dim), dtype=f16, device=dev)
+            self.vc = torch.zeros_like(self.kc)
+        else:
+            from .attention import Kv4Cache
+
+            self.kc = self.vc = None
+            self.kv4 = [Kv4Cache(slots, cfg.kv_heads, max_len, cfg.head_dim, dev) for _ in range(n_full)]
+            self.q16 = torch.zeros((R, cfg.heads, cfg.head_dim), dtype=f16, device=dev)
+            self.k32 = torch.zeros((R, cfg.kv_heads, cfg.head_dim), dtype=f32, device=dev)
+            # every slot's context read back, the keys and values of one layer at a time
+            self.kv16 = torch.zeros((2, slots * max_len, cfg.kv_heads, cfg.head_dim), dtype=f16, device=dev)
+            need = max((c.scratch_bytes(r, cfg.heads) for c in self.kv4[:1] for r in range(1, slots + 1)), default=0)
+            self.kv4_scratch = torch.zeros(max(need, 16), dtype=torch.uint8, device=dev)
         self.state = torch.zeros((max(n_gdn, 1), slots, cfg.heads, cfg.head_dim, cfg.head_dim), dtype=f32,
                                  device=dev)
         self.conv = torch.zeros((max(n_gdn, 1), slots, 3 * D, 3), dtype=f32, device=dev)
@@ -347,7 +379,7 @@ class HybridEngine:
         scale = 1.0 / float(np.sqrt(cfg.head_dim))
         if fused:
             self._forward_fused(rows, n_seq, nout, st, scale, row_seq, row_pos, row_offsets, seq_slot, logit_rows,
-                                feedback)
+                                feedback, stream)
             return feedback is not None
         delta = None
         for li, d in enumerate(self.layers):
@@ -360,15 +392,18 @@ class HybridEngine:
                 qkv = p.view(-1)[: self.max_rows * (D + 2 * KV)].view(self.max_rows, D + 2 * KV)
                 outs = [qkv[:, 0:D], qkv[:, D:D + KV], qkv[:, D + KV:D + 2 * KV]]
                 self._mm_batch(("q", "k", "v"), mats, self.xn, outs, rows, st)
-                c = d["cache"]
-                kc, vc = self.kc[c], self.vc[c]
-                check(L.exl3cu_hyb_attn_prep(_vp(qkv), rows, _vp(row_seq), _vp(row_pos), _vp(seq_slot),
-                                             _vp(d["q_norm"]), _vp(d["k_norm"]), _vp(self.inv_freq), cfg.eps,
-                                             _vp(kc), _vp(vc), self.max_len, self.slots, _vp(self.q), st))
-                sp = attn_splits(rows)
-                check(L.exl3cu_hyb_attn(_vp(self.q), rows, _vp(row_seq), _vp(row_pos), _vp(seq_slot), _vp(kc),
-                                        _vp(vc), self.max_len, self.slots, scale, sp, _vp(self.attn_part),
-                                        self.attn_part.numel() * 4, _vp(self.attn_tickets), _vp(self.mix), st))
+                if self.kv_bits == 4:
+                    self._attention4(d, qkv, rows, n_seq, stream)
+                else:
+                    c = d["cache"]
+                    kc, vc = self.kc[c], self.vc[c]
+                    check(L.exl3cu_hyb_attn_prep(_vp(qkv), rows, _vp(row_seq), _vp(row_pos), _vp(seq_slot),
+                                                 _vp(d["q_norm"]), _vp(d["k_norm"]), _vp(self.inv_freq), cfg.eps,
+                                                 _vp(kc), _vp(vc), self.max_len, self.slots, _vp(self.q), st))
+                    sp = attn_splits(rows)
+                    check(L.exl3cu_hyb_attn(_vp(self.q), rows, _vp(row_seq), _vp(row_pos), _vp(seq_slot), _vp(kc),
+                                            _vp(vc), self.max_len, self.slots, scale, sp, _vp(self.attn_part),
+                                            self.attn_part.numel() * 4, _vp(self.attn_tickets), _vp(self.mix), st))
             else:
                 p = self.proj
                 outs = [p[:, 0:D], p[:, D:2 * D], p[:, 2 * D:3 * D], p[:, 3 * D:4 * D]]
@@ -393,8 +428,32 @@ class HybridEngine:
         check(L.exl3cu_hyb_head(_vp(self.xn), _vp(logit_rows), nout, H, None, cfg.eps, _vp(self.embed), cfg.vocab,
                                 None, _vp(self.best), _vp(self.out_tokens), st))
 
+    def _attention4(self, d, qkv, rows, n_seq, stream):
+        """A full-attention layer over the 4-bit cache: qkv rows [q | k | v] -> self.mix.  Steps of one row per
+        sequence attend to the cache as it is; others read the sequences' contexts back and run the prompt
+        attention."""
+        from . import attention
+
+        cfg, m, cache = self.cfg, self.meta, self.kv4[d["cache"]]
+        D, KV, shape = cfg.heads * cfg.head_dim, self.KV, (-1, cfg.head_dim)
+        q, k, v = (t.unflatten(1, shape) for t in qkv[:rows].split((D, KV, KV), 1))
+        row_seq, row_pos, slot = m.view("row_seq")[:rows], m.view("row_pos")[:rows], m.view("seq_slot")[:n_seq]
+        mix = self.mix[:rows].unflatten(1, shape)
+        decode = rows == n_seq and m.one_row_each
+        q_out = self.q[:rows].unflatten(1, shape) if decode else self.q16[:rows]
+        attention.qk_norm_rope(q, k, row_pos, self.inv_freq, d["q_norm"], d["k_norm"], eps=cfg.eps, q_out=q_out,
+                               k_out=self.k32[:rows], stream=stream)
+        cache.append(self.k32[:rows], v, row_seq, row_pos, slot, stream=stream)
+        if decode:
+            cache.attend(q_out, row_seq, row_pos, slot, out=mix, scratch=self.kv4_scratch, stream=stream)
+            return
+        offsets, total = m.view("kv_offsets")[:n_seq + 1], m.kv_total
+        k16, v16 = self.kv16[0, :total], self.kv16[1, :total]
+        cache.read(slot, offsets, total, k_out=k16, v_out=v16, stream=stream)
+        attention.prompt_attention(q_out, k16, v16, m.view("row_offsets")[:n_seq + 1], offsets, out=mix, stream=stream)
+
     def _forward_fused(self, rows, n_seq, nout, st, scale, row_seq, row_pos, row_offsets, seq_slot, logit_rows,
-                       feedback=None):
+                       feedback=None, stream=None):
         """Steps of <= 8 rows: the layer glue folded into the packed operator -- RMSNorm on load for the
         projections (and inside the delta-rule gates), SwiGLU on load for the down projection, the o and
         down products added into the residual stream h -- so a layer is 4 operator launches plus its
@@ -410,9 +469,11 @@ class HybridEngine:
                 outs = [qkv[:, 0:D], qkv[:, D:D + KV], qkv[:, D + KV:D + 2 * KV]]
                 self._mm_batch(("q", "k", "v"), mats, self.h, outs, rows, st, 3, d["in_norm"], x_ss=self.h_ss)
                 c = d["cache"]
-                kc, vc = self.kc[c], self.vc[c]
                 sp = attn_splits(rows)
-                if rows == n_seq and self.meta.one_row_each:  # decode: prep + attention in one launch
+                kc, vc = (self.kc[c], self.vc[c]) if self.kv_bits == 16 else (None, None)
+                if self.kv_bits == 4:
+                    self._attention4(d, qkv, rows, n_seq, stream)
+                elif rows == n_seq and self.meta.one_row_each:  # decode: prep + attention in one launch
                     check(L.exl3cu_hyb_attn_decode(_vp(qkv), rows, _vp(row_seq), _vp(row_pos), _vp(seq_slot),
                                                    _vp(d["q_norm"]), _vp(d["k_norm"]), _vp(self.inv_freq), cfg.eps,
                                                    _vp(kc), _vp(vc), self.max_len, self.slots, scale, sp,
@@ -707,12 +768,13 @@ def main(argv=None) -> int:
     ap.add_argument("--prompt", type=int, default=64)
     ap.add_argument("--steps", type=int, default=4)
     ap.add_argument("--seed", type=int, default=7)
+    ap.add_argument("--kv-bits", type=int, choices=(4, 16), default=16, help="bits of the K/V cache's values")
     args = ap.parse_args(argv)
     if not 1 <= args.requests <= 8:
         ap.error("--requests must be 1..8 (one step's logit rows)")
     cfg = HybridConfig(layers=args.layers)
     eng = HybridEngine(synthetic_weights(cfg, seed=args.seed), device=0, slots=args.requests,
-                       max_len=args.prompt + args.steps + 1, max_rows=max(64, args.requests))
+                       max_len=args.prompt + args.steps + 1, max_rows=max(64, args.requests), kv_bits=args.kv_bits)
     rng = np.random.default_rng(args.seed)
     tok = []
     for sq in range(args.requests):
