@@ -48,7 +48,8 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
  * and stands for (code - 8) * scale.
  *   codes   [n_slots][kv_heads][max_len][head_dim / 2]
  *   scales  [n_slots][kv_heads][max_len][G]
- * max_len is a multiple of 64 and the arrays start on 16-byte boundaries. */
+ * max_len is a multiple of 64, at most 2^27, kv_heads at most 1024, and the arrays start
+ * on 16-byte boundaries. */
 typedef struct exl3cu_kv4_cache {
     uint8_t * k_codes;
     uint16_t * k_scales;

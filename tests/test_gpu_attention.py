@@ -310,6 +310,23 @@ def test_attend_long_and_many_rows(A):
     check_attend(got, q, cache, [1 - i % 2 for i in range(150)], lens)
 
 
+def test_attend_more_rows_than_are_cut_into_shares(A):
+    """Above 256 rows a CTA takes a row whole; rows of no position and of no sequence among them."""
+    g = gen(21)
+    cache = A.Kv4Cache(3, 2, 256, 64)
+    fill(cache, g)
+    lens = [int(x) for x in torch.randint(0, 256, (300,), generator=g, device="cuda")]
+    q = randn(g, 300, 6, 64).bfloat16()
+    out = torch.full((300, 6, 64), 7.0, device="cuda").bfloat16()
+    seq = [i % 4 - (1 if i % 50 == 49 else 0) * 8 for i in range(300)]  # 3: no such slot; negative: no sequence
+    cache.attend(q, ints(seq), ints([n - 1 for n in lens]), ints([2, 0, 1, 9]), out=out)
+    dead = [i for i in range(300) if seq[i] < 0]
+    zero = [i for i in range(300) if seq[i] == 3 or (seq[i] >= 0 and lens[i] == 0)]
+    live = [i for i in range(300) if i not in dead and i not in zero]
+    assert bool((out[dead] == 7).all()) and bool((out[zero] == 0).all())
+    check_attend(out[live], q[live], cache, [[2, 0, 1][seq[i]] for i in live], [lens[i] for i in live])
+
+
 def test_attend_rows_that_see_nothing(A):
     g = gen(6)
     cache = A.Kv4Cache(2, 4, 128, 128)
@@ -417,6 +434,22 @@ def test_prompt_not_finite_where_masked(A, value):
     seven = got[150:170, :, 7]
     assert bool(seven.isnan().all()) if math.isnan(value) else bool((seven == value).all())
     assert bool(got[170:].isnan().all())
+
+
+def test_prompt_long_flat_tail(A):
+    """One strong key before 20000 weak ones, each 2^-26 of it: together they move the result, and no part of
+    them is lost to the 16-bit weights."""
+    n = 20001
+    k = torch.zeros((n, 1, 64), device="cuda").half()
+    k[0, 0, 0] = 8.0
+    v = torch.zeros((n, 1, 64), device="cuda").half()
+    v[0], v[1:] = 1.0, 16384.0
+    q = torch.zeros((n, 1, 64), device="cuda").half()
+    q[:, :, 0] = 1.0
+    scale = 26 * math.log(2) / 8
+    got = A.prompt_attention(q=q[-200:], k=k, v=v, q_offsets=ints([0, 200]), kv_offsets=ints([0, n]), scale=scale,
+                             out=torch.empty((200, 1, 64), device="cuda"))
+    check_prompt(got, q[-200:], k, v, [200], [(0, n)], scale)
 
 
 def test_prompt_in_a_slot_cache_and_strided(A):

@@ -1078,7 +1078,7 @@ bool rows_ok(const void * p, size_t stride, size_t width, int dtype) {
 
 bool cache_ok(const exl3cu_kv4_cache * c) {
     return c && c->k_codes && c->k_scales && c->v_codes && c->v_scales && c->n_slots > 0 && c->kv_heads > 0 &&
-           c->kv_heads <= 1024 && c->max_len > 0 && c->max_len % 64 == 0 && (c->head_dim == 64 || c->head_dim == 128) &&
+           c->kv_heads <= 1024 && c->max_len > 0 && c->max_len % 64 == 0 && c->max_len <= 1 << 27 && (c->head_dim == 64 || c->head_dim == 128) &&
            (reinterpret_cast<uintptr_t>(c->k_codes) | reinterpret_cast<uintptr_t>(c->k_scales) |
             reinterpret_cast<uintptr_t>(c->v_codes) | reinterpret_cast<uintptr_t>(c->v_scales)) % 16 == 0;
 }
@@ -1109,7 +1109,7 @@ template <typename... A> int call_with_words(int (*f)(A...), const void * words)
 }
 
 constexpr const char * kBadCache =
-    "kv4: bad cache (four 16-byte aligned arrays, head_dim 64 or 128, max_len a multiple of 64)";
+    "kv4: bad cache (four 16-byte aligned arrays, head_dim 64 or 128, max_len a multiple of 64 up to 2^27)";
 
 }  // namespace
 

@@ -15,7 +15,7 @@
 // row sum in f32, P rounded to the 16-bit type (half a step each: the product takes 16-bit operands) and stored over S
 // in TMEM;  O += P V, begun when three quarters of P are there, with P from TMEM, V from shared memory as it lies (MN-major), O in
 // TMEM.  The maximum that the weights refer to follows the true one only when it has grown by more than 2^8, so O is
-// rescaled rarely; weights stay at or below 256.
+// rescaled rarely.
 //
 // (Two threads a row instead of one: the exponentials of a tile take no less time, 1235 against 877 us at 16384
 // tokens.)
@@ -55,6 +55,9 @@ constexpr int kRegs = 168, kRegsRows = 216, kRegsRest = 72;
 static_assert(8 * kRegsRows + 4 * kRegsRest <= 12 * kRegs, "more registers than the launch has would wait forever");
 constexpr int kBlockBytes = kTile * 128;  // 64 dimensions of 128 rows
 constexpr int kEarly = 96;      // keys of a tile whose weights are handed to the products before the others are computed
+// Weights are scaled by 2^kShift, up to 2^14 when the maximum lags by its 2^8: so that a half holds those of a
+// long, flat tail too (2^-30 of the largest), and none overflows.
+constexpr int kShift = 6;
 constexpr uint32_t kNever = 0x7fffffffu;
 // Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
 // at most three tiles.
@@ -545,7 +548,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                 }
             }
             // a row that has seen nothing: all weights 0; +inf among the scores: all NaN, as inf - inf is
-            const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : m * c;
+            const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : m * c - float(kShift);
             const uint64_t c2 = two(c, c), mc2 = two(-mc, -mc);
             uint64_t add[2] = {0, 0};
             // masked scores have to become 0: at a view's end the polynomial is not used

@@ -12,7 +12,7 @@ Rows follow the ragged packer's conventions (ops.pack_ragged): row r belongs to 
 row_seq[r] at position row_pos[r]; sequence s uses cache slot seq_slot[s].  q, k and v are
 [rows, heads, head_dim] tensors (float32, float16 or bfloat16; head_dim 64 or 128) whose last two
 dimensions are contiguous or are made so; rows may be strided, e.g. the q, k and v columns of one
-packed projection.  Index tensors are int32.  Calls run on the tensors' device, on its current
+packed projection.  Index tensors are contiguous int32.  Calls run on the tensors' device, on its current
 stream or the one given as the keyword `stream`, and can be captured in a CUDA graph.  Invalid
 arguments raise ValueError, TypeError or Exl3InvalidArgument (a ValueError).
 """
@@ -99,19 +99,19 @@ def _op(call):
     copies and allocates on the way is ordered with what it launches, and its memory belongs to s."""
 
     @functools.wraps(call)
-    def wrapper(first, *args, stream=None, **kw):
+    def wrapper(*args, stream=None, **kw):
         if stream is not None:
             if not hasattr(stream, "cuda_stream"):
                 stream = torch.cuda.ExternalStream(int(stream))
             with torch.cuda.stream(stream):
-                return wrapper(first, *args, **kw)
-        index = first.get_device()
+                return wrapper(*args, **kw)
+        index = (args[0] if args else kw["q"]).get_device()
         if index < 0:
             raise ValueError("operands must be on a CUDA device")
         if _current_device() != index:
             with torch.cuda.device(index):
-                return call(first, *args, **kw)
-        return call(first, *args, **kw)
+                return call(*args, **kw)
+        return call(*args, **kw)
 
     return wrapper
 
