@@ -458,9 +458,13 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 
 constexpr int kKeys = 64;        // keys per tile
 constexpr int kAttnWarps = 4;    // warps of a CTA, each with tiles of its own
+constexpr int kAttnThreads = 32 * kAttnWarps;
+constexpr int kAttnCtas = 3;     // per SM
+constexpr int kScanThreads = 128;
+static_assert(kAttnThreads >= kScanThreads, "the rows are scanned by the first 128 threads");
 constexpr int kStages = 2;       // tiles in flight per warp
 constexpr int kSplitRows = 256;  // rows up to which the tiles of all rows are cut into equal shares
-constexpr int kRowCost = 2;
+constexpr int kRowCost = 8;      // 8 rows between 1 and 32768 positions: 19.0 us with 2, 15.0 with 8, 15.1 with 12
 constexpr int kPlanFloats = 2 * kSplitRows;  // scratch begins with (first share, shares) of every row
 constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
 constexpr int kLazy = 6, kTop = 14 - kLazy;  // weights times value scales are up to 2^kTop, 2^14 before m moves
@@ -497,8 +501,8 @@ __device__ __forceinline__ int visible(const Kv4Attn & a, int r, int & slot) {
 __device__ __forceinline__ int tiles_of(int n) { return (max(n, 0) + kKeys - 1) / kKeys; }
 __device__ __forceinline__ int list_of(int n) { return n > 0 ? tiles_of(n) + kRowCost : 0; }
 
-// Visible keys and slots of rows 2 i and 2 i + 1 for thread i of 128, the list before them, and the whole
-// list's length.  sm: 4 ints.
+// Visible keys and slots of rows 2 i and 2 i + 1 for thread i of the first 128, the list before them, and the whole
+// list's length for every thread.  sm: 4 ints.
 __device__ __forceinline__ void scan_rows(const Kv4Attn & a, int (&n)[2], int (&slot)[2], int & before, int & total,
                                           int * sm) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -506,7 +510,7 @@ __device__ __forceinline__ void scan_rows(const Kv4Attn & a, int (&n)[2], int (&
     for (int i = 0; i < 2; ++i) {
         const int r = threadIdx.x * 2 + i;
         n[i] = -1;
-        if (r < a.rows) n[i] = visible(a, r, slot[i]);
+        if (r < a.rows && threadIdx.x < kScanThreads) n[i] = visible(a, r, slot[i]);
     }
     const int mine = list_of(n[0]) + list_of(n[1]);
     int upto = mine;
@@ -515,7 +519,7 @@ __device__ __forceinline__ void scan_rows(const Kv4Attn & a, int (&n)[2], int (&
         const int o = __shfl_up_sync(0xffffffffu, upto, x);
         if (lane >= x) upto += o;
     }
-    if (lane == 31) sm[warp] = upto;
+    if (lane == 31 && warp < kScanThreads / 32) sm[warp] = upto;
     __syncthreads();
     before = upto - mine;
     total = 0;
@@ -578,7 +582,7 @@ template <int D> __device__ __forceinline__ int key_of(int g) {
 }
 
 template <typename T, int D, int HC>
-__global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
+__global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4Attn a) {
     using Tile = Kv4Tile<D>;
     constexpr int G = D / 32, H = HC / 4;  // groups, heads of a lane's scores
     constexpr bool PAIR = HC == 4, LO = sizeof(T) == 4;  // a head to two columns; the second one its low halves
@@ -611,7 +615,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = threadIdx.x * 2 + i, list = list_of(n[i]);
-            if (r < a.rows) {
+            if (r < a.rows && r < kSplitRows) {
                 sm_n[r] = n[i];
                 sm_slot[r] = slot[i];
             }
@@ -620,7 +624,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
                 sm_row = r;
                 sm_off = begin - before;
             }
-            if (blockIdx.x == 0 && blockIdx.y == 0 && r < a.rows) {
+            if (blockIdx.x == 0 && blockIdx.y == 0 && r < a.rows && r < kSplitRows) {
                 const int x0 = before / share;
                 reinterpret_cast<int2 *>(a.part)[r] = make_int2(x0, n[i] > 0 ? (before + tiles_of(n[i]) - 1) / share - x0 + 1 : 0);
             }
@@ -926,7 +930,7 @@ __global__ void __launch_bounds__(128, 3) k_kv4_attn(const Kv4Attn a) {
         const bool whole = t0 == 0 && t1 == tiles;
         float * part = whole ? nullptr
                              : a.part + kPlanFloats + ((size_t(blockIdx.y) * gridDim.x + blockIdx.x) * 2 + (t0 ? 1 : 0)) * (HC * kRec);
-        for (int i = threadIdx.x; i < nh * D; i += 128) {
+        for (int i = threadIdx.x; i < nh * D; i += kAttnThreads) {
             const int h = i / D, d = i % D;
             const float * rec = reinterpret_cast<const float *>(ring_all) + h * kRec;
             constexpr int kNext = kStages * Tile::kBytes / 4;
@@ -1043,7 +1047,7 @@ AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     if (rows > kSplitRows) return p;
     // as many CTAs as are resident together (three per SM), no more than there can be shares
     const long long most = ((long long)rows * (c->max_len / kKeys + kRowCost) + kMinShare - 1) / kMinShare;
-    p.shares = int(std::max(1ll, std::min((long long)(3 * kSms / p.ys), most)));
+    p.shares = int(std::max(1ll, std::min((long long)(kAttnCtas * kSms / p.ys), most)));
     p.scratch = kPlanFloats * sizeof(float) + size_t(p.ys) * p.shares * 2 * p.heads_per_cta * (c->head_dim + 4) * sizeof(float);
     return p;
 }
@@ -1237,7 +1241,7 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
                 done.fetch_or(bit);
             }
             const int rc = attn_launch(k_kv4_attn<T, D, HC>, dim3(unsigned(p.shares ? p.shares : rows), unsigned(p.ys)),
-                                       dim3(128), size_t(smem), stream, a);
+                                       dim3(kAttnThreads), size_t(smem), stream, a);
             if (rc || !p.shares) return rc;
             // a row has about shares / rows parts: above 8, a CTA per head, below, one for all heads of a K/V head
             if (p.shares > 8 * rows)
