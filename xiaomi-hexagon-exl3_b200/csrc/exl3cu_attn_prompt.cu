@@ -58,6 +58,7 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 // Weights are scaled by 2^kShift, up to 2^14 when the maximum lags by its 2^8: so that a half holds those of a
 // long, flat tail too (2^-30 of the largest), and none overflows.
 constexpr int kShift = 6;
+constexpr int kOutBytes = 128;  // of a row that the epilogue writes at a time: what the smaller head has of 16-bit values
 constexpr uint32_t kNever = 0x7fffffffu;
 // Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
 // at most three tiles.
@@ -232,38 +233,50 @@ template <typename T> __device__ __forceinline__ uint32_t not_finite(uint32_t w)
 // Clears what is not finite in keys [first, 128) of the V tile at `tile` (whose keys start at `base`); first
 // keys that held a NaN, +inf or -inf go to seen[0 .. 2][dimension], keys from `keys` on are only cleared.
 template <typename T, int D>
-__device__ __noinline__ void clean_values(unsigned char * tile, int first, int base, int keys, uint32_t * seen,
-                                          uint32_t * dirty) {
+__device__ __noinline__ void clean_found(unsigned char * tile, int first, int base, int keys, uint32_t * seen,
+                                         uint32_t * dirty) {
     const int lane = threadIdx.x & 31;
     constexpr uint32_t e = std::is_same_v<T, __half> ? 0x7c00u : 0x7f80u;
-    constexpr uint32_t e2 = e | e << 16, one = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
-    // 8 lanes to a 128-byte row of a block, 4 rows at a time
     for (int b = 0; b < D / 64; ++b)
-#pragma unroll 8
         for (int r = (first & ~3) + (lane >> 3); r < kTile; r += 4) {
-            uint4 * at = reinterpret_cast<uint4 *>(tile + b * kBlockBytes + r * 128 + (lane & 7) * 16);
-            const uint4 w = *at;
-            // an exponent of all ones carries into the sign's place
-            const uint32_t any = (((w.x & e2) + one) | ((w.y & e2) + one) | ((w.z & e2) + one) | ((w.w & e2) + one)) & 0x80008000u;
-            if (any && r >= first) {
-                const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-                uint32_t o[4];
-                const int d0 = b * 64 + (((lane & 7) ^ (r & 7)) << 3);  // the swizzle: 16-byte chunk ^ (row mod 8)
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t mask = not_finite<T>(v[i]);
-                    o[i] = v[i] & ~mask;
-                    for (int h = 0; h < 2; ++h)
-                        if ((mask >> 16 * h & 1u) && base + r < keys) {
-                            const uint32_t x = v[i] >> 16 * h & 0xffffu;
-                            const int kind = (x & 0x7fffu) != e ? 0 : x & 0x8000u ? 2 : 1;
-                            atomicMin(seen + kind * D + d0 + 2 * i + h, uint32_t(base + r));
-                            *dirty = 1u;
-                        }
-                }
-                *at = make_uint4(o[0], o[1], o[2], o[3]);
+            uint32_t * at = reinterpret_cast<uint32_t *>(tile + b * kBlockBytes + r * 128 + (lane & 7) * 16);
+            const int d0 = b * 64 + (((lane & 7) ^ (r & 7)) << 3);  // the swizzle: 16-byte chunk ^ (row mod 8)
+            for (int i = 0; i < 4 && r >= first; ++i) {
+                const uint32_t v = at[i], mask = not_finite<T>(v);
+                if (!mask) continue;
+                at[i] = v & ~mask;
+                for (int h = 0; h < 2; ++h)
+                    if ((mask >> 16 * h & 1u) && base + r < keys) {
+                        const uint32_t x = v >> 16 * h & 0xffffu;
+                        const int kind = (x & 0x7fffu) != e ? 0 : x & 0x8000u ? 2 : 1;
+                        atomicMin(seen + kind * D + d0 + 2 * i + h, uint32_t(base + r));
+                        *dirty = 1u;
+                    }
             }
         }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the products read them
+}
+
+// The same; reads only where all is finite, which is what a short prompt waits for: the loads of a pass go out
+// together (64 16-byte loads a lane took 8700 cycles with the clearing between them).
+template <typename T, int D>
+__device__ __forceinline__ void clean_values(unsigned char * tile, int first, int base, int keys, uint32_t * seen,
+                                             uint32_t * dirty) {
+    const int lane = threadIdx.x & 31;
+    constexpr uint32_t e2 = std::is_same_v<T, __half> ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t one = std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+    uint32_t any = 0;
+    // 8 lanes to a 128-byte row of a block, 4 rows at a time; rows before `first` may be read, and decide nothing wrong
+    for (int r0 = first & ~31; r0 < kTile; r0 += 32)
+#pragma unroll
+        for (int b = 0; b < D / 64; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(tile + b * kBlockBytes + (r0 + 4 * i) * 128 + lane * 16);
+                // an exponent of all ones carries into the sign's place
+                any |= ((w.x & e2) + one) | ((w.y & e2) + one) | ((w.z & e2) + one) | ((w.w & e2) + one);
+            }
+    if (__any_sync(0xffffffffu, (any & 0x80008000u) != 0u)) clean_found<T, D>(tile, first, base, keys, seen, dirty);
     __syncwarp();
 }
 
@@ -301,6 +314,8 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             }
             bars.dirty = 0;
             mbar_init_fence();
+            for (const CUtensorMap * map : {&map_q, &map_k, &map_v})
+                asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
         }
     } else if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&bars.tmem)),
@@ -308,19 +323,29 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp == 0) {
         // which sequence and block: blocks of all sequences in order, counted from the end so that a
-        // sequence's longest block starts first
+        // sequence's longest block starts first.  A lane holds a sequence; up to 32 are read once.
         pdl_wait_primary();
-        int total = 0;
+        int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+        const auto read = [&](int s) {
+            q0 = q1 = k0 = k1 = 0;
+            if (s < a.n_seq) {
+                q0 = max(a.q_offsets[s], 0);
+                q1 = min(a.q_offsets[s + 1], a.q_rows);
+                k0 = min(max(a.kv_begin[s], 0), a.kv_rows);
+                k1 = max(min(a.kv_end[s], a.kv_rows), k0);
+            }
+            return q1 > q0 ? (q1 - q0 + 2 * ppt - 1) / (2 * ppt) : 0;
+        };
+        int total = 0, mine = 0;
         for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-            const int s = s0 + lane;
-            const int n = s < a.n_seq ? min(a.q_offsets[s + 1], a.q_rows) - max(a.q_offsets[s], 0) : 0;
-            total += __reduce_add_sync(0xffffffffu, unsigned(n > 0 ? (n + 2 * ppt - 1) / (2 * ppt) : 0));
+            mine = read(s0 + lane);
+            total += int(__reduce_add_sync(0xffffffffu, unsigned(mine)));
         }
-        int want = total - 1 - blk, seq = -1, before = 0;
+        int want = total - 1 - blk;
+        if (lane == 0) bars.seq = -1;
+        __syncwarp();
         for (int s0 = 0; want >= 0 && s0 < a.n_seq; s0 += 32) {
-            const int s = s0 + lane;
-            const int n = s < a.n_seq ? min(a.q_offsets[s + 1], a.q_rows) - max(a.q_offsets[s], 0) : 0;
-            const int mine = n > 0 ? (n + 2 * ppt - 1) / (2 * ppt) : 0;
+            if (a.n_seq > 32) mine = read(s0 + lane);
             int upto = mine;
 #pragma unroll
             for (int x = 1; x < 32; x <<= 1) {
@@ -329,22 +354,17 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             }
             const unsigned hit = __ballot_sync(0xffffffffu, want < upto);
             if (hit) {
-                const int src = __ffs(hit) - 1;
-                before = want - __shfl_sync(0xffffffffu, upto - mine, src);
-                seq = s0 + src;
+                if (lane == __ffs(hit) - 1) {
+                    bars.seq = s0 + lane;
+                    bars.q0 = q0;
+                    bars.q1 = q1;
+                    bars.k0 = k0;
+                    bars.k1 = k1;
+                    bars.p0 = (want - (upto - mine)) * 2 * ppt;
+                }
                 break;
             }
             want -= __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (lane == 0) {
-            bars.seq = seq;
-            if (seq >= 0) {
-                bars.q0 = max(a.q_offsets[seq], 0);
-                bars.q1 = min(a.q_offsets[seq + 1], a.q_rows);
-                bars.k0 = min(max(a.kv_begin[seq], 0), a.kv_rows);
-                bars.k1 = max(min(a.kv_end[seq], a.kv_rows), bars.k0);
-                bars.p0 = before * 2 * ppt;
-            }
         }
     }
     for (int i = threadIdx.x; i < 3 * D; i += kThreads) seen[i] = kNever;
@@ -589,42 +609,65 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             sum += added.x + added.y;
         }
         if (ok && tiles > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.o_done[t], 0));
+        if (ok && tiles == 0 && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_full, 0));  // a copy to the stage
         if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
         fence_after();
         const bool live = work && ok && p < nq;
         const float inv = lim > 0 ? 1.f / sum : 0.f;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         const long long at = live ? (long long)(q0 + p) * a.out_stride + head * D : 0;
+        // Rows go out by way of the query tile's memory (its products are complete), kOutBytes of a row at a time, so
+        // that its lanes write them together: a row to a lane and 16 bytes at a time take a wavefront per row.
+        unsigned char * const stage = sq + t * Sh::kTileBytes + (warp & 3) * 32 * kOutBytes;
+        const int passes = a.out_f32 ? D * 4 / kOutBytes : D * 2 / kOutBytes;
+        const int elems = a.out_f32 ? kOutBytes / 4 : kOutBytes / 2;  // of a row in a pass
+        for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll 1
-        for (int i = 0; i < D; i += 32) {
-            uint32_t o[32];
-            if (tiles > 0 && ok) {
-                tmem_ld(to + i, o);
-                wait_ld();
-            }
-            if (!live) continue;
-            float v[32];
+            for (int i = pass * elems; i < (pass + 1) * elems; i += 32) {
+                uint32_t o[32];
+                if (tiles > 0 && ok) {
+                    tmem_ld(to + i, o);
+                    wait_ld();
+                }
+                float v[32];
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = lim > 0 ? __uint_as_float(o[x]) * inv : 0.f;
-            if (dirty) {
+                for (int x = 0; x < 32; ++x) v[x] = lim > 0 ? __uint_as_float(o[x]) * inv : 0.f;
+                if (dirty) {
 #pragma unroll
-                for (int x = 0; x < 32; ++x) {
-                    if (seen[D + i + x] < uint32_t(lim)) v[x] += INFINITY;
-                    if (seen[2 * D + i + x] < uint32_t(lim)) v[x] -= INFINITY;
-                    if (seen[i + x] < uint32_t(lim)) v[x] = NAN;
+                    for (int x = 0; x < 32; ++x) {
+                        if (seen[D + i + x] < uint32_t(lim)) v[x] += INFINITY;
+                        if (seen[2 * D + i + x] < uint32_t(lim)) v[x] -= INFINITY;
+                        if (seen[i + x] < uint32_t(lim)) v[x] = NAN;
+                    }
+                }
+                const int c0 = (i - pass * elems) / (elems / (kOutBytes / 16));  // first 16-byte chunk
+                const auto put = [&](int chunk, uint4 w) {
+                    *reinterpret_cast<uint4 *>(stage + lane * kOutBytes + ((chunk ^ (lane & 7)) << 4)) = w;
+                };
+                if (a.out_f32) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        put(c0 + x, make_uint4(__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]),
+                                               __float_as_uint(v[4 * x + 2]), __float_as_uint(v[4 * x + 3])));
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        put(c0 + x, make_uint4(pack2<T>(v[8 * x], v[8 * x + 1]), pack2<T>(v[8 * x + 2], v[8 * x + 3]),
+                                               pack2<T>(v[8 * x + 4], v[8 * x + 5]), pack2<T>(v[8 * x + 6], v[8 * x + 7])));
                 }
             }
-            if (a.out_f32) {
-                float4 * dst = reinterpret_cast<float4 *>(static_cast<float *>(a.out) + at + i);
-#pragma unroll
-                for (int x = 0; x < 8; ++x) dst[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
-            } else {
-                uint4 * dst = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + at + i);
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    dst[x] = make_uint4(pack2<T>(v[8 * x], v[8 * x + 1]), pack2<T>(v[8 * x + 2], v[8 * x + 3]),
-                                        pack2<T>(v[8 * x + 4], v[8 * x + 5]), pack2<T>(v[8 * x + 6], v[8 * x + 7]));
+            __syncwarp();
+            constexpr int kChunks = kOutBytes / 16, kAtOnce = 32 / kChunks;  // rows written together
+            const int chunk = lane % kChunks;
+            const long long part = (long long)pass * kOutBytes + chunk * 16;
+#pragma unroll 4
+            for (int r = lane / kChunks; r < 32; r += kAtOnce) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(stage + r * kOutBytes + ((chunk ^ (r & 7)) << 4));
+                const long long row_at = __shfl_sync(0xffffffffu, at, r);
+                if (__shfl_sync(0xffffffffu, int(live), r))
+                    *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + row_at * (a.out_f32 ? 4 : 2) + part) = w;
             }
+            __syncwarp();
         }
     }
     fence_before();
