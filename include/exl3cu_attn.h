@@ -107,12 +107,16 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
  * result, whatever it holds.  Packed K/V: kv_begin = offsets, kv_end = offsets + 1.
  * dtype (q, k, v): EXL3CU_F16 or EXL3CU_BF16; scale > 0; out_dtype: the same or EXL3CU_F32.
  * Query rows outside every sequence are left as they were; q_rows is the rows
- * that d_q and d_out hold. */
+ * that d_q and d_out hold.  With d_scratch (exl3cu_prompt_attn_scratch_bytes()
+ * bytes, 16-byte aligned, contents arbitrary; calls that may run at the same time
+ * need scratch of their own) a call of few query rows and many keys divides the
+ * keys over the GPU; NULL: it does not. */
+size_t exl3cu_prompt_attn_scratch_bytes(int q_rows, int n_seq, int kv_rows, int heads, int kv_heads, int head_dim);
 int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void * d_k, size_t k_row_stride, size_t k_head_stride,
                        const void * d_v, size_t v_row_stride, size_t v_head_stride, int kv_rows, int dtype, int heads,
                        int kv_heads, int head_dim, const int32_t * d_q_offsets, const int32_t * d_kv_begin,
                        const int32_t * d_kv_end, int n_seq, int q_rows, float scale, void * d_out, size_t out_stride,
-                       int out_dtype, void * stream);
+                       int out_dtype, void * d_scratch, size_t scratch_bytes, void * stream);
 
 /* The calls above for bindings whose conversion of arguments costs more than a launch (ctypes: 24 arguments
  * about 6 us): `words` are the arguments of the call in order, 8 bytes each; integers and pointers as 64-bit

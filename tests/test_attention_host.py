@@ -93,14 +93,14 @@ def test_bad_attend_arguments_are_refused(L, kw):
 
 
 PROMPT = dict(q=P, qs=2048, k=P, krs=512, khs=128, v=P, vrs=512, vhs=128, kv_rows=10, dtype=1, heads=16, kv=4, dim=128,
-              qo=P, b=P, e=P, n=1, rows=10, scale=1.0, out=P, os=2048, ot=1, stream=Z)
+              qo=P, b=P, e=P, n=1, rows=10, scale=1.0, out=P, os=2048, ot=1, scratch=P, bytes=1 << 40, stream=Z)
 
 
 @pytest.mark.parametrize("kw", [
     dict(dtype=0), dict(dtype=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan), dict(scale=math.inf), dict(ot=4), dict(dim=80), dict(heads=15), dict(kv=0), dict(heads=2048, qs=1 << 20),
     dict(n=-1), dict(rows=-1), dict(kv_rows=-1), dict(q=None), dict(q=P + 2), dict(qs=2044), dict(qs=1024), dict(k=None),
     dict(krs=100), dict(krs=132), dict(khs=64), dict(vhs=129), dict(v=P + 8), dict(qo=None), dict(b=None), dict(e=None),
-    dict(out=None), dict(os=2040), dict(krs=1 << 40)])
+    dict(out=None), dict(os=2040), dict(krs=1 << 40), dict(kv_rows=10000, bytes=1000), dict(kv_rows=10000, scratch=P + 8)])
 def test_bad_prompt_arguments_are_refused(L, kw):
     assert L.exl3cu_prompt_attn(*{**PROMPT, **kw}.values()) == INVALID
     assert b"prompt_attn" in L.exl3cu_last_error()
@@ -153,7 +153,7 @@ def test_rope_frequencies():
 BY_WORDS = [
     (0, "PiPiiiiiiPPPfPiifPiiPiiP", ROPE, [dict(dim=96), dict(dtype=2), dict(kot=9), dict(kv=-1), dict(rotary=24), dict(ks=511),
                                           dict(pos=None), dict(kos=500), dict(heads=2000)]),
-    (4, "PiPiiPiiiiiiiPPPiifPiiP", PROMPT, [dict(dtype=0), dict(ot=4), dict(scale=-1.0), dict(kv_rows=-1), dict(khs=64),
+    (4, "PiPiiPiiiiiiiPPPiifPiiPiP", PROMPT, [dict(dtype=0), dict(ot=4), dict(scale=-1.0), dict(kv_rows=-1), dict(khs=64),
                                            dict(e=None), dict(out=None), dict(krs=1 << 40)])]
 
 

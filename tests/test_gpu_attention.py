@@ -436,6 +436,50 @@ def test_prompt_not_finite_where_masked(A, value):
     assert bool(got[170:].isnan().all())
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("heads,kv,dim,q_lens,past", [
+    (16, 4, 128, [1], 20000), (16, 4, 128, [130], 5001), (8, 2, 64, [3, 100, 1], 2500), (2, 2, 128, [300, 17], 900),
+    (16, 4, 128, [512], 1500)])
+def test_prompt_keys_divided_among_ctas(A, dtype, heads, kv, dim, q_lens, past):
+    """Few query rows behind long starts: the keys of a block are shared and the parts joined; without scratch
+    a block keeps its keys."""
+    g = gen(past + heads)
+    rows, kv_lens = sum(q_lens), [n + past * (i + 1) // len(q_lens) for i, n in enumerate(q_lens)]
+    assert A.prompt_scratch_bytes(rows, len(q_lens), sum(kv_lens), heads, kv, dim) > 0
+    q = (randn(g, rows, heads, dim) * 1.5).to(dtype)
+    k, v = (randn(g, sum(kv_lens), kv, dim).to(dtype) for _ in range(2))
+    ko = offsets(kv_lens)
+    spans = list(zip(ko.tolist(), ko.tolist()[1:]))
+    out = torch.full((rows + 3, heads, dim), 5.0, device="cuda").to(dtype)
+    padded = torch.cat((q, q.new_zeros(3, heads, dim)))
+    A.prompt_attention(padded, k, v, offsets(q_lens), ko, out=out)
+    check_prompt(out, q, k, v, q_lens, spans)
+    assert bool((out[rows:] == 5).all())
+    whole = A.prompt_attention(q, k, v, offsets(q_lens), ko, scratch=torch.empty(0, dtype=torch.uint8, device="cuda"))
+    check_prompt(whole, q, k, v, q_lens, spans)
+
+
+def test_prompt_divided_keys_not_finite(A):
+    """The same rules for what is seen and what is not when a block's keys are shared."""
+    g = gen(31)
+    n, m = 100, 4000
+    q = randn(g, n, 4, 128).bfloat16()
+    k, v = randn(g, m, 1, 128).bfloat16(), randn(g, m, 1, 128).bfloat16()
+    v[m - 40, 0, 3] = math.inf      # seen by the last 40 rows
+    v[m - 20, 0, 3] = -math.inf     # and this by the last 20
+    v[100, 0, 9] = math.nan         # seen by all, far from the end
+    clean = v.clone()
+    clean[m - 40, 0, 3] = clean[m - 20, 0, 3] = clean[100, 0, 9] = 0
+    got = A.prompt_attention(q, k, v, ints([0, n]), ints([0, m]))
+    want = A.prompt_attention(q, k, clean, ints([0, n]), ints([0, m]))
+    keep = [d for d in range(128) if d not in (3, 9)]
+    assert torch.equal(got[..., keep], want[..., keep]) and bool(got[..., 9].isnan().all())
+    assert torch.equal(got[:60, :, 3], want[:60, :, 3])
+    assert bool((got[61:80, :, 3] == math.inf).all()) and bool(got[81:, :, 3].isnan().all())
+    none = A.prompt_attention(q, k[:30], v[:30], ints([0, n]), ints([0, 30]))
+    assert bool((none[:70] == 0).all())
+
+
 def test_prompt_long_flat_tail(A):
     """One strong key before 20000 weak ones, each 2^-26 of it: together they move the result, and no part of
     them is lost to the 16-bit weights."""

@@ -59,6 +59,8 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 // long, flat tail too (2^-30 of the largest), and none overflows.
 constexpr int kShift = 6;
 constexpr int kOutBytes = 128;  // of a row that the epilogue writes at a time: what the smaller head has of 16-bit values
+constexpr int kMinSplit = 6;    // tiles of keys of a share at least, where a block's keys are shared among CTAs
+constexpr int kMaxSplits = 16;
 constexpr uint32_t kNever = 0x7fffffffu;
 // Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
 // at most three tiles.
@@ -80,6 +82,8 @@ struct PromptArgs {
     const int32_t * kv_end;
     int n_seq, q_rows, kv_rows, heads, kv_heads, out_f32;
     int log_p;        // heads per group P = 1 << log_p
+    int splits;       // CTAs that share a block's keys, blockIdx.y; more than 1 only with scratch
+    float * part;     // [blocks][splits][2 kTile][D] accumulators, then as many (reference, sum)
     float scale_log2; // scale * log2(e)
 };
 
@@ -218,10 +222,68 @@ template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float 
     return y;
 }
 
+// A block of query rows: positions p0 .. of a sequence with query rows [q0, q1) and keys [k0, k1).
+struct Work {
+    int seq;  // -1: none
+    int q0, q1, k0, k1, p0;
+};
+
+// Block `blk` of the call, by one warp: blocks of all sequences in order, counted from the end so that a
+// sequence's longest block starts first.  A lane holds a sequence; up to 32 are read once.
+__device__ __forceinline__ void find_block(const PromptArgs & a, int blk, Work & out) {
+    const int lane = threadIdx.x & 31, positions = 2 * kTile >> a.log_p;
+    int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
+    const auto read = [&](int s) {
+        q0 = q1 = k0 = k1 = 0;
+        if (s < a.n_seq) {
+            q0 = max(a.q_offsets[s], 0);
+            q1 = min(a.q_offsets[s + 1], a.q_rows);
+            k0 = min(max(a.kv_begin[s], 0), a.kv_rows);
+            k1 = max(min(a.kv_end[s], a.kv_rows), k0);
+        }
+        return q1 > q0 ? (q1 - q0 + positions - 1) / positions : 0;
+    };
+    int total = 0, mine = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
+        mine = read(s0 + lane);
+        total += int(__reduce_add_sync(0xffffffffu, unsigned(mine)));
+    }
+    int want = total - 1 - blk;
+    if (lane == 0) out.seq = -1;
+    __syncwarp();
+    for (int s0 = 0; want >= 0 && s0 < a.n_seq; s0 += 32) {
+        if (a.n_seq > 32) mine = read(s0 + lane);
+        int upto = mine;
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) {
+            const int o = __shfl_up_sync(0xffffffffu, upto, x);
+            if (lane >= x) upto += o;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, want < upto);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) out = Work{s0 + lane, q0, q1, k0, k1, (want - (upto - mine)) * positions};
+            break;
+        }
+        want -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+    __syncwarp();
+}
+
+// How a block's keys are shared: tiles of a share, shares that have any.
+struct Split {
+    int tiles, used;
+};
+__device__ __forceinline__ Split split_of(const PromptArgs & a, const Work & w) {
+    const int nq = w.q1 - w.q0, last = min(w.p0 + (2 * kTile >> a.log_p), nq) - 1;  // the block's last position sees most
+    const int all = (max(0, last + 1 + (w.k1 - w.k0) - nq) + kTile - 1) / kTile;
+    const int tiles = a.splits > 1 ? max(kMinSplit, (all + a.splits - 1) / a.splits) : max(all, 1);
+    return Split{tiles, max(1, (all + tiles - 1) / tiles)};
+}
+
 struct Bars {
     uint64_t full[8], empty[8], q_full, clean[kMasked], s_full[2], p_full[2][2], o_done[2];
     uint32_t tmem, dirty;
-    int seq, q0, q1, k0, k1, p0;  // the CTA's work; q1 <= q0: none
+    Work work;
 };
 
 // Elements of a 16-bit pair whose exponent is all ones, as a mask of the pair.
@@ -322,60 +384,24 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                      "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     } else if (warp == 0) {
-        // which sequence and block: blocks of all sequences in order, counted from the end so that a
-        // sequence's longest block starts first.  A lane holds a sequence; up to 32 are read once.
         pdl_wait_primary();
-        int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
-        const auto read = [&](int s) {
-            q0 = q1 = k0 = k1 = 0;
-            if (s < a.n_seq) {
-                q0 = max(a.q_offsets[s], 0);
-                q1 = min(a.q_offsets[s + 1], a.q_rows);
-                k0 = min(max(a.kv_begin[s], 0), a.kv_rows);
-                k1 = max(min(a.kv_end[s], a.kv_rows), k0);
-            }
-            return q1 > q0 ? (q1 - q0 + 2 * ppt - 1) / (2 * ppt) : 0;
-        };
-        int total = 0, mine = 0;
-        for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
-            mine = read(s0 + lane);
-            total += int(__reduce_add_sync(0xffffffffu, unsigned(mine)));
-        }
-        int want = total - 1 - blk;
-        if (lane == 0) bars.seq = -1;
-        __syncwarp();
-        for (int s0 = 0; want >= 0 && s0 < a.n_seq; s0 += 32) {
-            if (a.n_seq > 32) mine = read(s0 + lane);
-            int upto = mine;
-#pragma unroll
-            for (int x = 1; x < 32; x <<= 1) {
-                const int o = __shfl_up_sync(0xffffffffu, upto, x);
-                if (lane >= x) upto += o;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, want < upto);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    bars.seq = s0 + lane;
-                    bars.q0 = q0;
-                    bars.q1 = q1;
-                    bars.k0 = k0;
-                    bars.k1 = k1;
-                    bars.p0 = (want - (upto - mine)) * 2 * ppt;
-                }
-                break;
-            }
-            want -= __shfl_sync(0xffffffffu, upto, 31);
-        }
+        find_block(a, blk, bars.work);
     }
     for (int i = threadIdx.x; i < 3 * D; i += kThreads) seen[i] = kNever;
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = bars.tmem;
-    const bool work = bars.seq >= 0;
-    const int q0 = bars.q0, k0 = bars.k0, keys = bars.k1 - bars.k0, nq = bars.q1 - bars.q0, p0 = bars.p0;
-    // keys that position p of the sequence sees, and the tiles of each query tile
-    const auto sees = [&](int p) { return p < nq ? max(0, min(keys, p + 1 + keys - nq)) : 0; };
+    // the CTA's share of the block's keys, as if there were no others: every position's view is cut to it
+    const Work blockwork = bars.work;
+    const Split split = split_of(a, blockwork);
+    const bool work = blockwork.seq >= 0 && int(blockIdx.y) < split.used;
+    const int key0 = a.splits > 1 ? int(blockIdx.y) * split.tiles * kTile : 0;
+    const bool part = split.used > 1;
+    const int q0 = blockwork.q0, k0 = blockwork.k0 + key0, nq = blockwork.q1 - blockwork.q0, p0 = blockwork.p0;
+    const int all_keys = blockwork.k1 - blockwork.k0, keys = part ? min(all_keys - key0, split.tiles * kTile) : all_keys;
+    // keys of the share that position p of the sequence sees, and the tiles of each query tile
+    const auto sees = [&](int p) { return p < nq ? max(0, min(keys, p + 1 + all_keys - nq - key0)) : 0; };
     const auto tiles_of = [&](int t) {
         const int first = p0 + t * ppt;
         return !work || first >= nq ? 0 : (sees(min(first + ppt, nq) - 1) + kTile - 1) / kTile;
@@ -613,14 +639,22 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
         fence_after();
         const bool live = work && ok && p < nq;
-        const float inv = lim > 0 ? 1.f / sum : 0.f;
+        const float inv = part ? 1.f : lim > 0 ? 1.f / sum : 0.f;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
-        const long long at = live ? (long long)(q0 + p) * a.out_stride + head * D : 0;
+        // a share's part goes to scratch as it is, in f32, with what its weights refer to
+        const bool f32 = part || a.out_f32;
+        const size_t rec = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile + row;
+        char * const out = static_cast<char *>(part ? a.part : a.out);
+        const long long at = part ? (long long)rec * D : live ? (long long)(q0 + p) * a.out_stride + head * D : 0;
+        if (part && live) {
+            const float mr = m == -INFINITY ? m : m == INFINITY ? NAN : m * c - float(kShift);
+            reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
+        }
         // Rows go out by way of the query tile's memory (its products are complete), kOutBytes of a row at a time, so
         // that its lanes write them together: a row to a lane and 16 bytes at a time take a wavefront per row.
         unsigned char * const stage = sq + t * Sh::kTileBytes + (warp & 3) * 32 * kOutBytes;
-        const int passes = a.out_f32 ? D * 4 / kOutBytes : D * 2 / kOutBytes;
-        const int elems = a.out_f32 ? kOutBytes / 4 : kOutBytes / 2;  // of a row in a pass
+        const int passes = f32 ? D * 4 / kOutBytes : D * 2 / kOutBytes;
+        const int elems = f32 ? kOutBytes / 4 : kOutBytes / 2;  // of a row in a pass
         for (int pass = 0; pass < passes; ++pass) {
 #pragma unroll 1
             for (int i = pass * elems; i < (pass + 1) * elems; i += 32) {
@@ -644,7 +678,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                 const auto put = [&](int chunk, uint4 w) {
                     *reinterpret_cast<uint4 *>(stage + lane * kOutBytes + ((chunk ^ (lane & 7)) << 4)) = w;
                 };
-                if (a.out_f32) {
+                if (f32) {
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
                         put(c0 + x, make_uint4(__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]),
@@ -659,13 +693,13 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             __syncwarp();
             constexpr int kChunks = kOutBytes / 16, kAtOnce = 32 / kChunks;  // rows written together
             const int chunk = lane % kChunks;
-            const long long part = (long long)pass * kOutBytes + chunk * 16;
+            const long long column = (long long)pass * kOutBytes + chunk * 16;
 #pragma unroll 4
             for (int r = lane / kChunks; r < 32; r += kAtOnce) {
                 const uint4 w = *reinterpret_cast<const uint4 *>(stage + r * kOutBytes + ((chunk ^ (r & 7)) << 4));
                 const long long row_at = __shfl_sync(0xffffffffu, at, r);
                 if (__shfl_sync(0xffffffffu, int(live), r))
-                    *reinterpret_cast<uint4 *>(static_cast<char *>(a.out) + row_at * (a.out_f32 ? 4 : 2) + part) = w;
+                    *reinterpret_cast<uint4 *>(out + row_at * (f32 ? 4 : 2) + column) = w;
             }
             __syncwarp();
         }
@@ -674,6 +708,62 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
     __syncthreads();
     if (warp == 9)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+}
+
+// Joins a block's shares, in order: a warp to a row of the block, 32 rows to a CTA.  Bound by the bytes of the parts.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) k_prompt_merge(const PromptArgs a) {
+    __shared__ Work sm_work;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_trigger();
+    pdl_wait_primary();
+    const int groups = a.heads >> a.log_p;
+    if (warp == 0) find_block(a, int(blockIdx.x) / groups, sm_work);
+    __syncthreads();
+    const Work w = sm_work;
+    if (w.seq < 0) return;
+    const int used = split_of(a, w).used, nq = w.q1 - w.q0;
+    if (used <= 1) return;
+    constexpr int E = D / 32;
+    for (int i = 0; i < 4; ++i) {
+        const int row = blockIdx.y * 32 + warp * 4 + i;  // of the block's two tiles
+        const int p = w.p0 + (row >> a.log_p), head = ((int(blockIdx.x) % groups) << a.log_p) + (row & ((1 << a.log_p) - 1));
+        if (p >= nq) continue;
+        const size_t rec = size_t(blockIdx.x) * a.splits * (2 * kTile) + row;
+        const float2 * refs = reinterpret_cast<const float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D) + rec;
+        float2 mine = lane < used ? refs[lane * (2 * kTile)] : make_float2(-INFINITY, 0.f);
+        float o[kMaxSplits][E];
+#pragma unroll
+        for (int z = 0; z < kMaxSplits; ++z) {
+            if (z >= used) break;
+            const float * x = a.part + (rec + size_t(z) * (2 * kTile)) * D + lane * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[z][e] = x[e];
+        }
+        float top = mine.x;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        const float f = exp2_fast(mine.x - (top == -INFINITY ? 0.f : top));
+        float sum = mine.y * f;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        float v[E] = {};
+#pragma unroll
+        for (int z = 0; z < kMaxSplits; ++z) {
+            if (z >= used) break;
+            const float fz = __shfl_sync(0xffffffffu, f, z);
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = fmaf(o[z][e], fz, v[e]);
+        }
+        const bool any = p + 1 + w.k1 - w.k0 - nq > 0;
+        const long long at = (long long)(w.q0 + p) * a.out_stride + head * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float y = any ? v[e] / sum : 0.f;
+            if (a.out_f32) static_cast<float *>(a.out)[at + e] = y;
+            else static_cast<T *>(a.out)[at + e] = from_f32<T>(y);
+        }
+    }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -722,8 +812,31 @@ int launch(const PromptArgs & a, const CUtensorMap (&maps)[3], unsigned blocks, 
             return api_fail(EXL3CU_NO_SUPPORT, "prompt_attn: built with another number of registers than it divides up");
         done.fetch_or(bit);
     }
-    return attn_launch(k_prompt_attn<T, D>, dim3(blocks), dim3(kThreads), size_t(Shape<D>::kSmem), stream, a, maps[0],
-                       maps[1], maps[2]);
+    const int rc = attn_launch(k_prompt_attn<T, D>, dim3(blocks, unsigned(a.splits)), dim3(kThreads), size_t(Shape<D>::kSmem),
+                               stream, a, maps[0], maps[1], maps[2]);
+    if (rc || a.splits == 1) return rc;
+    return attn_launch(k_prompt_merge<T, D>, dim3(blocks, 2 * kTile / 32), dim3(256), 0, stream, a);
+}
+
+constexpr int kSms = 148;  // a B200's
+
+struct Plan {
+    int log_p;         // heads per CTA: the power of two in heads / kv_heads, at most 16
+    long long blocks;  // of all sequences: at most one part block per sequence more than the rows fill
+    int splits;
+    size_t scratch;
+};
+
+// A block's keys are shared among CTAs where the blocks alone leave most SMs idle (a prompt's chunk of 512 rows
+// behind a long start is 32 blocks for 148 SMs) and there are keys for it.
+Plan plan_prompt(int q_rows, int n_seq, int kv_rows, int heads, int kv_heads, int head_dim) {
+    Plan p{};
+    while (p.log_p < 4 && (heads / kv_heads) % (2 << p.log_p) == 0) ++p.log_p;
+    p.blocks = ((long long)q_rows / (2 * kTile >> p.log_p) + n_seq) * (heads >> p.log_p);
+    const long long tiles = ((long long)kv_rows + kTile - 1) / kTile;
+    p.splits = int(std::max(1ll, std::min({kSms / std::max(p.blocks, 1ll), (tiles + kMinSplit - 1) / kMinSplit, (long long)kMaxSplits})));
+    p.scratch = p.splits > 1 ? size_t(p.blocks) * p.splits * (2 * kTile) * (head_dim + 2) * sizeof(float) : 0;
+    return p;
 }
 
 }  // namespace
@@ -746,7 +859,7 @@ extern "C" int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void 
                                   int kv_rows, int dtype, int heads, int kv_heads, int head_dim,
                                   const int32_t * d_q_offsets, const int32_t * d_kv_begin, const int32_t * d_kv_end,
                                   int n_seq, int q_rows, float scale, void * d_out, size_t out_stride, int out_dtype,
-                                  void * stream) {
+                                  void * d_scratch, size_t scratch_bytes, void * stream) {
     const auto bad = [](const char * what) { return api_fail(EXL3CU_INVALID_ARGUMENT, what); };
     if (head_dim != 64 && head_dim != 128) return bad("prompt_attn: head_dim must be 64 or 128");
     if (dtype != EXL3CU_F16 && dtype != EXL3CU_BF16) return bad("prompt_attn: q, k and v must be f16 or bf16");
@@ -769,11 +882,12 @@ extern "C" int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void 
         return bad("prompt_attn: k or v null or misaligned, or a stride below head_dim or no multiple of 8");
     if (!d_q_offsets || !d_kv_begin || !d_kv_end) return bad("prompt_attn: offsets are NULL");
 
-    int log_p = 0;  // heads per CTA: the power of two in heads / kv_heads, at most 16
-    while (log_p < 4 && (heads / kv_heads) % (2 << log_p) == 0) ++log_p;
-    const int positions = 2 * kTile >> log_p;
-    // blocks of all sequences: at most one part block per sequence more than the rows fill
-    const long long blocks = ((long long)q_rows / positions + n_seq) * (heads >> log_p);
+    Plan plan = plan_prompt(q_rows, n_seq, kv_rows, heads, kv_heads, head_dim);
+    if (!d_scratch) plan.splits = 1;  // without scratch a block has its keys to itself
+    else if (plan.splits > 1 && (scratch_bytes < plan.scratch || !aligned(d_scratch)))
+        return bad("prompt_attn: scratch misaligned or too small (exl3cu_prompt_attn_scratch_bytes)");
+    const int log_p = plan.log_p;
+    const long long blocks = plan.blocks;
     if (blocks > 0x7fffffffll) return bad("prompt_attn: too many query rows");
     const bool bf16 = dtype == EXL3CU_BF16;
     CUtensorMap maps[3];
@@ -786,10 +900,17 @@ extern "C" int exl3cu_prompt_attn(const void * d_q, size_t q_stride, const void 
                 any ? v_head_stride : head_dim, any ? v_row_stride : head_dim, 1, kTile))
         return api_fail(EXL3CU_CUDA_ERROR, "prompt_attn: cuTensorMapEncodeTiled failed");
     const PromptArgs a{d_out, (long long)out_stride, d_q_offsets, d_kv_begin, d_kv_end, n_seq, q_rows, kv_rows, heads,
-                       kv_heads, out_dtype == EXL3CU_F32, log_p, scale * 1.4426950408889634f};
+                       kv_heads, out_dtype == EXL3CU_F32, log_p, plan.splits, static_cast<float *>(d_scratch),
+                       scale * 1.4426950408889634f};
     if (!bf16)
         return head_dim == 128 ? launch<__half, 128>(a, maps, unsigned(blocks), stream)
                                : launch<__half, 64>(a, maps, unsigned(blocks), stream);
     return head_dim == 128 ? launch<__nv_bfloat16, 128>(a, maps, unsigned(blocks), stream)
                            : launch<__nv_bfloat16, 64>(a, maps, unsigned(blocks), stream);
+}
+
+extern "C" size_t exl3cu_prompt_attn_scratch_bytes(int q_rows, int n_seq, int kv_rows, int heads, int kv_heads,
+                                                   int head_dim) {
+    if (q_rows <= 0 || n_seq <= 0 || kv_rows <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || head_dim <= 0) return 0;
+    return plan_prompt(q_rows, n_seq, kv_rows, heads, kv_heads, head_dim).scratch;
 }

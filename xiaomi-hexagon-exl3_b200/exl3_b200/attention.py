@@ -53,7 +53,9 @@ def _lib():
         L.exl3cu_kv4_attn_scratch_bytes.argtypes = [C, _I, _I]
         L.exl3cu_kv4_attn.argtypes = [C, _P, _S, _I, _I, _I, _P, _P, _P, _I, _F, _P, _S, _P, _S, _P]
         L.exl3cu_prompt_attn.argtypes = [_P, _S, _P, _S, _S, _P, _S, _S, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _F,
-                                         _P, _S, _I, _P]
+                                         _P, _S, _I, _P, _S, _P]
+        L.exl3cu_prompt_attn_scratch_bytes.restype = _S
+        L.exl3cu_prompt_attn_scratch_bytes.argtypes = [_I] * 6
         for name in ("exl3cu_qk_norm_rope", "exl3cu_kv4_append", "exl3cu_kv4_read", "exl3cu_kv4_attn",
                      "exl3cu_prompt_attn"):
             getattr(L, name).restype = _I
@@ -84,7 +86,13 @@ _rope_call = _call(0, "PiPiiiiiiPPPfPiifPiiPiiP")
 _append_call = _call(1, "PPiPiiiPPPiP")
 _read_call = _call(2, "PPPiiPiPiiP")
 _attn_call = _call(3, "PPiiiiPPPifPiPiP")
-_prompt_call = _call(4, "PiPiiPiiiiiiiPPPiifPiiP")
+_prompt_call = _call(4, "PiPiiPiiiiiiiPPPiifPiiPiP")
+
+
+@functools.lru_cache(maxsize=4096)
+def prompt_scratch_bytes(q_rows: int, n_seq: int, kv_rows: int, heads: int, kv_heads: int, head_dim: int) -> int:
+    """Scratch with which prompt_attention divides the keys of few query rows over the GPU (0: it would not)."""
+    return _lib().exl3cu_prompt_attn_scratch_bytes(q_rows, n_seq, kv_rows, heads, kv_heads, head_dim)
 
 
 _current_device = torch.cuda.current_device
@@ -398,13 +406,14 @@ def _kv(name, t, index, dtype, dim):
 
 @_op
 def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_end=None, scale: float | None = None,
-                     out=None):
+                     out=None, scratch=None):
     """Causal attention of packed sequences (exl3cu_prompt_attn): q [q_rows, heads, D], k and v
     [kv_rows, kv_heads, D], float16 or bfloat16; sequence s has query rows q_offsets[s] .. q_offsets[s+1]
     and key rows kv_offsets[s] .. kv_offsets[s+1] (or kv_begin[s] .. kv_end[s], for rows that lie in a
     slot cache).  Its last query sees all of its keys, the one before all but the last, and so on; a query
     that sees none becomes zero.  out may be float32 or of q's type; query rows outside every sequence are
-    left as they were (undefined where out is allocated here)."""
+    left as they were (undefined where out is allocated here).  scratch: a uint8 tensor of
+    prompt_scratch_bytes() that no other call uses at the same time; allocated per call when not given."""
     index, dtype = q.get_device(), q.dtype
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError("q, k and v must be float16 or bfloat16")
@@ -429,11 +438,18 @@ def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_e
         out, os_ = torch.empty_like(q, memory_format=_packed), heads * dim
     else:
         os_ = _into("out", out, rows, heads, dim, index, (dtype, torch.float32))
-    _prompt_call(qp, qs, kp, krs, khs, vp, vrs, vhs, k.shape[0], _DTYPES[dtype], heads,
-                 k.shape[1], dim, _index("q_offsets", q_offsets, n + 1, index), begin, end, n,
+    kv_rows, kv = k.shape[0], k.shape[1]
+    held = prompt_scratch_bytes(rows, n, kv_rows, heads, kv, dim) if scratch is None else scratch.numel() * scratch.element_size()
+    if scratch is None:
+        if held:
+            scratch = torch.empty(held, dtype=torch.uint8, device=q.device)
+    elif scratch.get_device() != index or not scratch.is_contiguous():
+        raise ValueError("scratch must be contiguous memory of q's device")
+    _prompt_call(qp, qs, kp, krs, khs, vp, vrs, vhs, kv_rows, _DTYPES[dtype], heads,
+                 kv, dim, _index("q_offsets", q_offsets, n + 1, index), begin, end, n,
                  rows, dim ** -0.5 if scale is None else scale, out.data_ptr(), os_,
-                 _DTYPES[out.dtype], _stream(index))
+                 _DTYPES[out.dtype], scratch.data_ptr() if held else 0, held, _stream(index))
     return out
 
 
-__all__ = ["Kv4Cache", "qk_norm_rope", "prompt_attention", "rope_frequencies"]
+__all__ = ["Kv4Cache", "qk_norm_rope", "prompt_attention", "prompt_scratch_bytes", "rope_frequencies"]
