@@ -438,7 +438,7 @@ def test_prompt_not_finite_where_masked(A, value):
 
 @pytest.mark.parametrize("dtype", TYPES[1:])
 @pytest.mark.parametrize("heads,kv,dim,q_lens,past", [
-    (16, 4, 128, [1], 20000), (16, 4, 128, [130], 5001), (8, 2, 64, [3, 100, 1], 2500), (2, 2, 128, [300, 17], 900),
+    (16, 4, 128, [1], 20000), (16, 4, 128, [130], 5001), (8, 2, 64, [3, 100, 1], 2500), (2, 2, 128, [300, 17], 1900),
     (16, 4, 128, [512], 1500)])
 def test_prompt_keys_divided_among_ctas(A, dtype, heads, kv, dim, q_lens, past):
     """Few query rows behind long starts: the keys of a block are shared and the parts joined; without scratch

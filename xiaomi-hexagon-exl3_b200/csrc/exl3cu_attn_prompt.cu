@@ -59,7 +59,9 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 // long, flat tail too (2^-30 of the largest), and none overflows.
 constexpr int kShift = 6;
 constexpr int kOutBytes = 128;  // of a row that the epilogue writes at a time: what the smaller head has of 16-bit values
-constexpr int kMinSplit = 6;    // tiles of keys of a share at least, where a block's keys are shared among CTAs
+// Tiles of keys of a share at least, where a block's keys are shared among CTAs: 512 rows behind 1000 keys 21.9 us
+// with 4, 24.6 with 6, 30.1 with 10, 26.9 without sharing; behind 4000 keys 30.9, 30.8, 32.2 and 65.6.
+constexpr int kMinSplit = 4;
 constexpr int kMaxSplits = 16;
 constexpr uint32_t kNever = 0x7fffffffu;
 // Tiles of keys in which some row's view ends: a CTA's rows see at most 255 keys more than its first, which is
@@ -830,11 +832,12 @@ struct Plan {
 // A block's keys are shared among CTAs where the blocks alone leave most SMs idle (a prompt's chunk of 512 rows
 // behind a long start is 32 blocks for 148 SMs) and there are keys for it.
 Plan plan_prompt(int q_rows, int n_seq, int kv_rows, int heads, int kv_heads, int head_dim) {
-    Plan p{};
+    Plan p{0, 0, 1, 0};
     while (p.log_p < 4 && (heads / kv_heads) % (2 << p.log_p) == 0) ++p.log_p;
     p.blocks = ((long long)q_rows / (2 * kTile >> p.log_p) + n_seq) * (heads >> p.log_p);
     const long long tiles = ((long long)kv_rows + kTile - 1) / kTile;
-    p.splits = int(std::max(1ll, std::min({kSms / std::max(p.blocks, 1ll), (tiles + kMinSplit - 1) / kMinSplit, (long long)kMaxSplits})));
+    if (tiles >= 3 * kMinSplit)  // two short shares and joining them take as long as one
+        p.splits = int(std::max(1ll, std::min({kSms / std::max(p.blocks, 1ll), tiles / kMinSplit, (long long)kMaxSplits})));
     p.scratch = p.splits > 1 ? size_t(p.blocks) * p.splits * (2 * kTile) * (head_dim + 2) * sizeof(float) : 0;
     return p;
 }
