@@ -282,6 +282,26 @@ __device__ __forceinline__ Split split_of(const PromptArgs & a, const Work & w) 
     return Split{tiles, max(1, (all + tiles - 1) / tiles)};
 }
 
+// A CTA's share of its block, as if there were no other keys: every position's view is cut to it.
+struct View {
+    bool work, part;  // part: other CTAs have shares of the block too
+    int q0, k0, nq, p0, keys, ahead;
+    __device__ __forceinline__ View(const PromptArgs & a, const Work & w) {
+        const Split split = split_of(a, w);
+        work = w.seq >= 0 && int(blockIdx.y) < split.used;
+        part = split.used > 1;
+        const int key0 = part ? int(blockIdx.y) * split.tiles * kTile : 0, all = w.k1 - w.k0;
+        q0 = w.q0;
+        k0 = w.k0 + key0;
+        nq = w.q1 - w.q0;
+        p0 = w.p0;
+        keys = part ? min(all - key0, split.tiles * kTile) : all;
+        ahead = all - nq - key0;
+    }
+    // keys of the share that position p of the sequence sees
+    __device__ __forceinline__ int sees(int p) const { return work && p < nq ? max(0, min(keys, p + 1 + ahead)) : 0; }
+};
+
 struct Bars {
     uint64_t full[8], empty[8], q_full, clean[kMasked], s_full[2], p_full[2][2], o_done[2];
     uint32_t tmem, dirty;
@@ -394,24 +414,15 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
     __syncthreads();
     fence_after();
     const uint32_t tmem = bars.tmem;
-    // the CTA's share of the block's keys, as if there were no others: every position's view is cut to it
-    const Work blockwork = bars.work;
-    const Split split = split_of(a, blockwork);
-    const bool work = blockwork.seq >= 0 && int(blockIdx.y) < split.used;
-    const int key0 = a.splits > 1 ? int(blockIdx.y) * split.tiles * kTile : 0;
-    const bool part = split.used > 1;
-    const int q0 = blockwork.q0, k0 = blockwork.k0 + key0, nq = blockwork.q1 - blockwork.q0, p0 = blockwork.p0;
-    const int all_keys = blockwork.k1 - blockwork.k0, keys = part ? min(all_keys - key0, split.tiles * kTile) : all_keys;
-    // keys of the share that position p of the sequence sees, and the tiles of each query tile
-    const auto sees = [&](int p) { return p < nq ? max(0, min(keys, p + 1 + all_keys - nq - key0)) : 0; };
+    const View view(a, bars.work);
     const auto tiles_of = [&](int t) {
-        const int first = p0 + t * ppt;
-        return !work || first >= nq ? 0 : (sees(min(first + ppt, nq) - 1) + kTile - 1) / kTile;
+        const int first = view.p0 + t * ppt;
+        return first >= view.nq ? 0 : (view.sees(min(first + ppt, view.nq) - 1) + kTile - 1) / kTile;
     };
     const int nt[2] = {tiles_of(0), tiles_of(1)};
     const int n = max(nt[0], nt[1]);
-    const int all_see = work ? sees(p0) : 0;  // keys that every row of the CTA sees
-    const int masked0 = all_see / kTile;      // first tile of keys in which some row's view ends
+    const int all_see = view.sees(view.p0);  // keys that every row of the CTA sees
+    const int masked0 = all_see / kTile;     // first tile of keys in which some row's view ends
 
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
@@ -423,7 +434,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                 mbar_arrive_expect_tx(&bars.q_full, uint32_t(2 * Sh::kTileBytes));
                 for (int t = 0; t < 2; ++t)
                     for (int b = 0; b < Sh::kBlocks; ++b)
-                        tma_load(sq + t * Sh::kTileBytes + b * kBlockBytes, &map_q, b * 64, head0, q0 + p0 + t * ppt,
+                        tma_load(sq + t * Sh::kTileBytes + b * kBlockBytes, &map_q, b * 64, head0, view.q0 + view.p0 + t * ppt,
                                  &bars.q_full);
             }
             bool ok = true;
@@ -437,7 +448,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                             mbar_arrive_expect_tx(&bars.full[slot], uint32_t(Sh::kTileBytes));
                             for (int b = 0; b < Sh::kBlocks; ++b)
                                 tma_load(ring + slot * Sh::kTileBytes + b * kBlockBytes, w ? &map_v : &map_k, b * 64,
-                                         kvh, k0 + j * kTile, &bars.full[slot]);
+                                         kvh, view.k0 + j * kTile, &bars.full[slot]);
                         }
                         ok = __all_sync(0xffffffffu, ok);
                     }
@@ -448,7 +459,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     ok = __all_sync(0xffffffffu, mbar_wait_sleep(&bars.full[slot], unsigned(vi / Sh::kSlots) & 1u));
                     if (ok) {
                         clean_values<T, D>(ring + slot * Sh::kTileBytes, max(0, all_see - (j - 1) * kTile), (j - 1) * kTile,
-                                           keys, seen, &bars.dirty);
+                                           view.keys, seen, &bars.dirty);
                         if (lane == 0) mbar_arrive(&bars.clean[j - 1 - masked0]);
                     }
                 }
@@ -552,9 +563,8 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const int t = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
-        const int p = p0 + t * ppt + (row >> a.log_p), head = head0 + (row & ((1 << a.log_p) - 1));
-        const int lim = work ? sees(p) : 0;
-        const int tile_sees = work ? sees(p0 + t * ppt) : 0;
+        const int lim = view.sees(view.p0 + t * ppt + (row >> a.log_p));
+        const int tile_sees = view.sees(view.p0 + t * ppt);
         const float c = a.scale_log2;
         float m = -INFINITY, sum = 0.f;
         const int tiles = nt[t];
@@ -640,14 +650,17 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         if (ok && tiles == 0 && n > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars.q_full, 0));  // a copy to the stage
         if (!ok && lane == 0) atomicOr(&g_prompt_status, kStatusWaitTimeout);
         fence_after();
-        const bool live = work && ok && p < nq;
+        // read again: the loop needs the registers
+        const View end(a, bars.work);
+        const int p = end.p0 + t * ppt + (row >> a.log_p), head = head0 + (row & ((1 << a.log_p) - 1));
+        const bool live = end.work && ok && p < end.nq, part = end.part;
         const float inv = part ? 1.f : lim > 0 ? 1.f / sum : 0.f;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         // a share's part goes to scratch as it is, in f32, with what its weights refer to
         const bool f32 = part || a.out_f32;
         const size_t rec = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile + row;
         char * const out = static_cast<char *>(part ? a.part : a.out);
-        const long long at = part ? (long long)rec * D : live ? (long long)(q0 + p) * a.out_stride + head * D : 0;
+        const long long at = part ? (long long)rec * D : live ? (long long)(end.q0 + p) * a.out_stride + head * D : 0;
         if (part && live) {
             const float mr = m == -INFINITY ? m : m == INFINITY ? NAN : m * c - float(kShift);
             reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
