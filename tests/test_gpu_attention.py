@@ -310,6 +310,17 @@ def test_attend_long_and_many_rows(A):
     check_attend(got, q, cache, [1 - i % 2 for i in range(150)], lens)
 
 
+def test_attend_as_many_rows_as_are_cut_into_shares(A):
+    g = gen(22)
+    cache = A.Kv4Cache(256, 1, 128, 128)
+    fill(cache, g)
+    lens = [int(x) for x in torch.randint(1, 129, (256,), generator=g, device="cuda")]
+    q = randn(g, 256, 2, 128)
+    order = torch.randperm(256, generator=g, device="cuda").to(torch.int32)
+    got = cache.attend(q, ints(list(range(256))), ints([n - 1 for n in lens]), order)
+    check_attend(got, q, cache, order.tolist(), lens)
+
+
 def test_attend_more_rows_than_are_cut_into_shares(A):
     """Above 256 rows a CTA takes a row whole; rows of no position and of no sequence among them."""
     g = gen(21)
@@ -494,6 +505,52 @@ def test_prompt_long_flat_tail(A):
     got = A.prompt_attention(q=q[-200:], k=k, v=v, q_offsets=ints([0, 200]), kv_offsets=ints([0, n]), scale=scale,
                              out=torch.empty((200, 1, 64), device="cuda"))
     check_prompt(got, q[-200:], k, v, [200], [(0, n)], scale)
+
+
+def test_prompt_many_sequences_and_rows_before_the_first(A):
+    """More sequences than a warp has lanes, empty ones among them; rows before the first one are left alone."""
+    g = gen(17)
+    lens = [(i * 7) % 40 for i in range(75)]
+    q_offs = torch.tensor([9] + lens, device="cuda").cumsum(0).to(torch.int32)
+    rows = int(q_offs[-1])
+    kv_lens = [n + (i % 3) * 50 if n else 0 for i, n in enumerate(lens)]
+    ko = offsets(kv_lens)
+    q = randn(g, rows, 8, 64).half()
+    k, v = randn(g, sum(kv_lens), 2, 64).half(), randn(g, sum(kv_lens), 2, 64).half()
+    out = torch.full((rows, 8, 64), 4.0, device="cuda").half()
+    A.prompt_attention(q, k, v, q_offs, ko, out=out)
+    assert bool((out[:9] == 4).all())
+    check_prompt(out[9:], q[9:], k, v, lens, list(zip(ko.tolist(), ko.tolist()[1:])))
+
+
+def test_captured_read_and_prompt_with_other_lengths(A):
+    """A captured step replayed for other lengths of the same capacity: offsets are read on the device."""
+    g = gen(18)
+    cache = A.Kv4Cache(3, 2, 320, 128)
+    fill(cache, g)
+    cap_q, cap_kv = 200, 900
+    q = randn(g, cap_q, 8, 128).half()
+    slots, q_offs, kv_offs = ints([2, 0, 1]), ints([0, 10, 20, 30]), ints([0, 10, 20, 30])
+    k, v = (torch.zeros((cap_kv, 2, 128), device="cuda").half() for _ in range(2))
+    out = torch.zeros((cap_q, 8, 128), device="cuda").half()
+    stream = torch.cuda.Stream()
+
+    def step():
+        cache.read(slots, kv_offs, cap_kv, k_out=k, v_out=v)
+        A.prompt_attention(q, k, v, q_offs, kv_offs, out=out)
+
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for lens, kv_lens in (([1, 150, 3], [300, 200, 3]), ([0, 0, 200], [0, 0, 320]), ([66, 65, 64], [66, 320, 100])):
+        q_offs.copy_(offsets(lens))
+        kv_offs.copy_(offsets(kv_lens))
+        graph.replay()
+        o = offsets(kv_lens).tolist()
+        check_prompt(out, q, k, v, lens, list(zip(o, o[1:])))
 
 
 def test_prompt_in_a_slot_cache_and_strided(A):
