@@ -375,6 +375,26 @@ def test_attend_extreme_values(A):
     assert bool(out[0, 5].isnan().all()) and bool(out[0, :5].isfinite().all()) and bool(out[0, 6:].isfinite().all())
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("dim,value", [(128, math.nan), (64, math.inf)])
+def test_attend_a_group_of_values_not_finite(A, dtype, dim, value):
+    """A NaN among the visible values reaches the dimensions of its group; the others are as exact as ever."""
+    g = gen(23)
+    cache = A.Kv4Cache(1, 2, 256, dim)
+    fill(cache, g)
+    G = dim // 32
+    cache.v_scales[0, 0, 5, 1] = value
+    q = randn(g, 3, 8, dim).to(dtype)
+    clean = A.Kv4Cache.from_tensors(cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales.nan_to_num(0, 0, 0))
+    at = (ints([0, 0, 0]), ints([199, 6, 4]), ints([0]))
+    got, want = cache.attend(q, *at), clean.attend(q, *at)
+    d = torch.arange(dim, device="cuda") % G == 1
+    # row 2 does not see position 5; heads 4 .. 7 read the other K/V head
+    assert not bool(got[:2, :4][..., d].isfinite().any())
+    got[:2, :4] = torch.where(d, want[:2, :4], got[:2, :4])
+    check_attend(got, q, clean, [0, 0, 0], [200, 7, 5])
+
+
 def ref_prompt(q, k, v, q_lens, kv_spans, scale):
     outs, tols = [], []
     heads, share = q.shape[1], q.shape[1] // k.shape[1]

@@ -799,6 +799,15 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 #pragma unroll
                 for (int i = 1; i < G; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
                 top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)) >> 10;
+                if (top == 31u) {  // not finite: its group of dimensions is, and the others' weights keep their range
+                    top = 0;
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
+                        top = max(top, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                    }
+                    top = __reduce_max_sync(0xffffffffu, top) >> 10;
+                }
             }
             const int grown = max(int(top) - ev, 0);
             bool moved = grown > 0;
