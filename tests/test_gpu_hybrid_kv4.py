@@ -90,6 +90,37 @@ def test_captured_and_multi_step_decoding_give_the_eager_tokens(engine):
     assert got[0] == got[1] == eager
 
 
+def test_captured_prompt_step_at_other_positions(engine):
+    """A prompt chunk captured at the start of a context and replayed further on."""
+    eng = engine
+    prompt = np.random.default_rng(4).integers(0, eng.cfg.vocab, 60).astype(np.int32)
+
+    def upload(p):
+        eng.meta.fill(prompt[p:p + 20], [0] * 20, list(range(p, p + 20)), [0, 20], [1], [19])
+        eng.meta.upload(None)
+
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    eng.reset_slot(1)
+    want = []
+    for p in (0, 20, 40):
+        upload(p)
+        torch.cuda.synchronize()
+        eng.forward(20, 1, 1, stream=stream)
+        torch.cuda.synchronize()
+        want.append(eng.mix[:20].clone())
+    eng.reset_slot(1)
+    upload(0)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        eng.forward(20, 1, 1, stream=stream)
+    for p, w in zip((0, 20, 40), want):
+        upload(p)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(eng.mix[:20], w)
+
+
 def test_continuous_admission(engine):
     """More requests than slots, prefill chunks between decode rows."""
     from exl3_b200.hybrid import Request, run_requests

@@ -447,7 +447,9 @@ class HybridEngine:
         if decode:
             cache.attend(q_out, row_seq, row_pos, slot, out=mix, scratch=self.kv4_scratch, stream=stream)
             return
-        offsets, total = m.view("kv_offsets")[:n_seq + 1], m.kv_total
+        # a captured step is replayed for other positions: all that the contexts can come to
+        total = self.slots * self.max_len if self.torch.cuda.is_current_stream_capturing() else m.kv_total
+        offsets = m.view("kv_offsets")[:n_seq + 1]
         k16, v16 = self.kv16[0, :total], self.kv16[1, :total]
         cache.read(slot, offsets, total, k_out=k16, v_out=v16, stream=stream)
         attention.prompt_attention(q_out, k16, v16, m.view("row_offsets")[:n_seq + 1], offsets, out=mix, stream=stream)
