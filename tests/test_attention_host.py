@@ -170,3 +170,18 @@ def test_calls_by_words_are_the_calls(L, which, kinds, args, bad):
         assert L.exl3cu_attn_words(which, words) == want == (INVALID if kw != dict(rows=0) else 0)
         assert L.exl3cu_last_error() == text
     assert L.exl3cu_attn_words(which, None) == INVALID and L.exl3cu_attn_words(9, b"") == INVALID
+
+
+def test_stream_of_another_device_is_refused():
+    from types import SimpleNamespace
+
+    from exl3_b200 import attention
+
+    q = SimpleNamespace(get_device=lambda: 0)
+    s = SimpleNamespace(cuda_stream=0, device=torch.device("cuda", 1))
+    with pytest.raises(ValueError, match="stream"):
+        attention.qk_norm_rope(q, None, None, stream=s)
+    with pytest.raises(TypeError):
+        attention.qk_norm_rope()
+    with pytest.raises(ValueError, match="CUDA device"):
+        attention.qk_norm_rope(torch.zeros(1, 1, 64), None, None)

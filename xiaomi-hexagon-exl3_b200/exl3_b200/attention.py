@@ -108,14 +108,19 @@ def _op(call):
 
     @functools.wraps(call)
     def wrapper(*args, stream=None, **kw):
-        if stream is not None:
-            if not hasattr(stream, "cuda_stream"):
-                stream = torch.cuda.ExternalStream(int(stream))
-            with torch.cuda.stream(stream):
-                return wrapper(*args, **kw)
-        index = (args[0] if args else kw["q"]).get_device()
+        first = args[0] if args else kw.get("q")
+        if first is None:
+            return call(*args, **kw)  # names the missing argument
+        index = first.get_device()
         if index < 0:
             raise ValueError("operands must be on a CUDA device")
+        if stream is not None:
+            if not hasattr(stream, "cuda_stream"):
+                stream = torch.cuda.ExternalStream(int(stream), device=index)
+            if stream.device.index != index:
+                raise ValueError("stream must be of the operands' device")
+            with torch.cuda.stream(stream):
+                return wrapper(*args, **kw)
         if _current_device() != index:
             with torch.cuda.device(index):
                 return call(*args, **kw)
