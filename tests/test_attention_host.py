@@ -172,6 +172,18 @@ def test_calls_by_words_are_the_calls(L, which, kinds, args, bad):
     assert L.exl3cu_attn_words(which, None) == INVALID and L.exl3cu_attn_words(9, b"") == INVALID
 
 
+def test_native_calls_leave_what_is_not_ordinary():
+    """Wrong types, unknown or doubled keywords, tensors without a GPU: all left to the Python functions."""
+    from exl3_b200 import attention
+
+    mod, t = attention._native(), torch.zeros(2, 4, 64)
+    for name in ("qk_norm_rope", "append", "read", "attend", "prompt_attention"):
+        call = getattr(mod, name)
+        for args, kw in (((), {}), ((t, t, t), {}), ((t,) * 12, {}), ((None, 1, "x"), {}), ((t, t), {"q": t}),
+                         ((t, t), {"nothing": 1}), ((t, t, t, t, t), {}), ((t, t, t, t), {"scale": "x"})):
+            assert call(*args, **kw) is NotImplemented, (name, len(args), kw)
+
+
 def test_stream_of_another_device_is_refused():
     from types import SimpleNamespace
 

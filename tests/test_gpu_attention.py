@@ -640,6 +640,36 @@ def test_layer_in_4_bits(A):
         check_attend(result, qs, cache, slots, [n + t + 1 for n in lens])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_native_and_python_calls_agree(A, dtype):
+    """The native module and the Python functions, which take the calls that it leaves, launch the same."""
+    g = gen(31)
+    qkv = randn(g, 6, 16, 64).to(dtype)
+    q, k, v = qkv[:, :8], qkv[:, 8:12], qkv[:, 12:]
+    pos, seq, slots = ints([3, 4, 5, 0, 1, 2]), ints([0, 0, 0, 1, 1, 1]), ints([1, 0])
+    inv, w = torch.tensor(A.rope_frequencies(32)[0], device="cuda"), randn(g, 64)
+    caches = [A.Kv4Cache(2, 4, 64, 64) for _ in range(2)]
+    got = []
+    for cache, form in zip(caches, (lambda f: f, lambda f: f.__wrapped__)):
+        r = list(form(A.qk_norm_rope)(q, k, pos, inv, w, None, eps=1e-5, interleaved=True, attention_factor=1.5,
+                                      out_dtype=torch.float32))
+        r += form(A.qk_norm_rope)(q, k, pos, q_out=torch.empty_like(q), k_weight=w)
+        assert form(A.Kv4Cache.append)(cache, k, v, seq, pos, slots) is None
+        r += form(A.Kv4Cache.read)(cache, slots, ints([0, 6, 9]), 9, dtype)
+        out = torch.zeros(6, 8, 64, device="cuda", dtype=dtype)
+        same = form(A.Kv4Cache.attend)(cache, q, seq, pos, slots, 0.2, out=out)
+        assert same is out
+        r += [out, form(A.Kv4Cache.attend)(cache, q, seq, pos, slots, scratch=torch.empty(1 << 20, dtype=torch.uint8, device="cuda"))]
+        if dtype != torch.float32:
+            kw = dict(kv_begin=ints([0, 3]), kv_end=ints([3, 6]))
+            r += [form(A.prompt_attention)(q, k, v, ints([0, 3, 6]), **kw),
+                  form(A.prompt_attention)(q, k, v, ints([0, 3, 6]), ints([0, 3, 6]), scale=1, out=torch.empty(6, 8, 64, device="cuda"))]
+        r += [cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales]
+        got.append(r)
+    for a, b in zip(*got):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
 def test_calls_on_two_streams_at_once(A):
     """Calls that overlap on two streams, given as arguments, leave each other's results alone."""
     g = gen(14)

@@ -1,18 +1,20 @@
-"""Build libexl3cu.so (sm_100a) and libexl3cu_ggml.so in-tree with nvcc.
+"""Build libexl3cu.so (sm_100a), libexl3cu_ggml.so and exl3cu_torch.so in-tree with nvcc and g++.
 
     python xiaomi-hexagon-exl3_b200/build.py [--verbose-ptxas] [--force]
 
-Objects go to xiaomi-hexagon-exl3_b200/_build/ (git-ignored); the two shared
+Objects go to xiaomi-hexagon-exl3_b200/_build/ (git-ignored); the shared
 libraries land next to this file so they travel with the source tree.
 """
 from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -22,6 +24,7 @@ INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 LIB = PKG / "libexl3cu.so"
 GGML_LIB = PKG / "libexl3cu_ggml.so"
+TORCH_LIB = PKG / "exl3cu_torch.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CUDA_SOURCES = ["exl3cu_api.cu", "exl3cu_kernels.cu", "exl3cu_gemv.cu", "exl3cu_gemv_cluster.cu", "exl3cu_gemv_mul1.cu",
@@ -85,6 +88,14 @@ def build(verbose_ptxas: bool = False, force: bool = False, quiet: bool = True) 
         _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{CSRC / 'ggml_stub'}",
               str(gsrc), "-o", str(GGML_LIB), f"-L{PKG}", "-lexl3cu",
               f"-Wl,-rpath,$ORIGIN"])
+    # the attention operators' calls with torch tensors (a Python extension module)
+    tsrc = CSRC / "exl3cu_attn_torch.cpp"
+    if force or _newer(TORCH_LIB, [tsrc, INCLUDE / "exl3cu.h", INCLUDE / "exl3cu_attn.h"]):
+        torch = Path(importlib.util.find_spec("torch").origin).parent
+        cuda = Path(cc).resolve().parents[1]
+        inc = [f"-I{p}" for p in (INCLUDE, torch / "include", cuda / "include", sysconfig.get_paths()["include"])]
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *inc, str(tsrc), "-o", str(TORCH_LIB),
+              f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
     if verbose_ptxas and not quiet:
         print("\n".join(logs))
     return LIB

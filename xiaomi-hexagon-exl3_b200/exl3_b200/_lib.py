@@ -11,6 +11,7 @@ from pathlib import Path
 PKG_DIR = Path(__file__).resolve().parents[1]
 LIB_PATH = PKG_DIR / "libexl3cu.so"
 GGML_LIB_PATH = PKG_DIR / "libexl3cu_ggml.so"
+TORCH_LIB_PATH = PKG_DIR / "exl3cu_torch.so"
 
 OK, INVALID_ARGUMENT, NO_SUPPORT, OUT_OF_MEMORY, CUDA_ERROR = range(5)
 F32, F16 = 0, 1

@@ -20,12 +20,14 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import struct
 
 import numpy as np
 import torch
 
-from ._lib import check, lib
+from ._lib import TORCH_LIB_PATH, check, lib
 
 BF16 = 4
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: BF16}
@@ -65,6 +67,19 @@ def _lib():
     return _L
 
 
+@functools.lru_cache(maxsize=None)
+def _native():
+    """csrc/exl3cu_attn_torch.cpp: the calls below in ordinary form (NotImplemented for any other)."""
+    L = _lib()
+    loader = importlib.machinery.ExtensionFileLoader("exl3cu_torch", str(TORCH_LIB_PATH))
+    mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("exl3cu_torch", loader))
+    loader.exec_module(mod)
+    mod.bind(*(ctypes.cast(getattr(L, "exl3cu_" + n), _P).value
+               for n in ("qk_norm_rope", "kv4_append", "kv4_read", "kv4_attn_scratch_bytes", "kv4_attn",
+                         "prompt_attn_scratch_bytes", "prompt_attn")))
+    return mod
+
+
 def _call(which, types):
     """A call by exl3cu_attn_words: arguments of the given kinds (P: address or None, i: integer, f: float) are
     packed into words, which takes ctypes a fraction of the time that converting them one by one does."""
@@ -102,12 +117,24 @@ _i32, _f32t, _packed = torch.int32, torch.float32, torch.contiguous_format
 
 
 def _op(call):
-    """An operator's entry.  It runs on the device of its first tensor argument (or of the cache that it is a
-    method of), whatever the current one is.  With stream=s it runs as if s were the current stream: what it
-    copies and allocates on the way is ordered with what it launches, and its memory belongs to s."""
+    """An operator's entry.  Calls in ordinary form (the current device, no copies to make) are carried out by the
+    native module; the Python function copies or refuses, and does the others.  It runs on the device of its first
+    tensor argument (or of the cache that it is a method of), whatever the current one is.  With stream=s it runs as
+    if s were the current stream: what it copies and allocates on the way is ordered with what it launches, and its
+    memory belongs to s."""
+    fast = None
 
     @functools.wraps(call)
     def wrapper(*args, stream=None, **kw):
+        nonlocal fast
+        if stream is None:
+            if fast is None:
+                fast = getattr(_native(), call.__name__)
+            result = fast(*args, **kw)
+            if result is not NotImplemented:
+                if result.__class__ is int:
+                    check(result)
+                return result
         first = args[0] if args else kw.get("q")
         if first is None:
             return call(*args, **kw)  # names the missing argument
@@ -343,7 +370,6 @@ class Kv4Cache:
                    _stream(index))
         return k_out, v_out
 
-    @_op
     def scratch_bytes(self, rows: int, heads: int) -> int:
         """Scratch that attend() needs for `rows` rows of `heads` query heads."""
         key = (rows, heads)
