@@ -106,18 +106,20 @@ __device__ __forceinline__ void rope_angle(int pos, float f, float factor, float
     sn *= factor;
 }
 
-// Four elements, 8 or 16 bytes, as floats.
-template <typename T> __device__ __forceinline__ void load4(const T * p, float * x) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    } else {
-        const uint2 v = *reinterpret_cast<const uint2 *>(p);
-        const T * e = reinterpret_cast<const T *>(&v);
+// Eight elements as they lie, and as floats side by side.
+template <typename T> struct Eight {
+    static constexpr int kWords = sizeof(T) / 2;
+    uint4 raw[kWords];
+    __device__ __forceinline__ void load(const T * p) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = to_f32(e[i]);
+        for (int i = 0; i < kWords; ++i) raw[i] = reinterpret_cast<const uint4 *>(p)[i];
     }
-}
+    __device__ __forceinline__ void get(uint64_t * x) const {
+        const T * e = reinterpret_cast<const T *>(raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = two(to_f32(e[2 * i]), to_f32(e[2 * i + 1]));
+    }
+};
 
 __device__ __forceinline__ void store4(void * p, int dtype, long long at, const float * x) {
     if (dtype == EXL3CU_F32) {
@@ -133,19 +135,49 @@ __device__ __forceinline__ void store4(void * p, int dtype, long long at, const 
     }
 }
 
-// D/8 threads to a head, each with two runs of four dimensions that hold both members of its pairs ((4 j, half + 4 j)
-// or 8 consecutive ones), so that the rotation needs no exchange.  A thread keeps its head (with its weights and
-// addresses) and goes through the CTA's rows, the next row's loads under way; the rows' angles are computed once for
-// all heads, kRopeRows rows at a time, into shared memory.  Bound by the bytes of q and k in and out; a call of few
-// rows by latency.  The CTAs of a call are resident together, each with an equal number of rows.
-constexpr int kRopeThreads = 512;    // at most: heads beyond kRopeThreads / (D / 8) are taken in turn
-constexpr int kRopeRows = 8;
-constexpr int kRopePerSm = 1024;     // threads resident on an SM
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(uint64_t x) {
+    const float2 v = of_two(x);
+    if constexpr (std::is_same_v<T, __half>) {
+        const __half2 y = __floats2half2_rn(v.x, v.y);
+        return *reinterpret_cast<const uint32_t *>(&y);
+    } else {
+        const __nv_bfloat162 y = __floats2bfloat162_rn(v.x, v.y);
+        return *reinterpret_cast<const uint32_t *>(&y);
+    }
+}
+
+// Eight elements as `dtype`.
+__device__ __forceinline__ void store8(void * p, int dtype, long long at, const uint64_t * x) {
+    if (dtype == EXL3CU_F32) {
+        ulonglong2 * to = reinterpret_cast<ulonglong2 *>(static_cast<float *>(p) + at);
+        to[0] = make_ulonglong2(x[0], x[1]);
+        to[1] = make_ulonglong2(x[2], x[3]);
+    } else if (dtype == EXL3CU_F16) {
+        *reinterpret_cast<uint4 *>(static_cast<__half *>(p) + at) =
+            make_uint4(pack_pair<__half>(x[0]), pack_pair<__half>(x[1]), pack_pair<__half>(x[2]), pack_pair<__half>(x[3]));
+    } else {
+        *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p) + at) =
+            make_uint4(pack_pair<__nv_bfloat16>(x[0]), pack_pair<__nv_bfloat16>(x[1]), pack_pair<__nv_bfloat16>(x[2]),
+                       pack_pair<__nv_bfloat16>(x[3]));
+    }
+}
+
+// D/16 threads to a head, each with two runs of eight dimensions that hold both members of its pairs ((8 j, half + 8 j)
+// or 16 consecutive ones), so that the rotation needs no exchange.  A thread keeps its head (with its weights and
+// addresses) and goes through the CTA's rows, the loads of the next kAhead under way; the rows' angles are computed once
+// for all heads, kRopeRows rows at a time, into shared memory, behind the first rows' loads.  The CTAs of a call are
+// resident together, each with an equal number of rows.  Bound by the bytes of q and k in and out (8191 rows of 20 heads of
+// 16 bits, 84 MB: 17.7 us, 4.7 TB/s); a call of few rows by latency (2.7 us).  What it took there: 8 dimensions a thread,
+// in accesses of 8 bytes, 26.2 us; kAhead 1 18.8; 8 rows of angles at a time 18.1.
+constexpr int kRopeThreads = 320;    // at most: heads beyond kRopeThreads / (D / 16) are taken in turn
+constexpr int kRopeRows = 16;
+constexpr int kAhead = 2;
+constexpr int kRopePerSm = 640;      // threads resident on an SM
 
 // SAME: the outputs are of the inputs' type.
 template <typename T, int D, bool SAME>
 __global__ void __launch_bounds__(kRopeThreads, 2) k_qk_norm_rope(const RopeArgs a) {
-    constexpr int L = D / 8;
+    constexpr int L = D / 16;
     constexpr int kType = std::is_same_v<T, float> ? EXL3CU_F32 : std::is_same_v<T, __half> ? EXL3CU_F16 : EXL3CU_BF16;
     __shared__ __align__(16) float sm_cos[2][kRopeRows * (D / 2)], sm_sin[2][kRopeRows * (D / 2)];
     __shared__ int sm_pos[2][kRopeRows];
@@ -154,14 +186,30 @@ __global__ void __launch_bounds__(kRopeThreads, 2) k_qk_norm_rope(const RopeArgs
     // the CTA's rows: an equal share
     const int first = int((long long)a.rows * blockIdx.x / gridDim.x), last = int((long long)a.rows * (blockIdx.x + 1) / gridDim.x);
     // the thread's two runs of dimensions, and the first of its pairs' frequencies where it rotates
-    int d0 = 8 * j, d1 = 8 * j + 4, f0 = a.interleaved ? 4 * j : -1;
-    if (!a.interleaved && 4 * j < half) d0 = f0 = 4 * j, d1 = half + 4 * j;
+    int d0 = 16 * j, d1 = 16 * j + 8, f0 = a.interleaved ? 8 * j : -1;
+    if (!a.interleaved && 8 * j < half) d0 = f0 = 8 * j, d1 = half + 8 * j;
     const bool turns = a.interleaved ? d0 < a.rotary : f0 >= 0;
     f0 = max(f0, 0);
     const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
     pdl_wait_primary();
     for (int row0 = first, buf = 0; row0 < last; row0 += kRopeRows, buf ^= 1) {
         const int rows = min(kRopeRows, last - row0);
+        Eight<T> ahead[kAhead][2];
+        const T * x;
+        long long stride;
+        const auto start = [&](int h) {  // the first rows of head h
+            const bool is_q = h < a.heads;
+            stride = is_q ? a.q_stride : a.k_stride;
+            x = (is_q ? static_cast<const T *>(a.q) + h * D : static_cast<const T *>(a.k) + (h - a.heads) * D) + row0 * stride;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u, x += stride)
+                if (u < rows) {
+                    ahead[u][0].load(x + d0);
+                    ahead[u][1].load(x + d1);
+                }
+        };
+        int h = threadIdx.x / L;
+        if (h < per_row) start(h);
         if (threadIdx.x < rows) sm_pos[buf][threadIdx.x] = a.row_pos[row0 + threadIdx.x];
         for (int i = threadIdx.x; i < rows * half; i += blockDim.x) {
             const int ar = i / half, f = i - ar * half, pos = a.row_pos[row0 + ar];
@@ -170,71 +218,78 @@ __global__ void __launch_bounds__(kRopeThreads, 2) k_qk_norm_rope(const RopeArgs
             sm_cos[buf][ar * (D / 2) + f] = cs;
             sm_sin[buf][ar * (D / 2) + f] = sn;
         }
-        bool ready = false;
-        for (int h = threadIdx.x / L; h < per_row || !ready; h += step) {
-            const bool is_q = h < a.heads, any = h < per_row;
-            const int kh = h - a.heads;
-            const T * x = is_q ? static_cast<const T *>(a.q) + row0 * a.q_stride + h * D
-                               : static_cast<const T *>(a.k) + row0 * a.k_stride + kh * D;
-            const long long stride = is_q ? a.q_stride : a.k_stride, out_stride = is_q ? a.q_out_stride : a.k_out_stride;
+        __syncthreads();  // the angles; with two buffers the next chunk's are not those still in use
+        while (h < per_row) {
+            const bool is_q = h < a.heads;
+            const long long out_stride = is_q ? a.q_out_stride : a.k_out_stride;
             const float * weights = is_q ? a.q_w : a.k_w;
             void * out = is_q ? a.q_out : a.k_out;
             const int dt = SAME ? kType : is_q ? a.q_out_dtype : a.k_out_dtype;
-            long long at = row0 * out_stride + (is_q ? h : kh) * D;
-            float next[8], w[8];
-            if (any) {
-                load4(x + d0, next);
-                load4(x + d1, next + 4);
+            long long at = row0 * out_stride + (is_q ? h : h - a.heads) * D;
+            uint64_t w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = weights ? weights[(i < 4 ? d0 : d1 - 4) + i] : 1.f;  // any alignment
+            for (int i = 0; i < 8; ++i) {  // any alignment
+                const float * at_w = weights + (i < 4 ? d0 : d1 - 8) + 2 * i;
+                w[i] = weights ? two(at_w[0], at_w[1]) : 0;
             }
-            if (!ready) __syncthreads();  // the angles; with two buffers the next chunk's are not those still in use
-            ready = true;
-            if (!any) break;
             const float * cos_at = sm_cos[buf] + f0, * sin_at = sm_sin[buf] + f0;
-            for (int r = 0; r < rows; ++r, at += out_stride, cos_at += D / 2, sin_at += D / 2) {
-                float v[8];
+            for (int r0 = 0; r0 < rows; r0 += kAhead)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = next[i];
-                if (r + 1 < rows) {
+            for (int u = 0; u < kAhead; ++u, at += out_stride, cos_at += D / 2, sin_at += D / 2) {
+                const int r = r0 + u;
+                if (r >= rows) break;
+                uint64_t v[8];
+                ahead[u][0].get(v);
+                ahead[u][1].get(v + 4);
+                if (r + kAhead < rows) {
+                    ahead[u][0].load(x + d0);
+                    ahead[u][1].load(x + d1);
                     x += stride;
-                    load4(x + d0, next);
-                    load4(x + d1, next + 4);
                 }
                 if (weights) {
-                    float ss = 0.f;
+                    uint64_t sq = mul2(v[0], v[0]);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
+                    for (int i = 1; i < 8; ++i) sq = fma2(v[i], v[i], sq);
+                    const float2 parts = of_two(sq);
+                    float ss = parts.x + parts.y;
 #pragma unroll
                     for (int s = L / 2; s; s >>= 1) ss += __shfl_xor_sync(mask, ss, s);
                     const float inv = rsqrtf(ss * (1.f / D) + a.eps);
+                    const uint64_t inv2 = two(inv, inv);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) v[i] = v[i] * inv * w[i];
+                    for (int i = 0; i < 8; ++i) v[i] = mul2(mul2(v[i], inv2), w[i]);
                 }
                 if (turns) {
-                    float cs[4], sn[4];
-                    load4(cos_at, cs);
-                    load4(sin_at, sn);
-                    if (a.interleaved) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x0 = v[2 * i], x1 = v[2 * i + 1];
-                            v[2 * i] = x0 * cs[i] - x1 * sn[i];
-                            v[2 * i + 1] = x1 * cs[i] + x0 * sn[i];
-                        }
-                    } else {
+                    for (int i = 0; i < 2; ++i) {  // four pairs at a time
+                        const float4 c4 = reinterpret_cast<const float4 *>(cos_at)[i], s4 = reinterpret_cast<const float4 *>(sin_at)[i];
+                        if (a.interleaved) {  // (x, y) (c, c) + (y, x) (-s, s)
+                            const float cs[4] = {c4.x, c4.y, c4.z, c4.w}, sn[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float x0 = v[i], x1 = v[i + 4];
-                            v[i] = x0 * cs[i] - x1 * sn[i];
-                            v[i + 4] = x1 * cs[i] + x0 * sn[i];
+                            for (int k = 0; k < 4; ++k) {
+                                uint64_t & y = v[4 * i + k];
+                                const float2 of = of_two(y);
+                                y = fma2(two(of.y, of.x), two(-sn[k], sn[k]), mul2(y, two(cs[k], cs[k])));
+                            }
+                        } else {
+                            const uint64_t cs[2] = {two(c4.x, c4.y), two(c4.z, c4.w)}, sn[2] = {two(s4.x, s4.y), two(s4.z, s4.w)};
+                            const uint64_t minus[2] = {two(-s4.x, -s4.y), two(-s4.z, -s4.w)};
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                uint64_t & y0 = v[2 * i + k], & y1 = v[4 + 2 * i + k];
+                                const uint64_t x0 = y0, x1 = y1;
+                                y0 = fma2(x1, minus[k], mul2(x0, cs[k]));
+                                y1 = fma2(x0, sn[k], mul2(x1, cs[k]));
+                            }
                         }
                     }
                 }
                 if (sm_pos[buf][r] < 0) continue;
-                store4(out, dt, at + d0, v);
-                store4(out, dt, at + d1, v + 4);
+                store8(out, dt, at + d0, v);
+                store8(out, dt, at + d1, v + 4);
             }
+            h += step;
+            if (h < per_row) start(h);
         }
     }
 }
@@ -1152,7 +1207,7 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
     const bool same = q_out_dtype == dtype && (!kv_heads || k_out_dtype == dtype);
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
-        const int lanes = head_dim / 8;
+        const int lanes = head_dim / 16;
         const int threads = (std::min((heads + kv_heads) * lanes, kRopeThreads) + 31) / 32 * 32;
         const dim3 grid(unsigned(std::min(rows, kRopePerSm / threads * kSms))), block{unsigned(threads)};
         if (head_dim == 128)

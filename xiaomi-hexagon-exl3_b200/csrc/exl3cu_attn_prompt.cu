@@ -178,28 +178,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return y;
 }
 
-// Two floats side by side, the operands of the two-wide instructions.
-__device__ __forceinline__ uint64_t two(float lo, float hi) {
-    uint64_t y;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(lo), "f"(hi));
-    return y;
-}
-__device__ __forceinline__ float2 of_two(uint64_t x) {
-    float2 y;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(x));
-    return y;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t y;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(y) : "l"(a), "l"(b), "l"(c));
-    return y;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t y;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(y) : "l"(a), "l"(b));
-    return y;
-}
-
 // 2^x of two x from -126 to 127 on the multiply-add pipe (the exponential unit does 16 a clock and SM, which is as
 // long as the products take): x = n + f, |f| <= 1/2, by a sum with 1.5 * 2^23; 2^f by a polynomial of degree 4 fitted
 // for the least relative error on [-1/2, 1/2], 2.6e-6 at most; n goes into the exponent.
