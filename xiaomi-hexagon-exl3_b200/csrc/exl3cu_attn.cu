@@ -25,13 +25,6 @@ namespace {
 
 constexpr int kSms = 148;  // a B200's
 
-// The largest of three, a NaN if one is.
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-
 // Constants of codes2 in registers: an instruction takes one immediate, and these need two.
 struct CodeConst {
     uint32_t magic, sixteenth, minus72;
@@ -298,114 +291,178 @@ __global__ void __launch_bounds__(kRopeThreads, 2) k_qk_norm_rope(const RopeArgs
 
 constexpr int kCacheThreads = 256;
 
-// Scaled codes of one thread's 8 dimensions (dimension i of group i mod G) as a word; inv = 1 / s within an ulp or two,
-// 0 where s is 0.  A sum with 1.5 * 2^23 + 8 rounds to the nearest integer, ties to even, and leaves the code in its low
-// bits; the constant high bits come off the assembled word at once.
+// Codes of 8 dimensions, the first of a group 0, as a word; x two side by side, s the scales, inv = 1 / s within an ulp or
+// two, 0 where s is 0.  A sum with 1.5 * 2^23 + 8 rounds to the nearest integer, ties to even, and leaves the code in its
+// low bits; the constant high bits come off the assembled word at once.
 //   x of 16 bits: x / s differs from a tie (n + 1/2) by at least 2^-16 unless it is one, since x has 11 bits and
 //   (n + 1/2) s at most 15; rounding the approximate quotient (off by 2^-20 at most) to multiples of 2^-18 first, by a
 //   sum with 48, makes ties exact and moves nothing else across one.
 //   f32: the remainder x - t s is exact; where it reaches half a step (a tie, or the quotient's error) the exact
 //   comparison of kv4_code decides.
 template <typename T, int G>
-__device__ __forceinline__ uint32_t kv4_word(const float (&x)[8], const float (&s)[G], const float (&inv)[G]) {
+__device__ __forceinline__ uint32_t kv4_word(const uint64_t (&x)[4], const float (&s)[G], const float (&inv)[G]) {
     constexpr float kMagic = 12582912.f + 8.f;
     constexpr uint32_t kHigh = 0x4b400000u;  // the bits of 1.5 * 2^23
+    const uint64_t magic = two(kMagic, kMagic);
     uint32_t word = 0, taken = 0;
     bool close = false;
 #pragma unroll
-    for (int i = 7; i >= 0; --i) {
-        float w;
+    for (int i = 3; i >= 0; --i) {
+        const uint64_t inv2 = two(inv[2 * i % G], inv[(2 * i + 1) % G]);
+        uint64_t w;
         if constexpr (sizeof(T) == 4) {
-            w = fmaf(x[i], inv[i % G], kMagic);
-            close = close || fabsf(fmaf(kMagic - w, s[i % G], x[i])) >= 0.5f * s[i % G];
+            w = fma2(x[i], inv2, magic);
+            const float2 d = of_two(fma2(add2(magic, mul2(w, two(-1.f, -1.f))), two(s[2 * i % G], s[(2 * i + 1) % G]), x[i]));
+            close = close || fabsf(d.x) >= 0.5f * s[2 * i % G] || fabsf(d.y) >= 0.5f * s[(2 * i + 1) % G];
         } else {
-            w = (fmaf(x[i], inv[i % G], 48.f) - 48.f) + kMagic;
+            w = add2(add2(fma2(x[i], inv2, two(48.f, 48.f)), two(-48.f, -48.f)), magic);
         }
-        word = word * 16u + __float_as_uint(w);
-        taken = taken * 16u + kHigh;
+        const float2 v = of_two(w);
+        word = (word * 16u + __float_as_uint(v.y)) * 16u + __float_as_uint(v.x);
+        taken = (taken * 16u + kHigh) * 16u + kHigh;
     }
     word -= taken;
     if (sizeof(T) == 4 && close) {
         word = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= kv4_code(x[i], s[i % G], inv[i % G]) << (4 * i);
+        for (int i = 0; i < 4; ++i) {
+            const float2 v = of_two(x[i]);
+            word |= kv4_code(v.x, s[2 * i % G], inv[2 * i % G]) << (8 * i);
+            word |= kv4_code(v.y, s[(2 * i + 1) % G], inv[(2 * i + 1) % G]) << (8 * i + 4);
+        }
     }
     return word;
 }
 
-// D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value: one word of codes each.
-// Dimension d is of group d mod G, so a thread holds 8 / G elements of every group, and the largest of a group is
-// taken over the threads by halving the groups that a thread carries.  Bound by the bytes of the rows.  blockIdx.y is
-// the head: the CTA's rows, consecutive positions of a prompt, are one piece of the cache.
+// The larger of the bits of |x|, of each half.
+__device__ __forceinline__ uint32_t most2(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
+
+// The scales of a head's groups (0, 1 in the first word, 2, 3 in the second) from its D/16 lanes' dimensions, 16 each, as
+// they lie; returns whether a group has a value beyond 7 times the largest scale (or one that is not finite).  |x| is
+// compared as an integer, so that a NaN is the largest; those of 16 bits two at a time, even and odd groups side by side.
+// Lanes halve the groups that they carry with each exchange, and come by the others' scales in the end.
+template <typename T, int D>
+__device__ __forceinline__ bool kv4_scales(const Eight<T> (&e)[2], unsigned mask, int j, uint32_t (&pair)[D / 64]) {
+    constexpr int G = D / 32;
+    constexpr uint32_t kMost = 0x48dfe400u;  // the bits of 7 * 65504
+    uint32_t own;
+    bool beyond;
+    if constexpr (sizeof(T) == 2) {
+        uint32_t m[G / 2];
+#pragma unroll
+        for (int g = 0; g < G / 2; ++g) {
+            const auto at = [&](int i) { return reinterpret_cast<const uint32_t *>(e[i / 4].raw)[i % 4]; };
+            m[g] = most2(at(g), at(g + G / 2));
+#pragma unroll
+            for (int i = g + G; i < 8; i += G / 2) m[g] = most2(m[g], at(i));
+        }
+        if constexpr (G == 4) {
+            const bool up = j & 4;
+            const uint32_t got = __shfl_xor_sync(mask, up ? m[0] : m[1], 4);
+            m[0] = __vmaxu2(up ? m[1] : m[0], got);
+        }
+        m[0] = __vmaxu2(m[0], __shfl_xor_sync(mask, m[0], 2));
+        m[0] = __vmaxu2(m[0], __shfl_xor_sync(mask, m[0], 1));
+        const auto bits = [](uint32_t h) {  // of the f32 that it stands for
+            return __float_as_uint(to_f32(*reinterpret_cast<const T *>(&h)));
+        };
+        const uint32_t lo = bits(m[0] & 0xffffu), hi = bits(m[0] >> 16);
+        own = uint32_t(__half_as_ushort(kv4_scale(lo))) | uint32_t(__half_as_ushort(kv4_scale(hi))) << 16;
+        beyond = max(lo, hi) > kMost;
+    } else {
+        uint32_t m[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            const auto at = [&](int i) { return reinterpret_cast<const uint32_t *>(e[i / 8].raw)[i % 8] & 0x7fffffffu; };
+            m[g] = at(g);
+#pragma unroll
+            for (int i = g + G; i < 16; i += G) m[g] = max(m[g], at(i));
+        }
+        if constexpr (G == 4) {
+            const bool up = j & 4;
+            const uint32_t a = __shfl_xor_sync(mask, up ? m[0] : m[2], 4), b = __shfl_xor_sync(mask, up ? m[1] : m[3], 4);
+            m[0] = max(up ? m[2] : m[0], a);
+            m[1] = max(up ? m[3] : m[1], b);
+        }
+        const bool up = j & 2;
+        const uint32_t got = __shfl_xor_sync(mask, up ? m[0] : m[1], 2);
+        m[0] = max(up ? m[1] : m[0], got);
+        m[0] = max(m[0], __shfl_xor_sync(mask, m[0], 1));
+        const uint32_t mine = __half_as_ushort(kv4_scale(m[0])), other = __shfl_xor_sync(mask, mine, 2);
+        own = up ? other | mine << 16 : mine | other << 16;
+        beyond = m[0] > kMost;
+    }
+    if constexpr (G == 4) {
+        const uint32_t other = __shfl_xor_sync(mask, own, 4);
+        pair[0] = j & 4 ? other : own;
+        pair[1] = j & 4 ? own : other;
+    } else {
+        pair[0] = own;
+    }
+    return beyond;
+}
+
+// D/16 threads a (row, head), each with 16 consecutive dimensions of the key and of the value: two words of codes each,
+// and 16 / G elements of every group (dimension d is of group d mod G).  24256 rows of 8 heads of 64 dimensions, 64 MB in
+// and out: 17.0 us, 3.7 TB/s, at 63 % of the issue slots (8 dimensions a thread: 18.8, 79 %).  blockIdx.y is the head: the
+// CTA's rows, consecutive positions of a prompt, are one piece of the cache (heads of a row side by side: 18.8).
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads)
 k_kv4_append(const Kv4 c, const T * k, long long k_stride, const T * v, long long v_stride, int rows,
              const int32_t * row_seq, const int32_t * row_pos, const int32_t * seq_slot, int n_seq) {
-    constexpr int G = D / 32, L = D / 8;
+    constexpr int G = D / 32, L = D / 16;
     pdl_trigger();
     const int r = blockIdx.x * (kCacheThreads / L) + threadIdx.x / L, h = blockIdx.y, j = threadIdx.x % L;
     const unsigned mask = ((1u << L) - 1u) << (threadIdx.x & 31 & ~(L - 1));
     pdl_wait_primary();
     if (r >= rows) return;
     const int seq = row_seq[r], pos = row_pos[r];
-    float x[2][8];
-    const T * src[2] = {k + r * k_stride + h * D + 8 * j, v + r * v_stride + h * D + 8 * j};
+    Eight<T> e[2][2];
 #pragma unroll
-    for (int w = 0; w < 2; ++w) load_row<8>(src[w], x[w]);
+    for (int w = 0; w < 2; ++w) {
+        const T * src = (w ? v + r * v_stride : k + r * k_stride) + h * D + 16 * j;
+        e[w][0].load(src);
+        e[w][1].load(src + 8);
+    }
     if (seq < 0 || seq >= n_seq) return;
     const int slot = seq_slot[seq];
     if (slot < 0 || slot >= c.n_slots || pos < 0 || pos >= c.max_len) return;
     const size_t at = (size_t(slot) * c.kv_heads + h) * c.max_len + pos;
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-        uint32_t most[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            float m = 0.f;
-#pragma unroll
-            for (int i = g; i < 8; i += 2 * G) m = max3_nan(m, fabsf(x[w][i]), fabsf(x[w][i + G]));
-            most[g] = __float_as_uint(m);  // a NaN is the largest as an integer
-        }
-        // exchange: after it this thread carries group `mine` over all threads
-        int mine = 0;
-        if constexpr (G == 4) {
-            const bool up = j & (L / 2);
-            const uint32_t a0 = up ? most[0] : most[2], a1 = up ? most[1] : most[3];
-            most[0] = max(up ? most[2] : most[0], __shfl_xor_sync(mask, a0, L / 2));
-            most[1] = max(up ? most[3] : most[1], __shfl_xor_sync(mask, a1, L / 2));
-            mine = up ? 2 : 0;
-        }
-        constexpr int S = G == 4 ? L / 4 : L / 2;
-        const bool up = j & S;
-        uint32_t m = max(up ? most[1] : most[0], __shfl_xor_sync(mask, up ? most[0] : most[1], S));
-        mine += up ? 1 : 0;
-#pragma unroll
-        for (int s = S / 2; s; s >>= 1) m = max(m, __shfl_xor_sync(mask, m, s));
-        const __half scale = kv4_scale(m);
-        const float own = __half2float(scale), own_inv = own > 0.f ? __fdividef(1.f, own) : 0.f;
-        if (!(j & (S - 1))) (w ? c.v_scales : c.k_scales)[at * G + mine] = __half_as_ushort(scale);
+        uint32_t pair[G / 2];
+        const bool beyond = kv4_scales<T, D>(e[w], mask, j, pair);
+        if (!(j & 3)) reinterpret_cast<uint32_t *>((w ? c.v_scales : c.k_scales) + at * G)[j / 4] = pair[j / 4 % (G / 2)];
         float s[G], inv[G];
-        // thread g * S of the head carries group g in the order of the halvings
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-            s[g] = __shfl_sync(mask, own, g * S, L);
-            inv[g] = __shfl_sync(mask, own_inv, g * S, L);
+            const float2 f = h2f2(pair[g / 2]);
+            s[g] = g & 1 ? f.y : f.x;
+            inv[g] = s[g] > 0.f ? __fdividef(1.f, s[g]) : 0.f;
         }
+        uint64_t x[2][4];
+        e[w][0].get(x[0]);
+        e[w][1].get(x[1]);
         // a group beyond the largest scale saturates; one that is not finite has codes of zero
-        if (__any_sync(mask, m > __float_as_uint(7.f * 65504.f))) {
+        if (__any_sync(mask, beyond)) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float most_x = 7.f * s[i % G];
-                x[w][i] = inv[i % G] > 0.f ? fminf(fmaxf(x[w][i], -most_x), most_x) : 0.f;
+                float2 y = of_two(x[i / 4][i % 4]);
+                const float a = 7.f * s[2 * i % G], b = 7.f * s[(2 * i + 1) % G];
+                y.x = inv[2 * i % G] > 0.f ? fminf(fmaxf(y.x, -a), a) : 0.f;
+                y.y = inv[(2 * i + 1) % G] > 0.f ? fminf(fmaxf(y.y, -b), b) : 0.f;
+                x[i / 4][i % 4] = two(y.x, y.y);
             }
         }
-        reinterpret_cast<uint32_t *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j] = kv4_word<T, G>(x[w], s, inv);
+        reinterpret_cast<uint2 *>((w ? c.v_codes : c.k_codes) + at * (D / 2))[j] =
+            make_uint2(kv4_word<T, G>(x[0], s, inv), kv4_word<T, G>(x[1], s, inv));
     }
 }
 
 // D/8 threads a (row, head), each with 8 consecutive dimensions of the key and of the value; kReadRows rows a thread,
-// whose loads are under way together.  Bound by the bytes written.  blockIdx.y is the head.
-constexpr int kReadRows = 4;
+// whose loads are under way together; the heads of a row side by side, as they lie in the output.  Bound by the bytes
+// written: 50 MB 14.4 us, 3.4 TB/s, as fast as so many are filled with zeros (4 rows a thread 14.9, 1 16.7).
+constexpr int kReadRows = 2;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads)
@@ -413,8 +470,8 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
            long long k_stride, T * v, long long v_stride) {
     constexpr int G = D / 32, L = D / 8, kStep = kCacheThreads / L;
     pdl_trigger();
-    const int j = threadIdx.x % L, h = blockIdx.y;
-    const int first = blockIdx.x * (kReadRows * kStep) + threadIdx.x / L;  // rows first, first + kStep, ...
+    const int blk = blockIdx.x / c.kv_heads, h = blockIdx.x - blk * c.kv_heads, j = threadIdx.x % L;
+    const int first = blk * (kReadRows * kStep) + threadIdx.x / L;  // rows first, first + kStep, ...
     const CodeConst kc2;
     pdl_wait_primary();
     if (first >= total) return;
@@ -1228,7 +1285,7 @@ int exl3cu_kv4_append(const exl3cu_kv4_cache * cache, const void * d_k, size_t k
         !rows_ok(d_v, v_stride, width, dtype))
         return bad("kv4_append: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
-    const int per_cta = kCacheThreads / (cache->head_dim / 8);
+    const int per_cta = kCacheThreads / (cache->head_dim / 16);
     const dim3 grid(unsigned((rows - 1) / per_cta + 1), unsigned(cache->kv_heads));
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -1251,7 +1308,7 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
         return bad("kv4_read: null or misaligned operand, or rows closer than their width");
     const Kv4 c = device_cache(cache);
     const int per_cta = kReadRows * (kCacheThreads / (cache->head_dim / 8));
-    const dim3 grid(unsigned((total_rows - 1) / per_cta + 1), unsigned(cache->kv_heads));
+    const dim3 grid(unsigned((total_rows - 1) / per_cta + 1) * unsigned(cache->kv_heads));
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_read<T, 128> : k_kv4_read<T, 64>,
