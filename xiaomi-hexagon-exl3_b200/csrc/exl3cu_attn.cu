@@ -403,7 +403,7 @@ __device__ __forceinline__ bool kv4_scales(const Eight<T> (&e)[2], unsigned mask
 }
 
 // D/16 threads a (row, head), each with 16 consecutive dimensions of the key and of the value: two words of codes each,
-// and 16 / G elements of every group (dimension d is of group d mod G).  24256 rows of 8 heads of 64 dimensions, 64 MB in
+// and 16 / G elements of every group (dimension d is of group d mod G).  24234 rows of 8 heads of 64 dimensions, 64 MB in
 // and out: 17.0 us, 3.7 TB/s, at 63 % of the issue slots (8 dimensions a thread: 18.8, 79 %).  blockIdx.y is the head: the
 // CTA's rows, consecutive positions of a prompt, are one piece of the cache (heads of a row side by side: 18.8).
 template <typename T, int D>
