@@ -542,8 +542,11 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 // ---- attention of single rows over the cache ------------------------------------------------------
 //
 // One pass over the keys of a row in tiles of 64, on the matrix instructions, with the running maximum and sum
-// of a softmax.  Bound by the bytes of the cache (2 (D/2 + D/16) a key and K/V head) as long as a code costs about
-// one instruction; so codes are never multiplied by their scales:
+// of a softmax.  The bytes of the cache (2 (D/2 + D/16) a key and K/V head) are its floor, if a code costs few
+// instructions; so codes are never multiplied by their scales.  8 rows of 131072 positions (604 MB): 117 us, 5.2 TB/s;
+// the loads alone 94.  The difference is a tile's chain of products, softmax and products with the three warps that a
+// scheduler has: a tenth fewer instructions (uncentred codes on the key side) gave 118 for 119, copies of keys and values
+// that start separately 124.
 //
 //   Codes become halves by one logic operation on two at a time (into the mantissa of 1024) and one multiply-add
 //   (to c - 8, exact), after a shift for every other four.
@@ -902,42 +905,44 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 #pragma unroll
                             for (int j = 0; j < H; ++j) sc[x][y][j] = -INFINITY;
             }
-            // exponent of the largest value scale: two keys a lane
-            uint32_t top;
+            // exponent of the largest value scale of the lane's two keys; the lane's largest scores.  The others' are
+            // asked for only where something has moved: exchanges would stand in every tile's way.
+            int top;
             {
-                uint32_t w[G];
+                uint32_t w[G], most;
                 lds(vs + lane * (4 * G), w);
-                top = w[0] & 0x7fff7fffu;
+                most = w[0] & 0x7fff7fffu;
 #pragma unroll
-                for (int i = 1; i < G; ++i) top = __vmaxu2(top, w[i] & 0x7fff7fffu);
-                top = __reduce_max_sync(0xffffffffu, max(top & 0xffffu, top >> 16)) >> 10;
-                if (top == 31u) {  // not finite: its group of dimensions is, and the others' weights keep their range
-                    top = 0;
-#pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
-                        top = max(top, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top) >> 10;
-                }
+                for (int i = 1; i < G; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+                top = int(max(most & 0xffffu, most >> 16) >> 10);
             }
-            const int grown = max(int(top) - ev, 0);
-            bool moved = grown > 0;
+            bool moved = top > ev;
             float mx[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) {
                 mx[j] = max3(m[j], sc[0][0][j], sc[0][1][j]);
 #pragma unroll
                 for (int x = 1; x < 4; ++x) mx[j] = max3(mx[j], sc[x][0][j], sc[x][1][j]);
-#pragma unroll
-                for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
                 moved = moved || (mx[j] - m[j]) * cs[j] > float(kLazy);  // no: both -inf
             }
             if (__any_sync(0xffffffffu, moved)) {
+                if (top == 31) {  // not finite: its group of dimensions is, and the others' weights keep their range
+                    uint32_t w[G], most = 0;
+                    lds(vs + lane * (4 * G), w);
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
+                        most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                    }
+                    top = int(most >> 10);
+                }
+                const int grown = max(__reduce_max_sync(0xffffffffu, top) - ev, 0);
                 ev += grown;
                 const float down = pow2(-grown);
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
                     const float f = (mx[j] == m[j] ? 1.f : exp2_approx((m[j] - mx[j]) * cs[j])) * down;
                     m[j] = mx[j];
                     l[j] *= f;
