@@ -297,6 +297,33 @@ def test_attend(A, dtype, heads, kv, dim, lens):
     check_attend(got, q, clean, slots, lens)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim,lens", [
+    (16, 4, 128, [767]), (16, 4, 128, [1, 2, 63, 64, 65, 1000, 2049, 31]), (32, 4, 64, [5, 300, 128]), (8, 8, 128, [129, 15]),
+    (10, 2, 64, [257, 4097]), (64, 2, 128, [100, 5000])])
+def test_attend_in_a_long_cache(A, dtype, heads, kv, dim, lens):
+    """Short contexts in a cache for long ones: the rows' tiles are cut into shares, not dealt to clusters."""
+    g = gen(heads + len(lens) + 1)
+    n = len(lens)
+    cache = A.Kv4Cache(n, kv, 5120, dim)
+    fill(cache, g)
+    q = randn(g, n, heads, dim).to(dtype)
+    got = cache.attend(q, ints(list(range(n))), ints([m - 1 for m in lens]), ints(list(range(n))[::-1]))
+    check_attend(got, q, cache, list(range(n))[::-1], lens)
+
+
+@pytest.mark.parametrize("n", [1, 64, 65, 449, 512, 513, 577, 4033, 4096])
+def test_attend_at_the_edges_of_a_clusters_shares(A, n):
+    g = gen(n)
+    cache = A.Kv4Cache(2, 2, 4096, 64)
+    fill(cache, g)
+    q = randn(g, 3, 8, 64)
+    # the last row sees nothing: its cluster has nothing to join
+    got = cache.attend(q, ints([0, 1, 0]), ints([n - 1, 4095, -1]), ints([1, 0]))
+    check_attend(got[:2], q[:2], cache, [1, 0], [n, 4096])
+    assert bool((got[2] == 0).all())
+
+
 def test_attend_long_and_many_rows(A):
     """A context long enough to be split many ways, and more rows than the GPU has places."""
     g = gen(11)

@@ -11,6 +11,8 @@
 #include "exl3cu_attn.h"
 #include "exl3cu_internal.h"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <cstring>
@@ -569,7 +571,7 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 // The tiles of all rows form one list that is cut into equal shares, one per CTA, so that a batch of a long and
 // many short contexts fills the GPU evenly (a row counts kRowCost tiles more than it has: what taking up a row costs
 // a CTA).  A CTA's part of a row that it does not hold whole goes to scratch as (maximum, sum, accumulator), and
-// k_kv4_merge joins the parts in order.
+// k_kv4_merge joins the parts in order.  (Few rows of few positions: a cluster of CTAs to a row instead.)
 
 constexpr int kKeys = 64;        // keys per tile
 constexpr int kAttnWarps = 4;    // warps of a CTA, each with tiles of its own
@@ -582,12 +584,21 @@ constexpr int kSplitRows = 256;  // rows up to which the tiles of all rows are c
 constexpr int kRowCost = 8;      // 8 rows between 1 and 32768 positions: 19.0 us with 2, 15.0 with 8, 15.1 with 12
 constexpr int kPlanFloats = 2 * kSplitRows;  // scratch begins with (first share, shares) of every row
 constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
+// Few rows in a cache of few positions: a cluster of CTAs takes a row and joins its parts from their shared memory, which
+// spares the second kernel: 1 row behind 767 positions 6.5 us (f32; with shares 7.9), behind 2047 6.5 (bf16; 9.3), 8 rows
+// behind 4095 11.9 (14.6).  Above 4096 positions, or with more clusters than are resident together, shares are faster:
+// 8191 positions 10.6 against 9.7, 32 rows of 767 21.2 against 13.9.
+constexpr int kCluster = 8;
+constexpr int kClusterTiles = 64;
 constexpr int kLazy = 6, kTop = 14 - kLazy;  // weights times value scales are up to 2^kTop, 2^14 before m moves
 
 template <int D> struct Kv4Tile {
     static constexpr int kCodes = kKeys * D / 2, kScales = kKeys * D / 16;  // bytes of one of K and V
     static constexpr int kBytes = 2 * (kCodes + kScales);
 };
+
+// How the tiles are divided: a CTA a row; equal shares of all rows' tiles; a cluster of CTAs a row.
+enum Split { kWhole, kShares, kClusters };
 
 struct Kv4Attn {
     Kv4 c;
@@ -600,7 +611,7 @@ struct Kv4Attn {
     float * part;  // kPlanFloats; [y][x][2][HC][D + 4]: a CTA's row that it begins and does not end, and the one
                    // that it goes on with
     int rows, n_seq, heads, chunks;
-    int split;          // 0: one CTA per row
+    int split;          // see Split
     float scale_log2;   // scale * log2(e)
 };
 
@@ -721,8 +732,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
     };
     // the next row (of the list; row0 + row of the call), where in it to begin, what is left of the share
     int row = 0, off = 0, left;
-    const int row0 = a.split ? 0 : blockIdx.x;
-    if (a.split) {
+    const int row0 = a.split == kShares ? 0 : a.split == kClusters ? blockIdx.x / kCluster : blockIdx.x;
+    if (a.split == kShares) {
         int n[2], slot[2], before, total;
         scan_rows(a, n, slot, before, total, sm_scan);
         const int share = share_of(total, gridDim.x), begin = blockIdx.x * share;
@@ -755,11 +766,16 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         if (threadIdx.x == 0) {
             sm_n[0] = n;
             sm_slot[0] = slot;
-            if (n == 0) zero_row(row0);
+            if (n == 0 && (a.split == kWhole || blockIdx.x % kCluster == 0)) zero_row(row0);
         }
         __syncthreads();
-        if (n <= 0) return;
+        if (n <= 0) return;  // the whole cluster
         left = list_of(n);
+        if (a.split == kClusters) {
+            const int share = (tiles_of(n) + kCluster - 1) / kCluster;
+            off = blockIdx.x % kCluster * share;
+            left = share;
+        }
     }
 
     const CodeConst kc2;
@@ -767,7 +783,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
     bool ok = true;
     while (left > 0) {
         const int n = sm_n[row], tiles = tiles_of(n), t0 = min(off, tiles), t1 = min(tiles, off + left);
-        left -= min(left, list_of(n) - off);
+        left = a.split == kClusters ? 0 : left - min(left, list_of(n) - off);
         off = 0;
         const int call_row = row0 + row, slot = sm_slot[row];
         ++row;
@@ -1055,7 +1071,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         __syncthreads();
         const bool whole = t0 == 0 && t1 == tiles;
         float * part = whole ? nullptr
-                             : a.part + kPlanFloats + ((size_t(blockIdx.y) * gridDim.x + blockIdx.x) * 2 + (t0 ? 1 : 0)) * (HC * kRec);
+                       : a.split == kClusters
+                           ? reinterpret_cast<float *>(ring_all) + HC * kRec  // behind the first warp's record
+                           : a.part + kPlanFloats + ((size_t(blockIdx.y) * gridDim.x + blockIdx.x) * 2 + (t0 ? 1 : 0)) * (HC * kRec);
         for (int i = threadIdx.x; i < nh * D; i += kAttnThreads) {
             const int h = i / D, d = i % D;
             const float * rec = reinterpret_cast<const float *>(ring_all) + h * kRec;
@@ -1086,6 +1104,34 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
             if (threadIdx.x == 0) atomicOr(&g_attn_status, kStatusWaitTimeout);
             break;
         }
+    }
+    if (a.split == kClusters) {  // join the parts, in order; the outputs are dealt out among the cluster's threads
+        namespace cg = cooperative_groups;
+        constexpr int kRec = D + 4;
+        const int tiles = tiles_of(sm_n[0]), share = (tiles + kCluster - 1) / kCluster, used = (tiles + share - 1) / share;
+        if (used == 1) return;  // the whole cluster
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        for (int i = blockIdx.x % kCluster * kAttnThreads + threadIdx.x; i < nh * D; i += kCluster * kAttnThreads) {
+            float M[kCluster], L = 0.f, A = 0.f, top = -INFINITY;
+            const float * rec = reinterpret_cast<const float *>(ring_all) + HC * kRec + i / D * kRec;
+#pragma unroll
+            for (int u = 0; u < kCluster; ++u) {
+                M[u] = u < used ? cluster.map_shared_rank(rec, u)[D] : -INFINITY;
+                top = fmaxf(top, M[u]);
+            }
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int u = 0; u < kCluster; ++u)
+                if (u < used) {
+                    const float * r = cluster.map_shared_rank(rec, u);
+                    const float f = exp2_approx(M[u] - ref);
+                    L = fmaf(r[D + 1], f, L);
+                    A = fmaf(r[i % D], f, A);
+                }
+            out[row0 * a.out_stride + i] = from_f32<T>(A / L);
+        }
+        cluster.sync();  // the others' reads
     }
 }
 
@@ -1159,6 +1205,7 @@ __global__ void __launch_bounds__(WIDE ? kMergeThreads : HC * D) k_kv4_merge(con
 // How a call is cut up: shares (CTAs) per K/V head chunk, 0 for one CTA per row.
 struct AttnPlan {
     int heads_per_cta, chunks, ys, shares;
+    Split split;
     size_t scratch;
 };
 
@@ -1170,7 +1217,9 @@ AttnPlan plan_attn(const exl3cu_kv4_cache * c, int rows, int heads, int dtype) {
     p.ys = c->kv_heads * p.chunks;
     p.shares = 0;
     p.scratch = 0;
+    p.split = kWhole;
     if (rows > kSplitRows) return p;
+    p.split = c->max_len / kKeys <= kClusterTiles && (long long)rows * p.ys * kCluster <= kAttnCtas * kSms ? kClusters : kShares;
     // as many CTAs as are resident together (three per SM), no more than there can be shares
     const long long most = ((long long)rows * (c->max_len / kKeys + kRowCost) + kMinShare - 1) / kMinShare;
     p.shares = int(std::max(1ll, std::min((long long)(kAttnCtas * kSms / p.ys), most)));
@@ -1273,8 +1322,8 @@ int exl3cu_qk_norm_rope(const void * d_q, size_t q_stride, const void * d_k, siz
         const int threads = (std::min((heads + kv_heads) * lanes, kRopeThreads) + 31) / 32 * 32;
         const dim3 grid(unsigned(std::min(rows, kRopePerSm / threads * kSms))), block{unsigned(threads)};
         if (head_dim == 128)
-            return attn_launch(same ? k_qk_norm_rope<T, 128, true> : k_qk_norm_rope<T, 128, false>, grid, block, 0, stream, a);
-        return attn_launch(same ? k_qk_norm_rope<T, 64, true> : k_qk_norm_rope<T, 64, false>, grid, block, 0, stream, a);
+            return attn_launch(same ? k_qk_norm_rope<T, 128, true> : k_qk_norm_rope<T, 128, false>, grid, block, 0, stream, 1, a);
+        return attn_launch(same ? k_qk_norm_rope<T, 64, true> : k_qk_norm_rope<T, 64, false>, grid, block, 0, stream, 1, a);
     });
 }
 
@@ -1295,7 +1344,7 @@ int exl3cu_kv4_append(const exl3cu_kv4_cache * cache, const void * d_k, size_t k
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_append<T, 128> : k_kv4_append<T, 64>,
-                           grid, dim3(kCacheThreads), 0, stream, c, static_cast<const T *>(d_k),
+                           grid, dim3(kCacheThreads), 0, stream, 1, c, static_cast<const T *>(d_k),
                            (long long)k_stride, static_cast<const T *>(d_v), (long long)v_stride, rows, d_row_seq,
                            d_row_pos, d_seq_slot, n_seq);
     });
@@ -1317,7 +1366,7 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
         return attn_launch(cache->head_dim == 128 ? k_kv4_read<T, 128> : k_kv4_read<T, 64>,
-                           grid, dim3(kCacheThreads), 0, stream, c, d_seq_slot, d_kv_offsets, n_seq,
+                           grid, dim3(kCacheThreads), 0, stream, 1, c, d_seq_slot, d_kv_offsets, n_seq,
                            total_rows, static_cast<T *>(d_k), (long long)k_stride, static_cast<T *>(d_v),
                            (long long)v_stride);
     });
@@ -1348,7 +1397,7 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
     if (p.scratch && (!d_scratch || scratch_bytes < p.scratch || reinterpret_cast<uintptr_t>(d_scratch) % 16))
         return bad("kv4_attn: scratch missing, misaligned or too small (exl3cu_kv4_attn_scratch_bytes)");
     const Kv4Attn a{device_cache(cache), d_q, d_out, (long long)q_stride, (long long)out_stride, d_row_seq, d_row_pos,
-                    d_seq_slot, static_cast<float *>(d_scratch), rows, n_seq, heads, p.chunks, p.shares > 0,
+                    d_seq_slot, static_cast<float *>(d_scratch), rows, n_seq, heads, p.chunks, p.split,
                     scale * 1.4426950408889634f};
     return with_type(dtype, [&](auto t) {
         using T = decltype(t);
@@ -1366,15 +1415,16 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
                 if (e != cudaSuccess) return api_cuda_fail(e, "kv4_attn: shared memory");
                 done.fetch_or(bit);
             }
-            const int rc = attn_launch(k_kv4_attn<T, D, HC>, dim3(unsigned(p.shares ? p.shares : rows), unsigned(p.ys)),
-                                       dim3(kAttnThreads), size_t(smem), stream, a);
-            if (rc || !p.shares) return rc;
+            const int ctas = p.split == kShares ? p.shares : p.split == kClusters ? rows * kCluster : rows;
+            const int rc = attn_launch(k_kv4_attn<T, D, HC>, dim3(unsigned(ctas), unsigned(p.ys)), dim3(kAttnThreads), size_t(smem),
+                                       stream, p.split == kClusters ? kCluster : 1, a);
+            if (rc || p.split != kShares) return rc;
             // a row has about shares / rows parts: above 8, a CTA per head, below, one for all heads of a K/V head
             if (p.shares > 8 * rows)
                 return attn_launch(k_kv4_merge<T, D, HC, true>, dim3(unsigned(rows), unsigned(p.ys), HC),
-                                   dim3(kMergeThreads), 0, stream, a, p.shares);
+                                   dim3(kMergeThreads), 0, stream, 1, a, p.shares);
             return attn_launch(k_kv4_merge<T, D, HC, false>, dim3(unsigned(rows), unsigned(p.ys)), dim3(HC * D), 0,
-                               stream, a, p.shares);
+                               stream, 1, a, p.shares);
         };
         constexpr std::integral_constant<int, 64> d64;
         constexpr std::integral_constant<int, 128> d128;

@@ -102,19 +102,23 @@ int with_type(int dtype, F && f) {
 }
 
 // Launch with programmatic stream serialization (the kernels wait for their predecessor with
-// griddepcontrol.wait before touching memory).
+// griddepcontrol.wait before touching memory); clusters of
+// `cluster` CTAs along x.
 template <typename... KArgs, typename... Args>
-int attn_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void * stream, Args... args) {
+int attn_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, void * stream, int cluster, Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(cluster);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
     if (e == cudaSuccess) return EXL3CU_OK;
     (void)cudaGetLastError();

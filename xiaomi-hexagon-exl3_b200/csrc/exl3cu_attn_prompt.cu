@@ -806,9 +806,9 @@ int launch(const PromptArgs & a, const CUtensorMap (&maps)[3], unsigned blocks, 
         done.fetch_or(bit);
     }
     const int rc = attn_launch(k_prompt_attn<T, D>, dim3(blocks, unsigned(a.splits)), dim3(kThreads), size_t(Shape<D>::kSmem),
-                               stream, a, maps[0], maps[1], maps[2]);
+                               stream, 1, a, maps[0], maps[1], maps[2]);
     if (rc || a.splits == 1) return rc;
-    return attn_launch(k_prompt_merge<T, D>, dim3(blocks, 2 * kTile / 32), dim3(256), 0, stream, a);
+    return attn_launch(k_prompt_merge<T, D>, dim3(blocks, 2 * kTile / 32), dim3(256), 0, stream, 1, a);
 }
 
 constexpr int kSms = 148;  // a B200's
