@@ -58,7 +58,6 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 // Weights are scaled by 2^kShift, up to 2^14 when the maximum lags by its 2^8: so that a half holds those of a
 // long, flat tail too (2^-30 of the largest), and none overflows.
 constexpr int kShift = 6;
-constexpr int kOutBytes = 128;  // of a row that the epilogue writes at a time: what the smaller head has of 16-bit values
 // Tiles of keys of a share at least, where a block's keys are shared among CTAs: 512 rows behind 1000 keys 21.9 us
 // with 4, 24.6 with 6, 30.1 with 10, 26.9 without sharing; behind 4000 keys 30.9, 30.8, 32.2 and 65.6.
 constexpr int kMinSplit = 4;
@@ -211,7 +210,9 @@ struct Work {
 // Block `blk` of the call, by one warp: blocks of all sequences in order, counted from the end so that a
 // sequence's longest block starts first.  A lane holds a sequence; up to 32 are read once.
 __device__ __forceinline__ void find_block(const PromptArgs & a, int blk, Work & out) {
-    const int lane = threadIdx.x & 31, positions = 2 * kTile >> a.log_p;
+    constexpr int kLogRows = 8;
+    static_assert(1 << kLogRows == 2 * kTile, "rows of a block");
+    const int lane = threadIdx.x & 31, log_positions = kLogRows - a.log_p, positions = 1 << log_positions;
     int q0 = 0, q1 = 0, k0 = 0, k1 = 0;
     const auto read = [&](int s) {
         q0 = q1 = k0 = k1 = 0;
@@ -221,7 +222,7 @@ __device__ __forceinline__ void find_block(const PromptArgs & a, int blk, Work &
             k0 = min(max(a.kv_begin[s], 0), a.kv_rows);
             k1 = max(min(a.kv_end[s], a.kv_rows), k0);
         }
-        return q1 > q0 ? (q1 - q0 + positions - 1) / positions : 0;
+        return q1 > q0 ? (q1 - q0 + positions - 1) >> log_positions : 0;
     };
     int total = 0, mine = 0;
     for (int s0 = 0; s0 < a.n_seq; s0 += 32) {
@@ -256,7 +257,8 @@ struct Split {
 __device__ __forceinline__ Split split_of(const PromptArgs & a, const Work & w) {
     const int nq = w.q1 - w.q0, last = min(w.p0 + (2 * kTile >> a.log_p), nq) - 1;  // the block's last position sees most
     const int all = (max(0, last + 1 + (w.k1 - w.k0) - nq) + kTile - 1) / kTile;
-    const int tiles = a.splits > 1 ? max(kMinSplit, (all + a.splits - 1) / a.splits) : max(all, 1);
+    if (a.splits == 1) return Split{max(all, 1), 1};  // no divisions: a short prompt waits for them
+    const int tiles = max(kMinSplit, (all + a.splits - 1) / a.splits);
     return Split{tiles, max(1, (all + tiles - 1) / tiles)};
 }
 
@@ -588,7 +590,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             const uint64_t c2 = two(c, c), mc2 = two(-mc, -mc);
             uint64_t add[2] = {0, 0};
             // masked scores have to become 0: at a view's end the polynomial is not used
-            const auto weights = [&](auto polynomial) {
+            const auto weights = [&](auto polynomial, int need) {
                 const auto some = [&](auto from, auto to_key) {
 #pragma unroll
                     for (int i = decltype(from)::value; i < decltype(to_key)::value; i += 2) {
@@ -611,16 +613,34 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars.p_full[t][part]);
                 };
-                some(std::integral_constant<int, 0>{}, std::integral_constant<int, kEarly>{});
+                if constexpr (decltype(polynomial)::value) {
+                    some(std::integral_constant<int, 0>{}, std::integral_constant<int, kEarly>{});
+                } else {  // no row of the warp sees keys from `need` on
+                    const auto third = [&](auto from) {
+                        constexpr int at = decltype(from)::value;
+                        if (at < need) some(from, std::integral_constant<int, at + 32>{});
+                        else
+#pragma unroll
+                            for (int i = at / 2; i < at / 2 + 16; ++i) s[i] = 0;
+                    };
+                    third(std::integral_constant<int, 0>{});
+                    third(std::integral_constant<int, 32>{});
+                    third(std::integral_constant<int, 64>{});
+                }
                 tmem_st(ts, s);
                 tmem_st16(ts + 32, s + 32);
                 hand_over(0);
-                some(std::integral_constant<int, kEarly>{}, std::integral_constant<int, kTile>{});
+                if (decltype(polynomial)::value || kEarly < need) {
+                    some(std::integral_constant<int, kEarly>{}, std::integral_constant<int, kTile>{});
+                } else {
+#pragma unroll
+                    for (int i = kEarly / 2; i < kTile / 2; ++i) s[i] = 0;
+                }
                 tmem_st16(ts + 48, s + 48);
                 hand_over(1);
             };
-            if (edge) weights(std::false_type{});
-            else weights(std::true_type{});
+            if (edge) weights(std::false_type{}, __reduce_max_sync(0xffffffffu, left));
+            else weights(std::true_type{}, kTile);
             const float2 added = of_two(add2(add[0], add[1]));
             sum += added.x + added.y;
         }
@@ -630,71 +650,80 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         fence_after();
         // read again: the loop needs the registers
         const View end(a, bars.work);
-        const int p = end.p0 + t * ppt + (row >> a.log_p), head = head0 + (row & ((1 << a.log_p) - 1));
+        const int p = end.p0 + t * ppt + (row >> a.log_p);
         const bool live = end.work && ok && p < end.nq, part = end.part;
         const float inv = part ? 1.f : lim > 0 ? 1.f / sum : 0.f;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         // a share's part goes to scratch as it is, in f32, with what its weights refer to
         const bool f32 = part || a.out_f32;
-        const size_t rec = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile + row;
+        const size_t rec0 = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile, rec = rec0 + row;
         char * const out = static_cast<char *>(part ? a.part : a.out);
-        const long long at = part ? (long long)rec * D : live ? (long long)(end.q0 + p) * a.out_stride + head * D : 0;
         if (part && live) {
             const float mr = m == -INFINITY ? m : m == INFINITY ? NAN : m * c - float(kShift);
             reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
         }
-        // Rows go out by way of the query tile's memory (its products are complete), kOutBytes of a row at a time, so
-        // that its lanes write them together: a row to a lane and 16 bytes at a time take a wavefront per row.
-        unsigned char * const stage = sq + t * Sh::kTileBytes + (warp & 3) * 32 * kOutBytes;
-        const int passes = f32 ? D * 4 / kOutBytes : D * 2 / kOutBytes;
-        const int elems = f32 ? kOutBytes / 4 : kOutBytes / 2;  // of a row in a pass
-        for (int pass = 0; pass < passes; ++pass) {
-#pragma unroll 1
-            for (int i = pass * elems; i < (pass + 1) * elems; i += 32) {
-                uint32_t o[32];
-                if (tiles > 0 && ok) {
-                    tmem_ld(to + i, o);
-                    wait_ld();
-                }
-                float v[32];
+        // Rows go out by way of the query tile's memory (its products are complete), 2 D bytes of a row at a time, so that
+        // its lanes write them together: a row to a lane and 16 bytes at a time take a wavefront per row.
+        if (__any_sync(0xffffffffu, live)) {
+            constexpr int kRowBytes = 2 * D, kChunks = kRowBytes / 16, kAtOnce = 32 / kChunks;  // rows written together
+            unsigned char * const stage = sq + t * Sh::kTileBytes + (warp & 3) * 32 * kRowBytes;
+            const auto place = [&](int r, int chunk) {
+                return reinterpret_cast<uint4 *>(stage + r * kRowBytes + ((chunk & ~7) | ((chunk ^ r) & 7)) * 16);
+            };
+            const auto values = [&](int from, uint32_t * o) {  // 32 dimensions, scaled
 #pragma unroll
-                for (int x = 0; x < 32; ++x) v[x] = lim > 0 ? __uint_as_float(o[x]) * inv : 0.f;
+                for (int x = 0; x < 32; ++x) o[x] = lim > 0 ? __float_as_uint(__uint_as_float(o[x]) * inv) : 0u;
                 if (dirty) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) {
-                        if (seen[D + i + x] < uint32_t(lim)) v[x] += INFINITY;
-                        if (seen[2 * D + i + x] < uint32_t(lim)) v[x] -= INFINITY;
-                        if (seen[i + x] < uint32_t(lim)) v[x] = NAN;
+                        float v = __uint_as_float(o[x]);
+                        if (seen[D + from + x] < uint32_t(lim)) v += INFINITY;
+                        if (seen[2 * D + from + x] < uint32_t(lim)) v -= INFINITY;
+                        if (seen[from + x] < uint32_t(lim)) v = NAN;
+                        o[x] = __float_as_uint(v);
                     }
                 }
-                const int c0 = (i - pass * elems) / (elems / (kOutBytes / 16));  // first 16-byte chunk
-                const auto put = [&](int chunk, uint4 w) {
-                    *reinterpret_cast<uint4 *>(stage + lane * kOutBytes + ((chunk ^ (lane & 7)) << 4)) = w;
-                };
-                if (f32) {
-#pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        put(c0 + x, make_uint4(__float_as_uint(v[4 * x]), __float_as_uint(v[4 * x + 1]),
-                                               __float_as_uint(v[4 * x + 2]), __float_as_uint(v[4 * x + 3])));
-                } else {
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        put(c0 + x, make_uint4(pack2<T>(v[8 * x], v[8 * x + 1]), pack2<T>(v[8 * x + 2], v[8 * x + 3]),
-                                               pack2<T>(v[8 * x + 4], v[8 * x + 5]), pack2<T>(v[8 * x + 6], v[8 * x + 7])));
+            };
+            // the rows' places: row r of the warp is head (r mod P) of position r / P
+            const int first = (warp & 3) * 32, chunk = lane % kChunks, heads_mask = (1 << a.log_p) - 1;
+            const auto write = [&](int column) {  // bytes
+                __syncwarp();
+#pragma unroll 8
+                for (int r = lane / kChunks; r < 32; r += kAtOnce) {
+                    const uint4 w = *place(r, chunk);
+                    const int position = end.p0 + t * ppt + ((first + r) >> a.log_p), head = head0 + ((first + r) & heads_mask);
+                    const long long at = part ? (long long)(rec0 + first + r) * D : (long long)(end.q0 + position) * a.out_stride + head * D;
+                    if (position < end.nq && end.work && ok)
+                        *reinterpret_cast<uint4 *>(out + at * (f32 ? 4 : 2) + column + chunk * 16) = w;
                 }
+                __syncwarp();
+            };
+            uint32_t o[D];
+            if (tiles > 0 && ok) {
+#pragma unroll
+                for (int i = 0; i < D; i += 32) tmem_ld(to + i, o + i);
+                wait_ld();
             }
-            __syncwarp();
-            constexpr int kChunks = kOutBytes / 16, kAtOnce = 32 / kChunks;  // rows written together
-            const int chunk = lane % kChunks;
-            const long long column = (long long)pass * kOutBytes + chunk * 16;
-#pragma unroll 4
-            for (int r = lane / kChunks; r < 32; r += kAtOnce) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(stage + r * kOutBytes + ((chunk ^ (r & 7)) << 4));
-                const long long row_at = __shfl_sync(0xffffffffu, at, r);
-                if (__shfl_sync(0xffffffffu, int(live), r))
-                    *reinterpret_cast<uint4 *>(out + row_at * (f32 ? 4 : 2) + column) = w;
+#pragma unroll
+            for (int i = 0; i < D; i += 32) values(i, o + i);
+            if (f32) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                    for (int x = 0; x < kChunks; ++x) {
+                        const uint32_t * e = o + half * (D / 2) + 4 * x;
+                        *place(lane, x) = make_uint4(e[0], e[1], e[2], e[3]);
+                    }
+                    write(half * kRowBytes);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < kChunks; ++x) {
+                    const auto pair = [&](int i) { return pack2<T>(__uint_as_float(o[8 * x + 2 * i]), __uint_as_float(o[8 * x + 2 * i + 1])); };
+                    *place(lane, x) = make_uint4(pair(0), pair(1), pair(2), pair(3));
+                }
+                write(0);
             }
-            __syncwarp();
         }
     }
     fence_before();
