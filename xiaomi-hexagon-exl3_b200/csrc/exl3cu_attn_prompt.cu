@@ -127,7 +127,7 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint3
         : "memory");
 }
 
-// 32 consecutive TMEM columns of this thread's lane (wait_ld() before use).
+// 32 consecutive TMEM columns of this thread's lane (landed() before use).
 __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t * r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -137,6 +137,13 @@ __device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t * r) {
           "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
           "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
+}
+// wait_ld() for N columns: what uses them stays behind it.
+template <int N> __device__ __forceinline__ void landed(uint32_t * r) {
+    wait_ld();
+#pragma unroll
+    for (int i = 0; i < N; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t * r) {
     asm volatile(
@@ -558,7 +565,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             const int left = lim - j * kTile;
 #pragma unroll
             for (int i = 0; i < 4; ++i) tmem_ld(ts + 32 * i, s + 32 * i);
-            wait_ld();
+            landed<kTile>(s);
             if (edge) {
 #pragma unroll
                 for (int x = 0; x < kTile; ++x) s[x] = x < left ? s[x] : 0xff800000u;
@@ -578,7 +585,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     for (int i = 0; i < D; i += 32) {
                         uint32_t o[32];
                         tmem_ld(to + i, o);
-                        wait_ld();
+                        landed<32>(o);
 #pragma unroll
                         for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
                         tmem_st(to + i, o);
@@ -702,7 +709,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             if (tiles > 0 && ok) {
 #pragma unroll
                 for (int i = 0; i < D; i += 32) tmem_ld(to + i, o + i);
-                wait_ld();
+                landed<D>(o);
             }
 #pragma unroll
             for (int i = 0; i < D; i += 32) values(i, o + i);
