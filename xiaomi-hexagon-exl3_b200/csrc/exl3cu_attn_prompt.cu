@@ -679,7 +679,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             };
             const auto values = [&](int from, uint32_t * o) {  // 32 dimensions, scaled
 #pragma unroll
-                for (int x = 0; x < 32; ++x) o[x] = lim > 0 ? __float_as_uint(__uint_as_float(o[x]) * inv) : 0u;
+                for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * inv);
                 if (dirty) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x) {
@@ -709,7 +709,10 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             if (tiles > 0 && ok) {
 #pragma unroll
                 for (int i = 0; i < D; i += 32) tmem_ld(to + i, o + i);
-                landed<D>(o);
+                landed<D>(o);  // a row that sees nothing has sums of zero: its weights were, and the values are clean
+            } else {
+#pragma unroll
+                for (int i = 0; i < D; ++i) o[i] = 0;
             }
 #pragma unroll
             for (int i = 0; i < D; i += 32) values(i, o + i);
