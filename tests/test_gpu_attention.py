@@ -697,6 +697,58 @@ def test_native_and_python_calls_agree(A, dtype):
         assert a.dtype == b.dtype and torch.equal(a, b)
 
 
+def test_cache_past_32_bits(A):
+    """Slots whose codes begin beyond 4 GiB, rows at the end of a million positions; all the others are zeros."""
+    g = gen(41)
+    length, n = 1 << 20, 70
+    cache = A.Kv4Cache(9, 8, length, 128)
+    k, v = randn(g, n, 8, 128), randn(g, n, 8, 128)
+    slots = ints([8, 7])
+    cache.append(k, v, ints([0] * n), torch.arange(length - n, length, device="cuda").to(torch.int32), slots)
+    cache.append(k, v, ints([1] * n), torch.arange(n, device="cuda").to(torch.int32), slots)
+    kq, vq = (values(*stored(c[8, :, -n:], s[8, :, -n:])) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+    k1, v1 = cache.read(ints([7]), offsets([n + 3]), n + 3, torch.float32)
+    assert torch.equal(k1[:n], kq.transpose(0, 1).float()) and torch.equal(v1[:n], vq.transpose(0, 1).float())
+    assert not bool(k1[n:].any()) and not bool(v1[n:].any())
+    q = randn(g, 2, 8, 128) * 8
+    got = cache.attend(q, ints([0, 1]), ints([length - 1, n - 1]), slots)
+    s = torch.einsum("rhd,hnd->rhn", q.double(), kq) * 128 ** -0.5
+    rest = torch.tensor([length - n, 0], dtype=torch.float64, device="cuda")[:, None, None]  # scores of zero
+    top = s.amax(-1, keepdim=True).clamp_min(0)
+    e = (s - top).exp()
+    want = torch.einsum("rhn,hnd->rhd", e / (e.sum(-1, keepdim=True) + rest * (-top).exp()), vq)
+    size = torch.einsum("rhd,hnd->rhn", q.double().abs(), kq.abs()).amax(-1, keepdim=True) * 128 ** -0.5
+    close(got, want, (64 * size + 64) * U * vq.abs().max())
+
+
+def test_rows_past_32_bits(A):
+    """Rows 2^27 elements apart: queries, keys, values and outputs as columns of one buffer of 5.4 billion elements."""
+    g = gen(42)
+    n, stride = 40, 1 << 27
+    flat = torch.empty(n * stride, dtype=torch.float16, device="cuda")
+
+    def columns(at, heads):
+        return flat.as_strided((n, heads, 64), (stride, 64, 1), at)
+
+    q, k, v, out = columns(0, 8), columns(512, 2), columns(640, 2), columns(1024, 8)
+    for t in (q, k, v):
+        t.copy_(randn(g, *t.shape))
+    pos = torch.arange(n, device="cuda").to(torch.int32)
+    A.prompt_attention(q, k, v, offsets([n]), offsets([n]), out=out)
+    check_prompt(out, q, k, v, [n], [(0, n)])
+    inv = torch.tensor(A.rope_frequencies(64)[0], device="cuda")
+    A.qk_norm_rope(q, k, pos, inv, q_out=out, k_out=columns(2048, 2))
+    check_rope(out, q, None, pos, inv, 1e-6, False, 1.0)
+    check_rope(columns(2048, 2), k, None, pos, inv, 1e-6, False, 1.0)
+    cache = A.Kv4Cache(1, 2, n, 64)
+    cache.append(k, v, pos * 0, pos, ints([0]))
+    cache.read(ints([0]), offsets([n]), n, k_out=columns(4096, 2), v_out=columns(4224, 2))
+    kq, vq = (values(*stored(c[0, :, :n], s[0, :, :n])) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+    assert torch.equal(columns(4096, 2), kq.transpose(0, 1).half()) and torch.equal(columns(4224, 2), vq.transpose(0, 1).half())
+    cache.attend(q, pos * 0, pos, ints([0]), out=out)
+    check_attend(out, q, cache, [0] * n, list(range(1, n + 1)))
+
+
 def test_calls_on_two_streams_at_once(A):
     """Calls that overlap on two streams, given as arguments, leave each other's results alone."""
     g = gen(14)
