@@ -71,6 +71,8 @@ def _lib():
 def _native():
     """csrc/exl3cu_attn_torch.cpp: the calls below in ordinary form (NotImplemented for any other)."""
     L = _lib()
+    if not TORCH_LIB_PATH.exists():
+        raise ImportError(f"{TORCH_LIB_PATH} is not built; run xiaomi-hexagon-exl3_b200/build.py")
     loader = importlib.machinery.ExtensionFileLoader("exl3cu_torch", str(TORCH_LIB_PATH))
     mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("exl3cu_torch", loader))
     loader.exec_module(mod)
