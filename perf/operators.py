@@ -28,20 +28,13 @@ SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 EPS = 1e-6
 
 
-_module = None
-
-
 def _framework():
-    """exl3_b200.attention, imported once as a program does."""
-    global _module
-    if _module is None:
-        path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xiaomi-hexagon-exl3_b200")
-        if path not in sys.path:
-            sys.path.insert(0, path)
-        from exl3_b200 import attention
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "xiaomi-hexagon-exl3_b200")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    from exl3_b200 import attention
 
-        _module = attention
-    return _module
+    return attention
 
 
 def lengths(count, longest, shortest):
