@@ -243,7 +243,7 @@ def rope_frequencies(rotary_dim: int, theta: float = 1e4, factor: float = 1.0, o
     def dim_of(turns):  # the index whose frequency turns so often within original_len
         return rotary_dim * np.log(original_len / (turns * 2 * np.pi)) / (2 * np.log(theta))
 
-    low, high = max(np.floor(dim_of(fast)), 0), min(np.ceil(dim_of(slow)), rotary_dim // 2 - 1)
+    low, high = max(np.floor(dim_of(fast)), 0), min(np.ceil(dim_of(slow)), rotary_dim - 1)
     ramp = np.clip((i - low) / max(high - low, 1e-3), 0, 1)
     return (f / factor * ramp + f * (1 - ramp)).astype(np.float32), float(0.1 * np.log(factor) + 1.0)
 
