@@ -1,0 +1,63 @@
+"""Attention over the 4-bit cache where magnitudes differ: between groups of dimensions, between keys, between queries
+and scale.  References, tolerances' terms (u = 2^-24, A, W) and helpers are those of test_gpu_attention; here a result is
+held to the magnitudes of its own group of dimensions (dimension d is of group d mod D/32), not to the head's largest."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_attention import TYPES, U, close, fill, gen, half_step, ints, randn, ref_attention, stored, tiny, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def A(cuda_lib):
+    from exl3_b200 import attention
+
+    return attention
+
+
+def check_groups(got, q, cache, slots, lens, scale=None):
+    """check_attend with W and max |v| of each group by itself."""
+    rows, heads, dim = q.shape
+    scale = dim ** -0.5 if scale is None else scale
+    share, G = heads // cache.kv_heads, dim // 32
+    kv, vv = (values(*stored(c, s)) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+    for r, (slot, n) in enumerate(zip(slots, lens)):
+        for h in range(heads):
+            for j in range(G):
+                want, a, w, top = ref_attention(q[r, h:h + 1], kv[slot, h // share, :n], vv[slot, h // share, :n, j::G], n, scale)
+                tol = (64 * a + 64) * U * top + half_step(got.dtype) * want.abs() + tiny(got.dtype)
+                if got.dtype != torch.float32:
+                    tol = tol + 2.0 ** -11 * w
+                close(got[r, h:h + 1, j::G], want, tol, (r, h, n, j))
+
+
+# a cluster to a row, shares (few and many parts), a CTA to a row
+PATHS = [dict(rows=1, max_len=1024), dict(rows=2, max_len=8192), dict(rows=100, max_len=4160), dict(rows=257, max_len=1024)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (8, 1, 128), (8, 1, 64), (3, 1, 64)])
+@pytest.mark.parametrize("path", PATHS, ids=lambda p: f"{p['rows']}x{p['max_len']}")
+def test_small_groups_beside_large_ones(A, dtype, heads, kv, dim, path):
+    """Value scales of one group up to 2^32 times those of another, from the first key on and from a later one on."""
+    g = gen(dim + heads)
+    G, n = dim // 32, 1000
+    cache = A.Kv4Cache(2, kv, path["max_len"], dim)
+    fill(cache, g)
+    low, high = (0.02, 1e4) if dtype == torch.float16 else (1e-5, 6e4)
+    size = torch.full((G,), low, device="cuda")
+    size[1], size[-1] = high, (high if G == 2 else 1.0)
+    for slot in range(2):
+        x = torch.rand(cache.v_scales[slot].shape, generator=g, device="cuda") * 0.5 + 0.5
+        big = torch.ones(path["max_len"], dtype=torch.bool, device="cuda") if slot == 0 else \
+            torch.arange(path["max_len"], device="cuda") == 700
+        cache.v_scales[slot] = torch.where(big[None, :, None], x * size, x * low).half()
+    rows = path["rows"]
+    q = randn(g, rows, heads, dim).to(dtype)
+    slots = [r % 2 for r in range(rows)]
+    got = cache.attend(q, ints(slots), ints([n - 1] * rows), ints([0, 1]))
+    some = [r for r in range(rows) if r < 2 or r >= rows - 2]
+    check_groups(got[some], q[some], cache, [slots[r] for r in some], [n] * len(some))

@@ -564,7 +564,8 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 // halves what a lane computes around the products; of f32 rows the pair's second column holds the low half of the
 // operand, x = hi + lo to 2^-22.  (16-bit rows: weights rounded to 2^-11 of their value, the result's own precision.)
 // Both operands are scaled by powers of two into the half's range: q by its largest element, the weights by the largest
-// value scale seen, so that nothing overflows or vanishes whatever the cache holds.  The maximum that the weights
+// value scale seen of their group, so that nothing overflows and a group of small values beside one of large ones keeps
+// its digits.  The maximum that the weights
 // refer to follows the true one when it has grown by more than 2^kLazy.  Masked keys get a score of -inf and scales of
 // zero; codes are finite whatever they are.
 //
@@ -849,10 +850,18 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 
         // accumulators; the score that weights refer to (before cs); sum of the weights.  Weights are
         // exp2((s - m) cs + 14 + kTop - ev), ev the exponent of the largest value scale seen, which is below 2^(ev - 14).
+        // The value scales of a group whose own largest is smaller are raised by what it is smaller, a power of two up to
+        // 2^15, before they meet the weights: exact in a half, and a group 2^15 further down still has its weights at
+        // 2^(kTop - 15).  evs: the groups' own exponents as they stand in a half, two to a word.  (Accumulators o[i] are
+        // of group i mod G.)
         float o[D / 16][4] = {}, m[H], l[H] = {};
 #pragma unroll
         for (int j = 0; j < H; ++j) m[j] = -INFINITY;
         int ev = 0;
+        uint32_t evs[G / 2] = {};
+        // exponents of the groups' largest scales as raised, in a half's place: no more than 15 below ev
+        const auto raised = [&](int i) { return __vmaxu2(evs[i], uint32_t(max(ev - 15, 0)) * 0x04000400u); };
+        const auto exponent = [&](int j) { return int(raised(j / 2) >> (16 * (j & 1) + 10) & 31u); };  // of group j
         for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
             const unsigned char * kc = ring + (used % kStages) * Tile::kBytes;
             const unsigned char * ks = kc + Tile::kCodes, * vc = ks + Tile::kScales, * vs = vc + Tile::kCodes;
@@ -921,18 +930,16 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 #pragma unroll
                             for (int j = 0; j < H; ++j) sc[x][y][j] = -INFINITY;
             }
-            // exponent of the largest value scale of the lane's two keys; the lane's largest scores.  The others' are
-            // asked for only where something has moved: exchanges would stand in every tile's way.
-            int top;
+            // exponents of the groups' largest value scales of the lane's two keys; the lane's largest scores.  The others'
+            // are asked for only where something has moved: exchanges would stand in every tile's way.
+            bool moved = false;
             {
-                uint32_t w[G], most;
+                uint32_t w[G];
                 lds(vs + lane * (4 * G), w);
-                most = w[0] & 0x7fff7fffu;
 #pragma unroll
-                for (int i = 1; i < G; ++i) most = __vmaxu2(most, w[i] & 0x7fff7fffu);
-                top = int(max(most & 0xffffu, most >> 16) >> 10);
+                for (int i = 0; i < G / 2; ++i)
+                    moved = moved || __vmaxu2(__vmaxu2(w[i] & 0x7c007c00u, w[i + G / 2] & 0x7c007c00u), evs[i]) != evs[i];
             }
-            bool moved = top > ev;
             float mx[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) {
@@ -942,37 +949,57 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 moved = moved || (mx[j] - m[j]) * cs[j] > float(kLazy);  // no: both -inf
             }
             if (__any_sync(0xffffffffu, moved)) {
-                if (top == 31) {  // not finite: its group of dimensions is, and the others' weights keep their range
-                    uint32_t w[G], most = 0;
+                int before[G];
+#pragma unroll
+                for (int i = 0; i < G; ++i) before[i] = exponent(i);
+                const int ev_before = ev;
+                {
+                    uint32_t w[G];
                     lds(vs + lane * (4 * G), w);
 #pragma unroll
-                    for (int i = 0; i < G; ++i) {
-                        const uint32_t lo = w[i] & 0x7fffu, hi = w[i] >> 16 & 0x7fffu;
-                        most = max(most, max(lo < 0x7c00u ? lo : 0u, hi < 0x7c00u ? hi : 0u));
+                    for (int i = 0; i < G / 2; ++i) {
+                        uint32_t e = 0;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {  // a scale that is not finite does not count: its group's result is not either
+                            const uint32_t x = w[i + k * (G / 2)] & 0x7c007c00u;
+                            e = __vmaxu2(e, x & ~__vcmpeq2(x, 0x7c007c00u));
+                        }
+                        const uint32_t lo = __reduce_max_sync(0xffffffffu, e & 0xffffu), hi = __reduce_max_sync(0xffffffffu, e >> 16);
+                        evs[i] = __vmaxu2(evs[i], lo | hi << 16);
+                        ev = max(ev, int(max(evs[i] & 0xffffu, evs[i] >> 16) >> 10));
                     }
-                    top = int(most >> 10);
                 }
-                const int grown = max(__reduce_max_sync(0xffffffffu, top) - ev, 0);
-                ev += grown;
-                const float down = pow2(-grown);
+                float f[H];
 #pragma unroll
                 for (int j = 0; j < H; ++j) {
 #pragma unroll
                     for (int x = 4; x < 32; x <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], x));
-                    const float f = (mx[j] == m[j] ? 1.f : exp2_approx((m[j] - mx[j]) * cs[j])) * down;
+                    f[j] = mx[j] == m[j] ? 1.f : exp2_approx((m[j] - mx[j]) * cs[j]);
                     m[j] = mx[j];
-                    l[j] *= f;
+                }
+                if (tile != t0 + warp) {  // sums so far
+                    float down[G];
 #pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        o[i][j] *= f;
-                        o[i][2 + j] *= f;
-                        if (LO) {
-                            o[i][1] *= f;
-                            o[i][3] *= f;
+                    for (int i = 0; i < G; ++i) down[i] = pow2(before[i] - exponent(i));
+#pragma unroll
+                    for (int j = 0; j < H; ++j) {
+                        l[j] *= f[j] * pow2(ev_before - ev);
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i) {
+                            const float fg = f[j] * down[i % G];
+                            o[i][j] *= fg;
+                            o[i][2 + j] *= fg;
+                            if (LO) {
+                                o[i][1] *= fg;
+                                o[i][3] *= fg;
+                            }
                         }
                     }
                 }
             }
+            uint32_t raise[G / 2];  // 2^(ev - the exponent as raised), two halves
+#pragma unroll
+            for (int i = 0; i < G / 2; ++i) raise[i] = uint32_t(15 + ev) * 0x04000400u - raised(i);
             float ref[H];
 #pragma unroll
             for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : float(14 + kTop - ev) - m[j] * cs[j];
@@ -982,6 +1009,11 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 uint32_t s0[G / 2], s1[G / 2];
                 lds(vs + k0 * (2 * G), s0);
                 lds(vs + (k0 + 8) * (2 * G), s1);
+#pragma unroll
+                for (int j = 0; j < G / 2; ++j) {
+                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(s0[j]) : "r"(raise[j]));
+                    asm("mul.rn.f16x2 %0, %0, %1;" : "+r"(s1[j]) : "r"(raise[j]));
+                }
                 float p[2][H];
 #pragma unroll
                 for (int y = 0; y < 2; ++y)
@@ -1051,7 +1083,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         constexpr int kRec = D + 4;
         float * const mine = reinterpret_cast<float *>(ring);
         __syncwarp();
-        const float back = pow2(ev - 14 - kTop);
+        float back[G];
+#pragma unroll
+        for (int i = 0; i < G; ++i) back[i] = pow2(exponent(i) - 14 - kTop);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
 #pragma unroll
@@ -1060,12 +1094,12 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const int d = D == 128 ? 16 * g + i : 8 * g + i;
-                rec[d] = (LO ? o[i][0] + o[i][1] : o[i][j]) * back;
-                rec[d + (D == 128 ? 8 : 4)] = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) * back;
+                rec[d] = (LO ? o[i][0] + o[i][1] : o[i][j]) * back[i % G];
+                rec[d + (D == 128 ? 8 : 4)] = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) * back[i % G];
             }
             if (g == 0) {
                 rec[D] = m[j] * cs[j];
-                rec[D + 1] = l[j] * back;
+                rec[D + 1] = l[j] * pow2(ev - 14 - kTop);
             }
         }
         __syncthreads();
