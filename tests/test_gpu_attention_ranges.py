@@ -61,3 +61,32 @@ def test_small_groups_beside_large_ones(A, dtype, heads, kv, dim, path):
     got = cache.attend(q, ints(slots), ints([n - 1] * rows), ints([0, 1]))
     some = [r for r in range(rows) if r < 2 or r >= rows - 2]
     check_groups(got[some], q[some], cache, [slots[r] for r in some], [n] * len(some))
+
+
+def one_hot(rows, heads, dim, size, dtype):
+    q = torch.zeros((rows, heads, dim), device="cuda")
+    q[:, torch.arange(heads), torch.arange(heads) * 5 % dim] = size
+    return q.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,size,key", [
+    (torch.float32, 2.0 ** 10, 2.0 ** -3), (torch.float32, 2.0 ** 24, 2.0 ** -3), (torch.float32, 2.0 ** 40, 2.0 ** -3),
+    (torch.float32, 2.0 ** 100, 2.0 ** 3), (torch.bfloat16, 2.0 ** 26, 2.0 ** -3), (torch.bfloat16, 2.0 ** 90, 1.0),
+    (torch.float16, 2.0 ** 15, 2.0 ** 15)])
+@pytest.mark.parametrize("heads,dim", [(4, 128), (8, 128), (8, 64)])
+@pytest.mark.parametrize("max_len", [1024, 8192])
+def test_attend_scores_of_any_size(A, dtype, size, key, heads, dim, max_len):
+    """Scores are exact (one product of powers of two and a code), so that the term in A falls away: the keys of the
+    largest score share the result, however large it is."""
+    g = gen(heads + dim)
+    cache = A.Kv4Cache(1, 1, max_len, dim)
+    fill(cache, g)
+    cache.k_scales.fill_(key)
+    q = one_hot(3, heads, dim, size, dtype)
+    lens = [1, 77, 1000]
+    got = cache.attend(q, ints([0] * 3), ints([n - 1 for n in lens]), ints([0]), scale=1.0)
+    k, v = (values(*stored(c[0, 0], s[0, 0])) for c, s in ((cache.k_codes, cache.k_scales), (cache.v_codes, cache.v_scales)))
+    for r, n in enumerate(lens):
+        want, _, w, top = ref_attention(q[r], k[:n], v[:n], n, 1.0)
+        tol = 64 * U * top + half_step(dtype) * want.abs() + tiny(dtype)
+        close(got[r], want, tol if dtype == torch.float32 else tol + 2.0 ** -11 * w, (r, n))

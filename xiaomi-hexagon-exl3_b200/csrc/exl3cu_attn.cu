@@ -1000,9 +1000,13 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
             uint32_t raise[G / 2];  // 2^(ev - the exponent as raised), two halves
 #pragma unroll
             for (int i = 0; i < G / 2; ++i) raise[i] = uint32_t(15 + ev) * 0x04000400u - raised(i);
-            float ref[H];
+            // the difference to m before the factor: with a rounded m cs in its place, scores above 2^24 would be off by
+            // whole powers of two
+            const float top = float(14 + kTop - ev);
+            float less[H];
 #pragma unroll
-            for (int j = 0; j < H; ++j) ref[j] = m[j] == -INFINITY ? 0.f : float(14 + kTop - ev) - m[j] * cs[j];
+            for (int j = 0; j < H; ++j) less[j] = m[j] == -INFINITY ? 0.f : -m[j];
+            const uint64_t less2 = two(less[0], less[H - 1]), cs2 = two(cs[0], cs[H - 1]), top2 = two(top, top);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int k0 = 16 * x + key_of<D>(g);
@@ -1016,12 +1020,13 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 }
                 float p[2][H];
 #pragma unroll
-                for (int y = 0; y < 2; ++y)
-#pragma unroll
-                    for (int j = 0; j < H; ++j) {
-                        p[y][j] = exp2_approx(fmaf(sc[x][y][j], cs[j], ref[j]));
-                        l[j] += p[y][j];
-                    }
+                for (int i = 0; i < H; ++i) {  // two at a time: the keys of a head (PAIR), or the heads of a key
+                    const float2 e = of_two(fma2(add2(two(sc[x][PAIR ? 0 : i][0], PAIR ? sc[x][1][0] : sc[x][i][H - 1]), less2), cs2, top2));
+                    p[PAIR ? 0 : i][0] = exp2_approx(e.x);
+                    p[PAIR ? 1 : i][H - 1] = exp2_approx(e.y);
+                    l[0] += p[PAIR ? 0 : i][0];
+                    l[H - 1] += p[PAIR ? 1 : i][H - 1];
+                }
                 uint32_t pb[G][2];
 #pragma unroll
                 for (int j = 0; j < G; ++j)
