@@ -90,3 +90,17 @@ def test_attend_scores_of_any_size(A, dtype, size, key, heads, dim, max_len):
         want, _, w, top = ref_attention(q[r], k[:n], v[:n], n, 1.0)
         tol = 64 * U * top + half_step(dtype) * want.abs() + tiny(dtype)
         close(got[r], want, tol if dtype == torch.float32 else tol + 2.0 ** -11 * w, (r, n))
+
+
+@pytest.mark.parametrize("dtype,size,scale", [
+    (torch.float32, 1e-25, 1e25), (torch.float32, 1e-30, 1e30), (torch.float32, 1e-36, 1e30), (torch.bfloat16, 1e-30, 1e30),
+    (torch.float32, 1e20, 1e-20), (torch.bfloat16, 1e30, 1e-30), (torch.float16, 2.0 ** -18, 2.0 ** 18)])
+@pytest.mark.parametrize("max_len", [512, 8192])
+def test_attend_small_queries_and_large_scales(A, dtype, size, scale, max_len):
+    g = gen(52)
+    cache = A.Kv4Cache(2, 2, max_len, 128)
+    fill(cache, g)
+    cache.k_scales.mul_(4)
+    q = (randn(g, 2, 8, 128) * size).to(dtype)
+    lens = [500, 65]
+    check_groups(cache.attend(q, ints([0, 1]), ints([n - 1 for n in lens]), ints([1, 0]), scale=scale), q, cache, [1, 0], lens, scale)

@@ -823,7 +823,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int ex = int(__float_as_uint(top) >> 23);  // 255: an infinity
-            const int e = ex == 255 ? 0 : min(135 - ex, 60);  // below 2^-52 a query's scores are 0 but for 2^-40
+            const int e = ex == 255 ? 0 : min(135 - ex, 126);  // f32 has no smaller normal than 2^-126, which becomes 1
             const float up = pow2(e);
 #pragma unroll
             for (int i = 0; i < D / 4; ++i) {
