@@ -104,3 +104,32 @@ def test_attend_small_queries_and_large_scales(A, dtype, size, scale, max_len):
     q = (randn(g, 2, 8, 128) * size).to(dtype)
     lens = [500, 65]
     check_groups(cache.attend(q, ints([0, 1]), ints([n - 1 for n in lens]), ints([1, 0]), scale=scale), q, cache, [1, 0], lens, scale)
+
+
+@pytest.mark.parametrize("heads,kv,dim", [(4, 1, 128), (8, 2, 64)])
+@pytest.mark.parametrize("max_len", [1024, 8192])
+def test_attend_f32_rows_keep_their_digits(A, heads, kv, dim, max_len):
+    """f32 rows as pairs of halves: small elements of a query beside a large one where the keys make up for it, and
+    values 2^-21 of those of a key whose weight is below 2^-40; held to W instead of the largest value."""
+    g = gen(dim)
+    G, n = dim // 32, 900
+    cache = A.Kv4Cache(1, kv, max_len, dim)
+    fill(cache, g)
+    cache.k_scales[..., 0], cache.k_scales[..., 1:] = 2.0 ** -10, 2.0 ** 10
+    q = randn(g, 1, heads, dim)
+    q[..., [d for d in range(dim) if d % G]] *= 2.0 ** -20
+    scale = 2.0 ** 10 / dim ** 0.5
+    check_groups(cache.attend(q, ints([0]), ints([n - 1]), ints([0]), scale=scale), q, cache, [0], [n], scale)
+
+    cache.k_scales.fill_(2.0 ** -3)
+    cache.v_scales.copy_(torch.rand(cache.v_scales.shape, generator=g, device="cuda") * 0.01 + 0.02)
+    for at in (0, 500):
+        c = A.Kv4Cache.from_tensors(*(t.clone() for t in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)))
+        c.v_scales[:, :, at] = 6e4
+        c.k_codes[:, :, at] = 0x11                          # -7 everywhere
+        q = torch.full((1, heads, dim), 0.5, device="cuda") + 0.1 * randn(g, 1, heads, dim)
+        got = c.attend(q, ints([0]), ints([n - 1]), ints([0]), scale=1.0)
+        for h in range(heads):
+            k, v = (values(*stored(a[0, h // (heads // kv)], b[0, h // (heads // kv)]))[:n] for a, b in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
+            want, a, w, _ = ref_attention(q[0, h:h + 1], k, v, n, 1.0)
+            close(got[0, h:h + 1], want, (64 * a + 64) * U * w + half_step(torch.float32) * want.abs(), (at, h))

@@ -561,8 +561,9 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 //   (B: the score fragment, transposed by movmatrix).
 //
 // Columns: 8 heads of 16-bit rows, or, where no more than 4 share a K/V head, one head to a pair of columns, which
-// halves what a lane computes around the products; of f32 rows the pair's second column holds the low half of the
-// operand, x = hi + lo to 2^-22.  (16-bit rows: weights rounded to 2^-11 of their value, the result's own precision.)
+// halves what a lane computes around the products; of f32 rows the pair's second column holds what the first
+// one's rounding left, 2^11 times as large so that it keeps its digits where x is small: x = hi + 2^-11 lo to 2^-22 of x
+// down to 2^-25 of the largest, and to 2^-36 of a half's unit below.  (16-bit rows: weights rounded to 2^-11 of their value, the result's own precision.)
 // Both operands are scaled by powers of two into the half's range: q by its largest element, the weights by the largest
 // value scale seen of their group, so that nothing overflows and a group of small values beside one of large ones keeps
 // its digits.  The maximum that the weights
@@ -591,7 +592,8 @@ constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
 // 8191 positions 10.6 against 9.7, 32 rows of 767 21.2 against 13.9.
 constexpr int kCluster = 8;
 constexpr int kClusterTiles = 64;
-constexpr int kLazy = 6, kTop = 14 - kLazy;  // weights times value scales are up to 2^kTop, 2^14 before m moves
+constexpr int kLazy = 6, kTop = 15 - kLazy;  // weights times value scales are up to 2^kTop, 2^15 before m moves
+constexpr float kLow = 2048.f;   // of the low parts of f32 operands
 
 template <int D> struct Kv4Tile {
     static constexpr int kCodes = kKeys * D / 2, kScales = kKeys * D / 16;  // bytes of one of K and V
@@ -830,7 +832,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 x[i] *= up;
                 if (LO) {
                     const float hi = __half2float(__float2half_rn(x[i]));
-                    x[i] = g & 1 ? x[i] - hi : hi;
+                    x[i] = g & 1 ? (x[i] - hi) * kLow : hi;
                 } else if (PAIR && (g & 1)) {
                     x[i] = 0.f;
                 }
@@ -914,8 +916,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                     const float a0 = j & 1 ? f0.y : f0.x, a1 = j & 1 ? f1.y : f1.x;
 #pragma unroll
                     for (int jj = 0; jj < H; ++jj) {
-                        const float v0 = LO ? acc[j][0] + acc[j][1] : acc[j][jj];
-                        const float v1 = LO ? acc[j][2] + acc[j][3] : acc[j][2 + jj];
+                        const float v0 = LO ? fmaf(acc[j][1], 1.f / kLow, acc[j][0]) : acc[j][jj];
+                        const float v1 = LO ? fmaf(acc[j][3], 1.f / kLow, acc[j][2]) : acc[j][2 + jj];
                         sc[x][0][jj] = j ? fmaf(a0, v0, sc[x][0][jj]) : a0 * v0;
                         sc[x][1][jj] = j ? fmaf(a1, v1, sc[x][1][jj]) : a1 * v1;
                     }
@@ -1034,7 +1036,7 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                     for (int y = 0; y < 2; ++y) {
                         const float2 f = h2f2(y ? s1[j / 2] : s0[j / 2]);
                         const float sv = j & 1 ? f.y : f.x, v0 = p[y][0] * sv;
-                        pb[j][y] = transpose8x8(LO ? pack_h2(v0, v0 - __half2float(__float2half_rn(v0)))
+                        pb[j][y] = transpose8x8(LO ? pack_h2(v0, (v0 - __half2float(__float2half_rn(v0))) * kLow)
                                                    : pack_h2(v0, PAIR ? 0.f : p[y][H - 1] * sv));
                     }
                 // values of keys 2 t, 2 t + 1 and 8 further (as the score rows count them): dimensions of word(s) g
@@ -1099,8 +1101,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
                 const int d = D == 128 ? 16 * g + i : 8 * g + i;
-                rec[d] = (LO ? o[i][0] + o[i][1] : o[i][j]) * back[i % G];
-                rec[d + (D == 128 ? 8 : 4)] = (LO ? o[i][2] + o[i][3] : o[i][2 + j]) * back[i % G];
+                rec[d] = (LO ? fmaf(o[i][1], 1.f / kLow, o[i][0]) : o[i][j]) * back[i % G];
+                rec[d + (D == 128 ? 8 : 4)] = (LO ? fmaf(o[i][3], 1.f / kLow, o[i][2]) : o[i][2 + j]) * back[i % G];
             }
             if (g == 0) {
                 rec[D] = m[j] * cs[j];
