@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import TYPES, U, close, fill, gen, half_step, ints, randn, ref_attention, stored, tiny, values
+from test_gpu_attention import TYPES, U, close, fill, gen, half_step, ints, randn, ref_attention, ref_prompt, stored, tiny, values
 
 pytestmark = pytest.mark.gpu
 
@@ -90,6 +90,26 @@ def test_attend_scores_of_any_size(A, dtype, size, key, heads, dim, max_len):
         want, _, w, top = ref_attention(q[r], k[:n], v[:n], n, 1.0)
         tol = 64 * U * top + half_step(dtype) * want.abs() + tiny(dtype)
         close(got[r], want, tol if dtype == torch.float32 else tol + 2.0 ** -11 * w, (r, n))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("value", [-math.inf, math.inf, math.nan])
+def test_prompt_queries_not_finite(A, dtype, value):
+    """A query whose every score is -inf has no softmax: NaN, as with +inf and NaN; the other rows keep their results (to
+    the tolerance: when the reference of a row's weights moves is decided for a warp's rows together)."""
+    g = gen(51)
+    n = 400
+    q = randn(g, n, 4, 64).to(dtype)
+    k, v = randn(g, n, 1, 64).to(dtype), randn(g, n, 1, 64).to(dtype)
+    k[:, 0, 3] = k[:, 0, 3].abs() + 0.5
+    bad = q.clone()
+    rows = [0, 5, 127, 128, 300, 399]
+    bad[rows, 2, 3] = value
+    got = A.prompt_attention(bad, k, v, ints([0, n]), ints([0, n]))
+    assert bool(got[rows, 2].isnan().all())
+    want, tol = ref_prompt(q, k, v, [n], [(0, n)], 64 ** -0.5)
+    got[rows, 2] = want[rows, 2].to(dtype)
+    close(got, want, tol + half_step(dtype) * want.abs() + 8 * tiny(dtype))
 
 
 @pytest.mark.parametrize("dtype,size,scale", [

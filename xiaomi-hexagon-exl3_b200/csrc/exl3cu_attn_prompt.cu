@@ -660,7 +660,8 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const View end(a, bars.work);
         const int p = end.p0 + t * ppt + (row >> a.log_p);
         const bool live = end.work && ok && p < end.nq, part = end.part;
-        const float inv = part ? 1.f : lim > 0 ? 1.f / sum : 0.f;
+        // scores of -inf alone have no softmax (their weights on the multiply-add pipe are not quite 0)
+        const float inv = part ? 1.f : lim <= 0 ? 0.f : m == -INFINITY ? NAN : 1.f / sum;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         // a share's part goes to scratch as it is, in f32, with what its weights refer to
         const bool f32 = part || a.out_f32;
