@@ -106,6 +106,7 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
  * head can address.  A key or value that a query does not see never reaches its
  * result, whatever it holds.  Packed K/V: kv_begin = offsets, kv_end = offsets + 1.
  * dtype (q, k, v): EXL3CU_F16 or EXL3CU_BF16; scale > 0; out_dtype: the same or EXL3CU_F32.
+ * A row whose largest score (scale * q . k) is beyond 2^26 in size may become NaN.
  * Query rows outside every sequence are left as they were; q_rows is the rows
  * that d_q and d_out hold.  With d_scratch (exl3cu_prompt_attn_scratch_bytes()
  * bytes, 16-byte aligned, contents arbitrary; calls that may run at the same time

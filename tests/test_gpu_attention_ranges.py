@@ -92,6 +92,51 @@ def test_attend_scores_of_any_size(A, dtype, size, key, heads, dim, max_len):
         close(got[r], want, tol if dtype == torch.float32 else tol + 2.0 ** -11 * w, (r, n))
 
 
+@pytest.mark.parametrize("dtype,size,key", [
+    (torch.float16, 2.0 ** 15, 2.0 ** 4), (torch.float16, 2.0 ** 15, 2.0 ** 7), (torch.float16, 2.0 ** 15, 2.0 ** 8),
+    (torch.bfloat16, 2.0 ** 20, 2.0 ** 3), (torch.bfloat16, 2.0 ** 40, 2.0 ** -17),
+    (torch.float16, 2.0 ** 15, 2.0 ** 12), (torch.bfloat16, 2.0 ** 60, 2.0 ** 40)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("past", [0, 3000])
+def test_prompt_large_scores(A, dtype, size, key, dim, past):
+    """The same for prompts, whole and with their keys divided among CTAs, up to the documented 2^26; a row whose
+    largest score is beyond that becomes NaN."""
+    g = gen(dim + past)
+    n = 300
+    q = one_hot(n, 4, dim, size, dtype)
+    k = (torch.randint(-7, 8, (n + past, 1, dim), generator=g, device="cuda") * key).to(dtype)
+    k[0] = 7 * key                                          # the largest score is 7 size key for every row
+    v = randn(g, n + past, 1, dim).to(dtype)
+    got = A.prompt_attention(q, k, v, ints([0, n]), ints([0, n + past]), scale=1.0)
+    if 7 * size * key > 2.0 ** 27:
+        assert bool(got.isnan().all())
+        return
+    for h in range(4):
+        want, _, w, _ = ref_attention(q[:, h], k[:, 0], v[:, 0], past, 1.0)
+        tol = (1.5 * half_step(dtype) + 64 * U) * w + half_step(dtype) * want.abs() + 8 * tiny(dtype)
+        close(got[:, h], want, tol, h)
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("past", [1000, 6000])
+def test_prompt_scores_far_below_the_others(A, dtype, past):
+    """Scores of -2^29 before ordinary ones: they have no weight, as in 64 bits."""
+    g = gen(past)
+    n, early = 40, past // 2
+    q = randn(g, n, 4, 64).to(dtype)
+    q[..., 0] = 2.0 ** 15
+    k, v = randn(g, n + past, 1, 64).to(dtype), randn(g, n + past, 1, 64).to(dtype)
+    k[..., 0] = 0
+    k[:early, 0, 0] = -2.0 ** 14
+    got = A.prompt_attention(q, k, v, ints([0, n]), ints([0, n + past]), scale=1.0)
+    for h in range(4):
+        # the score's term in A is that of the keys that have weight: q and k without dimension 0
+        want, _, w, _ = ref_attention(q[:, h], k[early:, 0], v[early:, 0], past - early, 1.0)
+        _, a, _, _ = ref_attention(q[:, h, 1:], k[early:, 0, 1:], v[early:, 0], past - early, 1.0)
+        tol = (1.5 * half_step(dtype) + (64 * a + 64) * U) * w + half_step(dtype) * want.abs() + 8 * tiny(dtype)
+        close(got[:, h], want, tol, h)
+
+
 @pytest.mark.parametrize("dtype", TYPES[1:])
 @pytest.mark.parametrize("value", [-math.inf, math.inf, math.nan])
 def test_prompt_queries_not_finite(A, dtype, value):

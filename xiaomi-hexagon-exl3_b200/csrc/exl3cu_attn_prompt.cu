@@ -59,6 +59,7 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 // Weights are scaled by 2^kShift, up to 2^14 when the maximum lags by its 2^8: so that a half holds those of a
 // long, flat tail too (2^-30 of the largest), and none overflows.
 constexpr int kShift = 6;
+constexpr float kFar = 134217728.f;  // 2^27: scores (times log2 e) that a weight's exponent can still tell apart
 // Tiles of keys of a share at least, where a block's keys are shared among CTAs: 512 rows behind 1000 keys 21.5 us with 4,
 // 25.3 with 6 or without sharing; behind 4000 keys 29.8, 29.6 with 6, 33.7 with 10, 61.8 without.
 constexpr int kMinSplit = 4;
@@ -553,7 +554,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
         const int lim = view.sees(view.p0 + t * ppt + (row >> a.log_p));
         const int tile_sees = view.sees(view.p0 + t * ppt);
-        const float c = a.scale_log2;
+        const float c = a.scale_log2, far = kFar / c;
         float m = -INFINITY, sum = 0.f;
         const int tiles = nt[t];
         bool ok = true;
@@ -593,8 +594,10 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     }
                 }
             }
-            // a row that has seen nothing: all weights 0; +inf among the scores: all NaN, as inf - inf is
-            const float mc = m == -INFINITY ? 0.f : m == INFINITY ? NAN : m * c - float(kShift);
+            // A row that has seen nothing, or nothing above -kFar: all weights 0.  m c is rounded up, so that no weight
+            // overflows; the rounding takes up to 2^-16 off all of them where |m c| comes to kFar, and a half has room
+            // for that.  Above kFar, +inf included: all NaN.
+            const float mc = m < -far ? 0.f : m > far ? NAN : __fmaf_ru(m, c, -float(kShift));
             const uint64_t c2 = two(c, c), mc2 = two(-mc, -mc);
             uint64_t add[2] = {0, 0};
             // masked scores have to become 0: at a view's end the polynomial is not used
@@ -660,15 +663,15 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const View end(a, bars.work);
         const int p = end.p0 + t * ppt + (row >> a.log_p);
         const bool live = end.work && ok && p < end.nq, part = end.part;
-        // scores of -inf alone have no softmax (their weights on the multiply-add pipe are not quite 0)
-        const float inv = part ? 1.f : lim <= 0 ? 0.f : m == -INFINITY ? NAN : 1.f / sum;
+        // scores of -inf (or below -kFar) alone: NaN (their weights on the multiply-add pipe are not quite 0)
+        const float inv = part ? 1.f : lim <= 0 ? 0.f : m < -far ? NAN : 1.f / sum;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         // a share's part goes to scratch as it is, in f32, with what its weights refer to
         const bool f32 = part || a.out_f32;
         const size_t rec0 = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile, rec = rec0 + row;
         char * const out = static_cast<char *>(part ? a.part : a.out);
         if (part && live) {
-            const float mr = m == -INFINITY ? m : m == INFINITY ? NAN : m * c - float(kShift);
+            const float mr = m < -far ? -INFINITY : m > far ? NAN : __fmaf_ru(m, c, -float(kShift));
             reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
         }
         // Rows go out by way of the query tile's memory (its products are complete), 2 D bytes of a row at a time, so that

@@ -444,9 +444,10 @@ def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_e
     [kv_rows, kv_heads, D], float16 or bfloat16; sequence s has query rows q_offsets[s] .. q_offsets[s+1]
     and key rows kv_offsets[s] .. kv_offsets[s+1] (or kv_begin[s] .. kv_end[s], for rows that lie in a
     slot cache).  Its last query sees all of its keys, the one before all but the last, and so on; a query
-    that sees none becomes zero.  out may be float32 or of q's type; query rows outside every sequence are
-    left as they were (undefined where out is allocated here).  scratch: a uint8 tensor of
-    prompt_scratch_bytes() that no other call uses at the same time; allocated per call when not given."""
+    that sees none becomes zero, one whose largest score is beyond 2^26 in size may become NaN.  out may be
+    float32 or of q's type; query rows outside every sequence are left as they were (undefined where out is
+    allocated here).  scratch: a uint8 tensor of prompt_scratch_bytes() that no other call uses at the same
+    time; allocated per call when not given."""
     index, dtype = q.get_device(), q.dtype
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError("q, k and v must be float16 or bfloat16")
