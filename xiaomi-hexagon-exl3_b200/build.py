@@ -32,7 +32,7 @@ CUDA_SOURCES = ["exl3cu_api.cu", "exl3cu_kernels.cu", "exl3cu_gemv.cu", "exl3cu_
                 "exl3cu_hybrid.cu", "exl3cu_peers.cu", "exl3cu_attn.cu", "exl3cu_attn_prompt.cu"]
 CXX_SOURCES = ["exl3_codec_host.cpp"]
 HEADERS = ["exl3cu_internal.h", "exl3cu_decode.cuh", "exl3cu_common.cuh", "exl3cu_async.cuh", "exl3cu_mul1.cuh",
-           "exl3cu_json.h", "exl3cu_attn.cuh"]
+           "exl3cu_json.h", "exl3cu_attn.cuh", "exl3cu_ring.h"]
 
 
 def nvcc() -> str:

@@ -10,6 +10,7 @@
 #include "exl3cu_attn.cuh"
 #include "exl3cu_attn.h"
 #include "exl3cu_internal.h"
+#include "exl3cu_ring.h"
 
 #include <cooperative_groups.h>
 
@@ -782,8 +783,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
     }
 
     const CodeConst kc2;
-    unsigned issued = 0, used = 0;  // tiles of this warp: copies started, waited for
-    bool ok = true;
+    CopyRing<kStages> copies;  // tiles of this warp
+    const auto arrived = [&](unsigned slot, unsigned parity) { return bool(__all_sync(0xffffffffu, mbar_wait(&full[warp][slot], parity))); };
     while (left > 0) {
         const int n = sm_n[row], tiles = tiles_of(n), t0 = min(off, tiles), t1 = min(tiles, off + left);
         left = a.split == kClusters ? 0 : left - min(left, list_of(n) - off);
@@ -792,10 +793,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         ++row;
         if (t0 >= t1) continue;
         const size_t base = (size_t(slot) * a.c.kv_heads + kvh) * a.c.max_len;
-        const auto start = [&](int tile) {
-            unsigned char * dst = ring + (issued % kStages) * Tile::kBytes;
-            uint64_t * bar = &full[warp][issued % kStages];
-            ++issued;
+        const auto start = [&](int tile, unsigned to) {
+            unsigned char * dst = ring + to * Tile::kBytes;
+            uint64_t * bar = &full[warp][to];
             if (lane == 0) {
                 const size_t key = base + size_t(tile) * kKeys;
                 mbar_arrive_expect_tx(bar, Tile::kBytes);
@@ -805,8 +805,9 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 bulk_g2s(dst + 2 * Tile::kCodes + Tile::kScales, a.c.v_scales + key * G, Tile::kScales, bar);
             }
         };
-        int next = t0 + warp;
-        for (int i = 0; i < kStages && next < t1; ++i, next += kAttnWarps) start(next);
+#pragma unroll
+        for (int i = 0; i < kStages; ++i)
+            if (t0 + warp + i * kAttnWarps < t1) start(t0 + warp + i * kAttnWarps, copies.slot(i));
 
         // q as the B operand: column g is a head (PAIR: half of one); this lane's dimensions are
         // [t D/4, +D/4), words of 8, codes i and i + 4 of a word a pair.  Scaled by 2^e to a largest element in [2^8, 2^9).
@@ -864,12 +865,11 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         // exponents of the groups' largest scales as raised, in a half's place: no more than 15 below ev
         const auto raised = [&](int i) { return __vmaxu2(evs[i], uint32_t(max(ev - 15, 0)) * 0x04000400u); };
         const auto exponent = [&](int j) { return int(raised(j / 2) >> (16 * (j & 1) + 10) & 31u); };  // of group j
-        for (int tile = t0 + warp; tile < t1; tile += kAttnWarps) {
-            const unsigned char * kc = ring + (used % kStages) * Tile::kBytes;
+        int tile = t0 + warp;
+        for (; tile < t1; tile += kAttnWarps) {
+            const unsigned char * kc = ring + copies.slot() * Tile::kBytes;
             const unsigned char * ks = kc + Tile::kCodes, * vc = ks + Tile::kScales, * vs = vc + Tile::kCodes;
-            ok = ok && __all_sync(0xffffffffu, mbar_wait(&full[warp][used % kStages], (used / kStages) & 1u));
-            ++used;
-            if (!ok) break;
+            if (!copies.next(arrived)) break;
             const int keys = n - tile * kKeys;  // visible keys of the tile, >= 1
             if (keys < kKeys) {  // what lies behind them may not be finite: scales of zero
                 uint32_t * z = reinterpret_cast<uint32_t *>(const_cast<unsigned char *>(ks));
@@ -1077,19 +1077,25 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 take(std::integral_constant<int, 3>{});
             }
             __syncwarp();  // every lane has read the tile
-            if (next < t1) {
-                start(next);
-                next += kAttnWarps;
-            }
+            if (tile + kStages * kAttnWarps < t1) start(tile + kStages * kAttnWarps, copies.slot(kStages - 1));
         }
 
-        for (; used < issued; ++used)  // after a wait that ran out: copies in flight end before their memory is used
-            (void)mbar_wait(&full[warp][used % kStages], (used / kStages) & 1u);
+        // short of the end after a wait that ran out: copies in flight end before the CTA does
+        copies.drain(min(kStages, (t1 - tile + kAttnWarps - 1) / kAttnWarps), arrived);
+        constexpr int kRec = D + 4;
+        if (!__syncthreads_and(tile >= t1)) {
+            // no result: a row that the CTA has to itself stays as it was, and in the parts that a join will look for here
+            // a maximum that is NaN makes it the result
+            if (threadIdx.x == 0) atomicOr(&g_attn_status, kStatusWaitTimeout);
+            if (a.split == kShares && threadIdx.x < (t0 ? 2 * HC : HC))  // record 1, if any, comes before record 0
+                a.part[kPlanFloats + ((size_t(blockIdx.y) * gridDim.x + blockIdx.x) * (2 * HC) + threadIdx.x) * kRec + D] = NAN;
+            if (a.split == kClusters && threadIdx.x < HC)
+                reinterpret_cast<float *>(ring_all)[(HC + threadIdx.x) * kRec + D] = NAN;
+            break;
+        }
         // the warp's part: sums over the lanes of a head, then into the warp's own ring (its copies have landed):
         // [HC][D + 4], accumulator, maximum (times cs), sum
-        constexpr int kRec = D + 4;
         float * const mine = reinterpret_cast<float *>(ring);
-        __syncwarp();
         float back[G];
 #pragma unroll
         for (int i = 0; i < G; ++i) back[i] = pow2(exponent(i) - 14 - kTop);
@@ -1109,8 +1115,8 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
                 rec[D + 1] = l[j] * pow2(ev - 14 - kTop);
             }
         }
-        __syncthreads();
         const bool whole = t0 == 0 && t1 == tiles;
+        __syncthreads();
         float * part = whole ? nullptr
                        : a.split == kClusters
                            ? reinterpret_cast<float *>(ring_all) + HC * kRec  // behind the first warp's record
@@ -1141,10 +1147,6 @@ __global__ void __launch_bounds__(kAttnThreads, kAttnCtas) k_kv4_attn(const Kv4A
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the next copies overwrite these records
         __syncthreads();
-        if (!__syncthreads_and(ok)) {
-            if (threadIdx.x == 0) atomicOr(&g_attn_status, kStatusWaitTimeout);
-            break;
-        }
     }
     if (a.split == kClusters) {  // join the parts, in order; the outputs are dealt out among the cluster's threads
         namespace cg = cooperative_groups;
