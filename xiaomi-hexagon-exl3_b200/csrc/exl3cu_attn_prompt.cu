@@ -670,8 +670,8 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const bool f32 = part || a.out_f32;
         const size_t rec0 = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile, rec = rec0 + row;
         char * const out = static_cast<char *>(part ? a.part : a.out);
-        if (part && live) {
-            const float mr = m < -far ? -INFINITY : m > far ? NAN : __fmaf_ru(m, c, -float(kShift));
+        if (part && end.work && p < end.nq) {  // NaN after a wait that ran out: the join makes it the row's result
+            const float mr = !ok || m > far ? NAN : m < -far ? -INFINITY : __fmaf_ru(m, c, -float(kShift));
             reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
         }
         // Rows go out by way of the query tile's memory (its products are complete), 2 D bytes of a row at a time, so that
