@@ -188,19 +188,22 @@ def one_row_each(row_offsets) -> bool:
 
 class StepMeta:
     """Device int32 row metadata of one step, filled from one pinned host buffer by one copy:
-    [tokens R | row_seq R | row_pos R | row_offsets n_seq+1 | seq_slot n_seq | logit_rows nout |
-    kv_offsets n_seq+1], kv_offsets the running total of the sequences' positions after the step."""
+    [tokens R | row_seq R | row_pos R | row_offsets n_seq+1 | seq_slot n_seq | logit_rows nout], and with
+    `contexts` (what caches in 4 bits are read back by) kv_offsets n_seq+1, the running total of the sequences'
+    positions after the step."""
 
-    def __init__(self, torch, device, max_rows: int, max_seq: int, max_out: int):
+    def __init__(self, torch, device, max_rows: int, max_seq: int, max_out: int, contexts: bool = False):
         self.cap = (max_rows, max_seq, max_out)
-        n = 3 * max_rows + 3 * max_seq + 2 + max_out
+        n = 3 * max_rows + 2 * max_seq + 1 + max_out + (max_seq + 1 if contexts else 0)
         self.host = torch.zeros(n, dtype=torch.int32, pin_memory=True)
         self.dev = torch.zeros(n, dtype=torch.int32, device=device)
         R, Q, O = max_rows, max_seq, max_out
         self.off = {"tokens": 0, "row_seq": R, "row_pos": 2 * R, "row_offsets": 3 * R, "seq_slot": 3 * R + Q + 1,
-                    "logit_rows": 3 * R + 2 * Q + 1, "kv_offsets": 3 * R + 2 * Q + 1 + O}
-        self.len = {"tokens": R, "row_seq": R, "row_pos": R, "row_offsets": Q + 1, "seq_slot": Q, "logit_rows": O,
-                    "kv_offsets": Q + 1}
+                    "logit_rows": 3 * R + 2 * Q + 1}
+        self.len = {"tokens": R, "row_seq": R, "row_pos": R, "row_offsets": Q + 1, "seq_slot": Q, "logit_rows": O}
+        self.contexts = contexts
+        if contexts:
+            self.off["kv_offsets"], self.len["kv_offsets"] = 3 * R + 2 * Q + 1 + O, Q + 1
         self.kv_total = 0  # positions of the filled step's sequences together
         self.one_row_each = False  # every sequence of the filled step has exactly one row (a decode step)
 
@@ -210,19 +213,24 @@ class StepMeta:
 
     def fill(self, tokens, row_seq, row_pos, row_offsets, seq_slot, logit_rows):
         h = self.host.numpy()
-        offs, pos = np.asarray(row_offsets, np.int64), np.asarray(row_pos, np.int64)
-        last = offs[1:] - 1  # each sequence's last row
-        kv = np.where(np.diff(offs) > 0, pos[np.clip(last, 0, max(pos.size - 1, 0))] + 1, 0) if pos.size else 0 * last
-        kv_offsets = np.concatenate([[0], np.cumsum(kv)])
-        self.kv_total = int(kv_offsets[-1])
         for name, arr in (("tokens", tokens), ("row_seq", row_seq), ("row_pos", row_pos),
-                          ("row_offsets", row_offsets), ("seq_slot", seq_slot), ("logit_rows", logit_rows),
-                          ("kv_offsets", kv_offsets)):
+                          ("row_offsets", row_offsets), ("seq_slot", seq_slot), ("logit_rows", logit_rows)):
             a = np.asarray(arr, np.int32)
             if a.size > self.len[name]:
                 raise ValueError(f"{name}: {a.size} entries, capacity {self.len[name]}")
             h[self.off[name]:self.off[name] + a.size] = a
         self.one_row_each = one_row_each(row_offsets)
+        if self.contexts:
+            offs, pos = np.asarray(row_offsets, np.int64), np.asarray(row_pos, np.int64)
+            if self.one_row_each and pos.size == offs.size - 1:
+                kv = pos + 1
+            elif pos.size:
+                kv = np.where(np.diff(offs) > 0, pos[np.clip(offs[1:] - 1, 0, pos.size - 1)] + 1, 0)  # by the last rows
+            else:
+                kv = np.zeros(max(offs.size - 1, 0), np.int64)
+            total, o = np.cumsum(kv), self.off["kv_offsets"]
+            h[o], h[o + 1:o + 1 + kv.size] = 0, total
+            self.kv_total = int(total[-1]) if kv.size else 0
 
     def upload(self, stream):
         self.dev.copy_(self.host, non_blocking=True)
@@ -303,7 +311,7 @@ class HybridEngine:
             else:
                 d["cache"] = gi
                 gi += 1
-        self.meta = StepMeta(torch, dev, R, slots, 8)
+        self.meta = StepMeta(torch, dev, R, slots, 8, contexts=kv_bits == 4)
         part_bytes = max(L.exl3cu_hyb_attn_scratch_bytes(r, attn_splits(r)) for r in range(1, R + 1))
         self.attn_part = torch.zeros(max(1, part_bytes // 4), dtype=f32, device=dev)
         self.attn_tickets = torch.zeros(R * cfg.heads, dtype=torch.int32, device=dev)
