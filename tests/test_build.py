@@ -1,0 +1,72 @@
+"""build.py: the Python extension module beside the C libraries."""
+import importlib.util
+from pathlib import Path
+from types import SimpleNamespace
+
+import pytest
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+@pytest.fixture
+def build(monkeypatch, tmp_path):
+    """build.py with its commands recorded instead of run, its outputs under tmp_path, and a torch for CUDA there."""
+    spec = importlib.util.spec_from_file_location("exl3_build", ROOT / "xiaomi-hexagon-exl3_b200" / "build.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    (tmp_path / "torch" / "lib").mkdir(parents=True)
+    (tmp_path / "torch" / "lib" / "libc10_cuda.so").touch()
+    (tmp_path / "torch" / "version.py").write_text("__version__ = '2.11.0+cu128'\n")
+    mod.TORCH_LIB, mod.BUILD = tmp_path / "exl3cu_torch.so", tmp_path
+    mod.commands = []
+
+    def run(cmd):
+        mod.commands.append(cmd)
+        mod.TORCH_LIB.touch()
+
+    mod._run = run
+    mod.found = SimpleNamespace(origin=str(tmp_path / "torch" / "__init__.py"))
+    monkeypatch.setattr(mod.importlib.util, "find_spec", lambda name: mod.found)
+    mod.package = tmp_path / "torch"
+    return mod
+
+
+CC = "/usr/local/cuda/bin/nvcc"
+
+
+@pytest.mark.skipif(not (Path(importlib.import_module("sysconfig").get_paths()["include"]) / "Python.h").exists(),
+                    reason="no Python headers")
+class TestTorchModule:
+    def test_is_built_once(self, build):
+        assert build.build_torch_module(CC) and len(build.commands) == 1
+        assert build.build_torch_module(CC) and len(build.commands) == 1
+        assert build.build_torch_module(CC, force=True) and len(build.commands) == 2
+
+    def test_is_left_out_without_torch(self, build, capsys):
+        build.found = None
+        assert not build.build_torch_module(CC, force=True)
+        assert "torch is not installed" in capsys.readouterr().err and not build.commands
+
+    def test_is_left_out_without_cuda(self, build, capsys):
+        (build.package / "lib" / "libc10_cuda.so").unlink()
+        assert not build.build_torch_module(CC)
+        assert "not one for CUDA" in capsys.readouterr().err and not build.commands
+
+
+def test_build_without_torch_still_makes_the_c_libraries(build, monkeypatch, tmp_path):
+    """All of build(), its commands recorded: without torch it ends with the library as ever."""
+    build.found = None
+    monkeypatch.setattr(build, "nvcc", lambda: CC)
+    monkeypatch.setattr(build, "LIB", tmp_path / "libexl3cu.so")
+    monkeypatch.setattr(build, "GGML_LIB", tmp_path / "libexl3cu_ggml.so")
+    monkeypatch.setattr(build, "_newer", lambda target, deps: True)
+
+    def run(cmd):
+        build.commands.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).touch()
+        return ""
+
+    monkeypatch.setattr(build, "_run", run)
+    assert build.build() == tmp_path / "libexl3cu.so"
+    made = {Path(c[c.index("-o") + 1]).name for c in build.commands}
+    assert {"libexl3cu.so", "libexl3cu_ggml.so"} <= made and "exl3cu_torch.so" not in made

@@ -56,6 +56,27 @@ def _run(cmd):
     return r.stdout + r.stderr
 
 
+def build_torch_module(cc: str, force: bool = False) -> bool:
+    """exl3cu_torch.so, the attention operators' calls with torch tensors (a Python extension module).  The C libraries
+    need neither torch nor Python: without a torch for CUDA or without Python's headers it is left out, with a message."""
+    src = CSRC / "exl3cu_attn_torch.cpp"
+    spec = importlib.util.find_spec("torch")
+    python = Path(sysconfig.get_paths()["include"])
+    torch = Path(spec.origin).parent if spec and spec.origin else None
+    missing = ("torch is not installed" if torch is None else
+               "the installed torch is not one for CUDA" if not (torch / "lib" / "libc10_cuda.so").exists() else
+               f"no Python headers in {python}" if not (python / "Python.h").exists() else None)
+    if missing:
+        print(f"{TORCH_LIB.name} is not built, only exl3_b200.attention needs it: {missing}", file=sys.stderr)
+        return False
+    if force or _newer(TORCH_LIB, [src, INCLUDE / "exl3cu.h", INCLUDE / "exl3cu_attn.h"]):
+        cuda = Path(cc).resolve().parents[1]
+        inc = [f"-I{p}" for p in (INCLUDE, torch / "include", cuda / "include", python)]
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *inc, str(src), "-o", str(TORCH_LIB),
+              f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+    return True
+
+
 def build(verbose_ptxas: bool = False, force: bool = False, quiet: bool = True) -> Path:
     BUILD.mkdir(exist_ok=True)
     cc = nvcc()
@@ -88,14 +109,7 @@ def build(verbose_ptxas: bool = False, force: bool = False, quiet: bool = True) 
         _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f"-I{INCLUDE}", f"-I{CSRC / 'ggml_stub'}",
               str(gsrc), "-o", str(GGML_LIB), f"-L{PKG}", "-lexl3cu",
               f"-Wl,-rpath,$ORIGIN"])
-    # the attention operators' calls with torch tensors (a Python extension module)
-    tsrc = CSRC / "exl3cu_attn_torch.cpp"
-    if force or _newer(TORCH_LIB, [tsrc, INCLUDE / "exl3cu.h", INCLUDE / "exl3cu_attn.h"]):
-        torch = Path(importlib.util.find_spec("torch").origin).parent
-        cuda = Path(cc).resolve().parents[1]
-        inc = [f"-I{p}" for p in (INCLUDE, torch / "include", cuda / "include", sysconfig.get_paths()["include"])]
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *inc, str(tsrc), "-o", str(TORCH_LIB),
-              f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+    build_torch_module(cc, force)
     if verbose_ptxas and not quiet:
         print("\n".join(logs))
     return LIB
