@@ -42,6 +42,25 @@ class TestTorchModule:
         assert build.build_torch_module(CC) and len(build.commands) == 1
         assert build.build_torch_module(CC, force=True) and len(build.commands) == 2
 
+    def test_is_built_again_for_another_torch_or_python(self, build, monkeypatch):
+        assert build.build_torch_module(CC) and "2.11.0+cu128" in " ".join(build.commands[0])
+        (build.package / "version.py").write_text("__version__ = '2.12.0+cu130'\n")
+        assert build.build_torch_module(CC) and "2.12.0+cu130" in " ".join(build.commands[1])
+        assert build.build_torch_module(CC) and len(build.commands) == 2
+        monkeypatch.setattr(build.sysconfig, "get_config_var", lambda name: "cpython-399-none")
+        assert build.build_torch_module(CC) and "cpython-399-none" in " ".join(build.commands[2])
+
+    def test_is_built_again_after_a_build_that_failed(self, build, monkeypatch):
+        def fail(cmd):
+            build.TORCH_LIB.touch()
+            raise RuntimeError
+
+        with monkeypatch.context() as m:
+            m.setattr(build, "_run", fail)
+            with pytest.raises(RuntimeError):
+                build.build_torch_module(CC)
+        assert build.build_torch_module(CC) and len(build.commands) == 1
+
     def test_is_left_out_without_torch(self, build, capsys):
         build.found = None
         assert not build.build_torch_module(CC, force=True)
@@ -70,3 +89,14 @@ def test_build_without_torch_still_makes_the_c_libraries(build, monkeypatch, tmp
     assert build.build() == tmp_path / "libexl3cu.so"
     made = {Path(c[c.index("-o") + 1]).name for c in build.commands}
     assert {"libexl3cu.so", "libexl3cu_ggml.so"} <= made and "exl3cu_torch.so" not in made
+
+
+def test_module_of_another_torch_is_refused(monkeypatch):
+    """What was built says for which torch and Python; loaded into another, an error names both."""
+    import torch
+    from exl3_b200 import attention
+
+    attention._native()  # as built
+    monkeypatch.setattr(torch, "__version__", "1.2.3")
+    with pytest.raises(ImportError, match="built for .*" + str(attention._native().built_for.split()[-1]).replace("+", "\\+") + ".*1.2.3"):
+        attention._native.__wrapped__()

@@ -56,6 +56,13 @@ def _run(cmd):
     return r.stdout + r.stderr
 
 
+def _torch_version(package: Path) -> str:
+    """torch.__version__ without importing it."""
+    scope: dict = {}
+    exec((package / "version.py").read_text(), scope)
+    return scope["__version__"]
+
+
 def build_torch_module(cc: str, force: bool = False) -> bool:
     """exl3cu_torch.so, the attention operators' calls with torch tensors (a Python extension module).  The C libraries
     need neither torch nor Python: without a torch for CUDA or without Python's headers it is left out, with a message."""
@@ -69,11 +76,17 @@ def build_torch_module(cc: str, force: bool = False) -> bool:
     if missing:
         print(f"{TORCH_LIB.name} is not built, only exl3_b200.attention needs it: {missing}", file=sys.stderr)
         return False
-    if force or _newer(TORCH_LIB, [src, INCLUDE / "exl3cu.h", INCLUDE / "exl3cu_attn.h"]):
+    # what it is compiled against: Python's ABI and the installed torch
+    built_for = f"{sysconfig.get_config_var('SOABI')} {_torch_version(torch)}"
+    stamp = BUILD / (TORCH_LIB.name + ".for")
+    same = stamp.exists() and stamp.read_text() == built_for
+    if force or not same or _newer(TORCH_LIB, [src, INCLUDE / "exl3cu.h", INCLUDE / "exl3cu_attn.h"]):
+        stamp.unlink(missing_ok=True)
         cuda = Path(cc).resolve().parents[1]
         inc = [f"-I{p}" for p in (INCLUDE, torch / "include", cuda / "include", python)]
-        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", *inc, str(src), "-o", str(TORCH_LIB),
+        _run(["g++", "-std=c++17", "-O2", "-fPIC", "-shared", f'-DEXL3CU_BUILT_FOR="{built_for}"', *inc, str(src), "-o", str(TORCH_LIB),
               f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
+        stamp.write_text(built_for)
     return True
 
 

@@ -437,5 +437,7 @@ PyMODINIT_FUNC PyInit_exl3cu_torch() {
     for (Signature * s : {&rope_sig, &append_sig, &read_sig, &attend_sig, &prompt_sig})
         for (int i = 0; i < s->count; ++i)
             if (!(s->name[i] = PyUnicode_InternFromString(s->text[i]))) return nullptr;
-    return PyModule_Create(&module);
+    PyObject * mod = PyModule_Create(&module);
+    if (mod && PyModule_AddStringConstant(mod, "built_for", EXL3CU_BUILT_FOR)) Py_CLEAR(mod);  // Python's ABI, torch's version
+    return mod;
 }

@@ -23,6 +23,7 @@ import functools
 import importlib.machinery
 import importlib.util
 import struct
+import sysconfig
 
 import numpy as np
 import torch
@@ -72,10 +73,17 @@ def _native():
     """csrc/exl3cu_attn_torch.cpp: the calls below in ordinary form (NotImplemented for any other)."""
     L = _lib()
     if not TORCH_LIB_PATH.exists():
-        raise ImportError(f"{TORCH_LIB_PATH} is not built; run xiaomi-hexagon-exl3_b200/build.py")
+        raise ImportError(f"{TORCH_LIB_PATH} is not built; run xiaomi-hexagon-exl3_b200/build.py (with a torch for CUDA)")
     loader = importlib.machinery.ExtensionFileLoader("exl3cu_torch", str(TORCH_LIB_PATH))
     mod = importlib.util.module_from_spec(importlib.util.spec_from_loader("exl3cu_torch", loader))
-    loader.exec_module(mod)
+    again = "run xiaomi-hexagon-exl3_b200/build.py"
+    here = f"{sysconfig.get_config_var('SOABI')} {torch.__version__}"
+    try:
+        loader.exec_module(mod)
+    except ImportError as e:
+        raise ImportError(f"{TORCH_LIB_PATH} does not load into {here}; {again}") from e
+    if getattr(mod, "built_for", None) != here:
+        raise ImportError(f"{TORCH_LIB_PATH} was built for {getattr(mod, 'built_for', 'another torch')}, this is {here}; {again}")
     mod.bind(*(ctypes.cast(getattr(L, "exl3cu_" + n), _P).value
                for n in ("qk_norm_rope", "kv4_append", "kv4_read", "kv4_attn_scratch_bytes", "kv4_attn",
                          "prompt_attn_scratch_bytes", "prompt_attn")))
