@@ -100,7 +100,11 @@ def _call(which, types):
         nonlocal entry
         if entry is None:
             entry = _lib().exl3cu_attn_words
-        status = entry(which, pack(*args))
+        try:
+            words = pack(*args)
+        except (struct.error, OverflowError) as e:
+            raise TypeError(f"a number is expected: {e}") from None
+        status = entry(which, words)
         if status:
             check(status)
 
@@ -148,6 +152,8 @@ def _op(call):
         first = args[0] if args else kw.get("q")
         if first is None:
             return call(*args, **kw)  # names the missing argument
+        if not hasattr(first, "get_device"):
+            raise TypeError(f"{call.__name__} takes tensors, not {type(first).__name__}")
         index = first.get_device()
         if index < 0:
             raise ValueError("operands must be on a CUDA device")
@@ -174,9 +180,23 @@ if hasattr(torch._C, "_cuda_getCurrentRawStream"):  # the same handle without a 
     _stream = torch._C._cuda_getCurrentRawStream
 
 
+def _tensor(name, t):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a tensor, not {type(t).__name__}")
+    return t
+
+
+def _count(name, t):
+    """Entries of a tensor of one dimension."""
+    if _tensor(name, t).dim() != 1:
+        raise ValueError(f"{name} must have one dimension")
+    return t.shape[0]
+
+
 def _heads(name, t, index, dtype):
     """`t` as [rows, heads, head_dim] with contiguous heads and 16-byte aligned rows: the tensor (a copy where
     that is needed, to be kept until the launch), its address and its row stride."""
+    _tensor(name, t)
     if t.dtype is not dtype or t.dim() != 3 or t.get_device() != index:
         if t.dim() != 3:
             raise ValueError(f"{name} must be [rows, heads, head_dim]")
@@ -198,7 +218,7 @@ def _heads(name, t, index, dtype):
 
 def _into(name, t, rows, heads, dim, index, dtypes):
     """A caller's output: [rows, heads, dim] with contiguous heads, never copied; its row stride."""
-    if t.shape != (rows, heads, dim) or t.get_device() != index:
+    if _tensor(name, t).shape != (rows, heads, dim) or t.get_device() != index:
         raise ValueError(f"{name} must be [{rows}, {heads}, {dim}] on the device of the other operands")
     if t.dtype not in dtypes:
         raise TypeError(f"{name} has an unsupported type {t.dtype}")
@@ -212,7 +232,7 @@ def _into(name, t, rows, heads, dim, index, dtypes):
 
 def _index(name, t, count, index):
     """Address of a contiguous int32 tensor of `count` entries."""
-    if t.dtype is not _i32 or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
+    if _tensor(name, t).dtype is not _i32 or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {count} on the device of the other operands")
     return t.data_ptr()
 
@@ -220,7 +240,7 @@ def _index(name, t, count, index):
 def _f32(name, t, count, index):
     if t is None:
         return 0
-    if t.dtype is not _f32t or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
+    if _tensor(name, t).dtype is not _f32t or t.get_device() != index or t.shape != (count,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous float32 tensor of {count} on the device of the other operands")
     return t.data_ptr()
 
@@ -265,7 +285,7 @@ def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, *
     positions: int32 [rows]; rows of a negative position are not written.  inv_freq: float32
     [rotary_dim / 2] (rope_frequencies), or None for no rotation.  q_out / k_out may be q / k
     themselves, or of another of the three types; out_dtype is the type of outputs allocated here."""
-    index, dtype = q.get_device(), q.dtype
+    index, dtype = _tensor("q", q).get_device(), q.dtype
     code = _known("q", dtype)
     q, qp, qs = _heads("q", q, index, dtype)
     rows, heads, dim = q.shape
@@ -275,7 +295,7 @@ def qk_norm_rope(q, k, positions, inv_freq=None, q_weight=None, k_weight=None, *
         kv = k.shape[1]
         if k.shape != (rows, kv, dim):
             raise ValueError("k must have q's rows and head_dim")
-    rotary = 0 if inv_freq is None else 2 * inv_freq.shape[0]
+    rotary = 0 if inv_freq is None else 2 * _count("inv_freq", inv_freq)
     if q_out is None:
         q_out = torch.empty_like(q, dtype=out_dtype, memory_format=_packed)
         qos = heads * dim
@@ -348,11 +368,11 @@ class Kv4Cache:
     def append(self, k, v, row_seq, row_pos, seq_slot) -> None:
         """Quantise rows k, v [rows, kv_heads, D] into (seq_slot[row_seq], row_pos) (exl3cu_kv4_append).
         Rows outside the cache (a position, slot or sequence out of range) are skipped."""
-        index, dtype = self._index, k.dtype
+        index, dtype = self._index, _tensor("k", k).dtype
         code = _known("k", dtype)
         k, kp, ks = _heads("k", k, index, dtype)
         v, vp, vs = _heads("v", v, index, dtype)
-        rows, n = k.shape[0], seq_slot.shape[0]
+        rows, n = k.shape[0], _count("seq_slot", seq_slot)
         if k.shape != (rows, self.kv_heads, self.head_dim) or v.shape != k.shape:
             raise ValueError(f"k and v must be [rows, {self.kv_heads}, {self.head_dim}]")
         _append_call(self._at, kp, ks, vp, vs, code, rows, _index("row_seq", row_seq, rows, index),
@@ -364,10 +384,12 @@ class Kv4Cache:
         """Positions 0 .. kv_offsets[s+1] - kv_offsets[s] of each sequence's slot as packed rows
         [total_rows, kv_heads, D] of `dtype` (exl3cu_kv4_read); returns (k, v).  Rows from kv_offsets[-1]
         on are left as they were (undefined where allocated here)."""
-        index, n = self._index, seq_slot.shape[0]
+        index, n = self._index, _count("seq_slot", seq_slot)
+        if total_rows < 0:
+            raise ValueError("total_rows must not be negative")
         if k_out is None or v_out is None:
             for t in (k_out, v_out):
-                dtype = dtype if t is None else t.dtype
+                dtype = dtype if t is None else _tensor("k_out, v_out", t).dtype
             _known("dtype", dtype)
             shape = (total_rows, self.kv_heads, self.head_dim)
             k_out = torch.empty(shape, dtype=dtype, device=self.device) if k_out is None else k_out
@@ -393,11 +415,11 @@ class Kv4Cache:
         """Attention of rows q [rows, heads, D] over positions 0 .. row_pos of their slots
         (exl3cu_kv4_attn); scale defaults to 1/sqrt(D).  scratch: a uint8 tensor of scratch_bytes() that
         no other call uses at the same time; allocated per call when not given."""
-        index, dtype = self._index, q.dtype
+        index, dtype = self._index, _tensor("q", q).dtype
         code = _known("q", dtype)
         q, qp, qs = _heads("q", q, index, dtype)
         rows, heads, dim = q.shape
-        n = seq_slot.shape[0]
+        n = _count("seq_slot", seq_slot)
         if dim != self.head_dim or heads % self.kv_heads:
             raise ValueError(f"q must be [rows, a multiple of {self.kv_heads}, {self.head_dim}]")
         if out is None:
@@ -412,7 +434,7 @@ class Kv4Cache:
                 scratch = self.k_codes.new_empty(need)
             held = need
         else:
-            held = scratch.numel() * scratch.element_size()
+            held = _tensor("scratch", scratch).numel() * scratch.element_size()
             if scratch.get_device() != index or not scratch.is_contiguous():
                 raise ValueError("scratch must be contiguous memory of the cache's device")
         _attn_call(self._at, qp, qs, code, rows, heads, _index("row_seq", row_seq, rows, index),
@@ -426,7 +448,7 @@ class Kv4Cache:
 def _kv(name, t, index, dtype, dim):
     """k or v [rows, kv_heads, D] with any row and head strides that are multiples of 16 bytes: the tensor (or
     its copy), address, row and head strides."""
-    if t.dim() != 3 or t.shape[2] != dim:
+    if _tensor(name, t).dim() != 3 or t.shape[2] != dim:
         raise ValueError(f"{name} must be [rows, kv_heads, {dim}]")
     if t.dtype is not dtype or t.get_device() != index:
         raise TypeError(f"{name} must have q's type and device")
@@ -456,7 +478,7 @@ def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_e
     float32 or of q's type; query rows outside every sequence are left as they were (undefined where out is
     allocated here).  scratch: a uint8 tensor of prompt_scratch_bytes() that no other call uses at the same
     time; allocated per call when not given."""
-    index, dtype = q.get_device(), q.dtype
+    index, dtype = _tensor("q", q).get_device(), q.dtype
     if dtype is not torch.float16 and dtype is not torch.bfloat16:
         raise TypeError("q, k and v must be float16 or bfloat16")
     q, qp, qs = _heads("q", q, index, dtype)
@@ -468,20 +490,23 @@ def prompt_attention(q, k, v, q_offsets, kv_offsets=None, *, kv_begin=None, kv_e
     if kv_offsets is not None:
         if kv_begin is not None or kv_end is not None:
             raise ValueError("give kv_offsets, or kv_begin and kv_end")
-        n = q_offsets.shape[0] - 1
+        n = _count("q_offsets", q_offsets) - 1
         begin = _index("kv_offsets", kv_offsets, n + 1, index)
         end = begin + 4
     else:
         if kv_begin is None or kv_end is None:
             raise ValueError("give kv_offsets, or kv_begin and kv_end")
-        n = kv_begin.shape[0]
+        n = _count("kv_begin", kv_begin)
         begin, end = _index("kv_begin", kv_begin, n, index), _index("kv_end", kv_end, n, index)
     if out is None:
         out, os_ = torch.empty_like(q, memory_format=_packed), heads * dim
     else:
         os_ = _into("out", out, rows, heads, dim, index, (dtype, torch.float32))
     kv_rows, kv = k.shape[0], k.shape[1]
-    held = prompt_scratch_bytes(rows, n, kv_rows, heads, kv, dim) if scratch is None else scratch.numel() * scratch.element_size()
+    if scratch is None:
+        held = prompt_scratch_bytes(rows, n, kv_rows, heads, kv, dim)
+    else:
+        held = _tensor("scratch", scratch).numel() * scratch.element_size()
     if scratch is None:
         if held:
             scratch = torch.empty(held, dtype=torch.uint8, device=q.device)
