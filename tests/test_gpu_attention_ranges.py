@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_attention import TYPES, U, close, fill, gen, half_step, ints, randn, ref_attention, ref_prompt, stored, tiny, values
+from test_gpu_attention import TYPES, U, close, fill, gen, half_step, ints, offsets, randn, ref_attention, ref_prompt, stored, tiny, values
 
 pytestmark = pytest.mark.gpu
 
@@ -198,3 +198,19 @@ def test_attend_f32_rows_keep_their_digits(A, heads, kv, dim, max_len):
             k, v = (values(*stored(a[0, h // (heads // kv)], b[0, h // (heads // kv)]))[:n] for a, b in ((c.k_codes, c.k_scales), (c.v_codes, c.v_scales)))
             want, a, w, _ = ref_attention(q[0, h:h + 1], k, v, n, 1.0)
             close(got[0, h:h + 1], want, (64 * a + 64) * U * w + half_step(torch.float32) * want.abs(), (at, h))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:])
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 1e-31, 1e-20])
+def test_smallest_scales(A, dtype, scale):
+    """All visible keys alike; rows that see nothing are zero as ever."""
+    g = gen(53)
+    q, k, v = randn(g, 200, 4, 64).to(dtype), randn(g, 3000, 1, 64).to(dtype), randn(g, 3000, 1, 64).to(dtype)
+    for lens, spans in (([200], [(0, 3000)]), ([150, 50], [(0, 10), (10, 300)])):
+        begin, end = zip(*spans)
+        got = A.prompt_attention(q, k, v, offsets(lens), kv_begin=ints(begin), kv_end=ints(end), scale=scale)
+        want, tol = ref_prompt(q, k, v, lens, spans, scale)
+        close(got, want, tol + half_step(dtype) * want.abs() + 8 * tiny(dtype))
+    cache = A.Kv4Cache(1, 1, 700, 64)
+    fill(cache, g)
+    check_groups(cache.attend(q[:3], ints([0] * 3), ints([0, 99, 650]), ints([0]), scale=scale), q[:3], cache, [0] * 3, [1, 100, 651], scale)

@@ -554,7 +554,7 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
         const int lim = view.sees(view.p0 + t * ppt + (row >> a.log_p));
         const int tile_sees = view.sees(view.p0 + t * ppt);
-        const float c = a.scale_log2, far = kFar / c;
+        const float c = a.scale_log2, far = fminf(kFar / c, 3e38f);
         float m = -INFINITY, sum = 0.f;
         const int tiles = nt[t];
         bool ok = true;
@@ -577,10 +577,10 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
             for (int x = 0; x < kTile; x += 2)
                 mx[x / 2 % 4] = max3(mx[x / 2 % 4], __uint_as_float(s[x]), __uint_as_float(s[x + 1]));
             const float top = max3(mx[0], mx[1], max3(mx[2], mx[3], mx[3]));
-            // m: what the weights refer to.  It moves with the first tile, and when the true maximum is more
-            // than 2^8 above (or a NaN, which then stays); then the sums so far are scaled down.
+            // m: what the weights refer to (or -kFar, where it is below that).  It moves with the first tile, and when the
+            // true maximum is more than 2^8 above (or a NaN, which then stays); then the sums so far are scaled down.
             if (__any_sync(0xffffffffu, !((top - m) * c <= 8.f))) {
-                const float f = top == m ? 1.f : exp2_fast((m - top) * c);
+                const float f = exp2_fast((fmaxf(m, -far) - fmaxf(top, -far)) * c);
                 m = top;
                 sum *= f;
                 if (j > 0) {  // every product up to the tile before is complete: S of this tile came after them
@@ -594,10 +594,9 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
                     }
                 }
             }
-            // A row that has seen nothing, or nothing above -kFar: all weights 0.  m c is rounded up, so that no weight
-            // overflows; the rounding takes up to 2^-16 off all of them where |m c| comes to kFar, and a half has room
-            // for that.  Above kFar, +inf included: all NaN.
-            const float mc = m < -far ? 0.f : m > far ? NAN : __fmaf_ru(m, c, -float(kShift));
+            // m c is rounded up, so that no weight overflows; the rounding takes up to 2^-16 off all of them where |m c|
+            // comes to kFar, and a half has room for that.  (+inf among the scores: all NaN, as inf - inf is.)
+            const float mc = __fmaf_ru(fmaxf(m, -far), c, -float(kShift));
             const uint64_t c2 = two(c, c), mc2 = two(-mc, -mc);
             uint64_t add[2] = {0, 0};
             // masked scores have to become 0: at a view's end the polynomial is not used
@@ -663,15 +662,15 @@ k_prompt_attn(const PromptArgs a, const __grid_constant__ CUtensorMap map_q, con
         const View end(a, bars.work);
         const int p = end.p0 + t * ppt + (row >> a.log_p);
         const bool live = end.work && ok && p < end.nq, part = end.part;
-        // scores of -inf (or below -kFar) alone: NaN (their weights on the multiply-add pipe are not quite 0)
-        const float inv = part ? 1.f : lim <= 0 ? 0.f : m < -far ? NAN : 1.f / sum;
+        // nothing from -kFar on (scores of -inf alone), or something above kFar: NaN
+        const float inv = part ? 1.f : lim <= 0 ? 0.f : m >= -far && m <= far ? 1.f / sum : NAN;
         const bool dirty = *reinterpret_cast<volatile uint32_t *>(&bars.dirty) != 0u;
         // a share's part goes to scratch as it is, in f32, with what its weights refer to
         const bool f32 = part || a.out_f32;
         const size_t rec0 = (size_t(blockIdx.x) * a.splits + blockIdx.y) * (2 * kTile) + t * kTile, rec = rec0 + row;
         char * const out = static_cast<char *>(part ? a.part : a.out);
         if (part && end.work && p < end.nq) {  // NaN after a wait that ran out: the join makes it the row's result
-            const float mr = !ok || m > far ? NAN : m < -far ? -INFINITY : __fmaf_ru(m, c, -float(kShift));
+            const float mr = !ok || !(m <= far) ? NAN : m < -far ? -INFINITY : __fmaf_ru(m, c, -float(kShift));
             reinterpret_cast<float2 *>(a.part + size_t(gridDim.x) * a.splits * (2 * kTile) * D)[rec] = make_float2(mr, sum);
         }
         // Rows go out by way of the query tile's memory (its products are complete), 2 D bytes of a row at a time, so that
