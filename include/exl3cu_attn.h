@@ -1,4 +1,4 @@
-/* Attention operators of any head geometry (libexl3cu): query/key norms with
+/* Attention operators for any number of heads (libexl3cu): query/key norms with
  * the rotary embedding, a K/V cache held in 4 bits, attention of single tokens
  * over that cache, and causal attention of packed prompts on the tensor cores.
  *
@@ -11,7 +11,9 @@
  * (patches/llama-exl3.patch:175-183 routes FLASH_ATTN_EXT).
  *
  * Types: EXL3CU_F32, EXL3CU_F16 and EXL3CU_BF16.  Sums, softmax statistics and
- * norms are held in 32 bits whatever the type.  head_dim is 64 or 128.  A row's
+ * norms are held in 32 bits whatever the type; the weights of a softmax are
+ * rounded to 16 bits where they enter a product, as said below.  head_dim is 64
+ * or 128.  A row's
  * heads are contiguous (head h of row r starts at r * stride + h * head_dim);
  * strides count elements.  Rows start on 16-byte boundaries.
  */
@@ -86,7 +88,9 @@ int exl3cu_kv4_read(const exl3cu_kv4_cache * cache, const int32_t * d_seq_slot, 
  * 65535 rows.  A row of a negative
  * position, or of a slot outside the cache, becomes zero (nothing is visible); a
  * row whose sequence is outside [0, n_seq) is left as it was.  What the cache
- * holds past the last visible position never reaches a result.  d_scratch:
+ * holds past the last visible position never reaches a result.  A weight times a
+ * value's scale is rounded to a half for rows of 16 bits (by 2^-11 of it at most),
+ * to two for f32 (2^-22).  d_scratch:
  * exl3cu_kv4_attn_scratch_bytes() bytes, 16-byte aligned, contents arbitrary; two
  * calls that may run at the same time need scratch of their own. */
 size_t exl3cu_kv4_attn_scratch_bytes(const exl3cu_kv4_cache * cache, int rows, int heads);
@@ -106,6 +110,7 @@ int exl3cu_kv4_attn(const exl3cu_kv4_cache * cache, const void * d_q, size_t q_s
  * head can address.  A key or value that a query does not see never reaches its
  * result, whatever it holds.  Packed K/V: kv_begin = offsets, kv_end = offsets + 1.
  * dtype (q, k, v): EXL3CU_F16 or EXL3CU_BF16; scale > 0; out_dtype: the same or EXL3CU_F32.
+ * Weights are rounded to q's type (by 2^-11 of each at most for f16, 2^-8 for bf16).
  * A row whose largest score (scale * q . k) is beyond 2^26 in size may become NaN.
  * Query rows outside every sequence are left as they were; q_rows is the rows
  * that d_q and d_out hold.  With d_scratch (exl3cu_prompt_attn_scratch_bytes()

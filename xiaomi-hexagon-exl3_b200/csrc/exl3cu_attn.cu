@@ -1,4 +1,4 @@
-// Attention operators of any head geometry: the query/key norm with the rotary
+// Attention operators for any number of heads of 64 or 128: the query/key norm with the rotary
 // embedding, the 4-bit K/V cache's writer and reader, and attention of single
 // rows over that cache.  (exl3cu_attn_prompt.cu: causal attention of packed
 // prompts.)  Formats and conventions: exl3cu_attn.h.
@@ -588,9 +588,9 @@ constexpr int kRowCost = 8;      // 8 rows between 1 and 32768 positions: 19.0 u
 constexpr int kPlanFloats = 2 * kSplitRows;  // scratch begins with (first share, shares) of every row
 constexpr int kMinShare = 4;     // tiles of a share: one per warp at least
 // Few rows in a cache of few positions: a cluster of CTAs takes a row and joins its parts from their shared memory, which
-// spares the second kernel: 1 row behind 767 positions 6.5 us (f32; with shares 7.9), behind 2047 6.5 (bf16; 9.3), 8 rows
-// behind 4095 11.9 (14.6).  Above 4096 positions, or with more clusters than are resident together, shares are faster:
-// 8191 positions 10.6 against 9.7, 32 rows of 767 21.2 against 13.9.
+// spares the second kernel: 1 row behind 767 positions 6.8 us (f32; with shares 8.6), behind 2047 6.5 (bf16; 9.3), 8 rows
+// behind 4095 11.7 (14.7).  Above 4096 positions, or with more clusters than are resident together, shares are faster:
+// 8191 positions 10.6 against 9.6, 32 rows of 767 20.8 against 13.8.
 constexpr int kCluster = 8;
 constexpr int kClusterTiles = 64;
 constexpr int kLazy = 6, kTop = 15 - kLazy;  // weights times value scales are up to 2^kTop, 2^15 before m moves

@@ -4,7 +4,8 @@
 // out = softmax(scale Q K^T) V per query head, one pass over the keys in tiles of 128 with a running
 // maximum and sum per query row.  4 D flops a visible (query, key) pair and head: bound by the tensor cores
 // and, at the same rate at D = 128, by the exponentials (16 a clock and SM).  16384 tokens, 16 heads of 128:
-// 854 us, 1288 TFLOP/s; 37 tokens 7.5 us.
+// 836 us, 1315 TFLOP/s, in short runs; 975 us, 1128 TFLOP/s, in long ones, which the power limit holds back; 37 tokens
+// 7.2 us.
 //
 // One CTA serves one sequence's block of query rows for a group of P heads that share a K/V head (P: the largest
 // power of two, at most 16, that divides heads / kv_heads): two tiles of 128 rows, row = position * P + head, so
@@ -61,7 +62,7 @@ constexpr int kEarly = 96;      // keys of a tile whose weights are handed to th
 constexpr int kShift = 6;
 constexpr float kFar = 134217728.f;  // 2^27: scores (times log2 e) that a weight's exponent can still tell apart
 // Tiles of keys of a share at least, where a block's keys are shared among CTAs: 512 rows behind 1000 keys 21.5 us with 4,
-// 25.3 with 6 or without sharing; behind 4000 keys 29.8, 29.6 with 6, 33.7 with 10, 61.8 without.
+// 25.3 with 6, 25.7 without sharing; behind 4000 keys 29.7, 29.6 with 6, 33.7 with 10, 62.5 without.
 constexpr int kMinSplit = 4;
 constexpr int kMaxSplits = 16;
 constexpr uint32_t kNever = 0x7fffffffu;

@@ -1,4 +1,4 @@
-"""Attention operators of any head geometry (include/exl3cu_attn.h), torch-facing.
+"""Attention operators for any number of heads (include/exl3cu_attn.h), torch-facing.
 
 One attention layer of a decoder that keeps its K/V cache in 4 bits:
 
@@ -12,7 +12,8 @@ Rows follow the ragged packer's conventions (ops.pack_ragged): row r belongs to 
 row_seq[r] at position row_pos[r]; sequence s uses cache slot seq_slot[s].  q, k and v are
 [rows, heads, head_dim] tensors (float32, float16 or bfloat16; head_dim 64 or 128) whose last two
 dimensions are contiguous or are made so; rows may be strided, e.g. the q, k and v columns of one
-packed projection.  Index tensors are contiguous int32.  Calls run on the tensors' device, on its current
+packed projection.  Sums and softmax statistics are held in 32 bits; the weights of a softmax meet the values
+rounded to q's type (prompt_attention) or to 11 bits (attend with rows of 16 bits).  Index tensors are contiguous int32.  Calls run on the tensors' device, on its current
 stream or the one given as the keyword `stream`, and can be captured in a CUDA graph.  Invalid
 arguments raise ValueError, TypeError or Exl3InvalidArgument (a ValueError).
 """

@@ -239,7 +239,10 @@ class StepMeta:
 class HybridEngine:
     """The hybrid decoder resident on one GPU: EXL3 weights, fp16 embedding/head, KV caches and
     fp32 delta-rule states for `slots` concurrent sequences of up to `max_len` positions.  kv_bits: 16 (fp16
-    caches) or 4 (4.5 bits a value, 9/32 of the memory, for contexts that fp16 has no room for)."""
+    caches) or 4 (4.5 bits a value).  With 4 the caches take 9/32 of the memory, and steps with prompt rows need
+    every slot's context of one layer in fp16 beside them: 0.42 of the fp16 caches together for 7 such layers.
+    Those steps round queries to fp16 and attend to keys and values read back as fp16; decode steps keep fp32
+    queries and the cache's own values."""
 
     def __init__(self, weights: HybridWeights, device: int = 0, slots: int = 8, max_len: int = 1536,
                  max_rows: int = 512, kv_bits: int = 16):
