@@ -562,14 +562,14 @@ k_kv4_read(const Kv4 c, const int32_t * seq_slot, const int32_t * offsets, int n
 //   (B: the score fragment, transposed by movmatrix).
 //
 // Columns: 8 heads of 16-bit rows, or, where no more than 4 share a K/V head, one head to a pair of columns, which
-// halves what a lane computes around the products; of f32 rows the pair's second column holds what the first
-// one's rounding left, 2^11 times as large so that it keeps its digits where x is small: x = hi + 2^-11 lo to 2^-22 of x
-// down to 2^-25 of the largest, and to 2^-36 of a half's unit below.  (16-bit rows: weights rounded to 2^-11 of their value, the result's own precision.)
+// halves what a lane computes around the products; of f32 rows the pair's second column holds what the first one's
+// rounding left, 2^11 times as large so that it keeps its digits where x is small: x = hi + 2^-11 lo to 2^-22 of x down to
+// 2^-23 of the largest, and to 2^-45 of the largest below.  (16-bit rows: weights rounded to 2^-11 of their value, the
+// result's own precision.)
 // Both operands are scaled by powers of two into the half's range: q by its largest element, the weights by the largest
 // value scale seen of their group, so that nothing overflows and a group of small values beside one of large ones keeps
-// its digits.  The maximum that the weights
-// refer to follows the true one when it has grown by more than 2^kLazy.  Masked keys get a score of -inf and scales of
-// zero; codes are finite whatever they are.
+// its digits.  The maximum that the weights refer to follows the true one when it has grown by more than 2^kLazy.  Masked
+// keys get a score of -inf and scales of zero; codes are finite whatever they are.
 //
 // The tiles of all rows form one list that is cut into equal shares, one per CTA, so that a batch of a long and
 // many short contexts fills the GPU evenly (a row counts kRowCost tiles more than it has: what taking up a row costs
